@@ -75,6 +75,13 @@ SIGS = {
     "pcl_allreduce_sum_f64": "ppipppiiiqQpp",
     "pcl_ssp_commit": "piiqpp",
     "pcl_ssp_wait": "piqQpip",
+    "pcl_grouped_rows": "iiipqpqqpipqqiiiip",
+    "pcl_grouped_tn": "iipqpqpipqiiip",
+    "pcl_grouped_status": "pp",
+    "pcl_mx4_quantize": "pqippqip",
+    "pcl_mx4_dequantize": "pppqiqip",
+    "pcl_mx4_rows": "pppppipqiqiiiip",
+    "pcl_mx4_status": "pp",
 }
 
 
@@ -152,6 +159,15 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed: CUDA error {rc} ({msg})")
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call(name, *args, stream)`` on ``device``, on the stream that is current there."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream_ptr())
+        return
+    with torch.cuda.device(device):
+        call(name, *args, stream_ptr())
+
+
 class DeviceWaitTimeout(RuntimeError):
     """A bounded device-side wait (SSP clock, table flag, tile flag) ran out."""
 
@@ -180,6 +196,14 @@ def check_status(status: torch.Tensor, what: str = "device status") -> None:
     """Read a status block back (synchronises its stream), clear it and raise what it holds:
     code 1 -> :class:`DeviceWaitTimeout`, code 2 -> :class:`BadDeviceId`."""
     st = status.cpu()
+    if int(st[0].item()) & 0xFFFFFFFF == 0:
+        return
+    status.zero_()
+    raise_status(st, what)
+
+
+def raise_status(st: torch.Tensor, what: str) -> None:
+    """Raise what a status block copied to the host holds (nothing for code 0)."""
     word0 = int(st[0].item())
     code = word0 & 0xFFFFFFFF
     if code == 0:
@@ -187,7 +211,6 @@ def check_status(status: torch.Tensor, what: str = "device status") -> None:
     rank = (word0 >> 32) & 0xFFFFFFFF
     where = int(st[1].item()) & 0xFFFFFFFF
     a, b = int(st[2].item()), int(st[3].item())
-    status.zero_()
     if code == 2:
         raise BadDeviceId(what, rank, where, a, b)
     raise DeviceWaitTimeout(what, rank, where, a, b)

@@ -1,0 +1,156 @@
+"""Matrices in four bits with a shared scale for every 32 values of a row, and their products (``csrc/cuda/mx4.cu``).
+
+The format is OCP's MXFP4: elements E2M1 (0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign), scales E8M0 (code c stands for 2^(c - 127), 255 for
+NaN).  A table of factors, or the matrices of trained experts, take 17/32 of a byte a value: an eighth of fp32's.
+
+* ``mx4_quantize(X)``                    ``Mx4Matrix`` of a float32, bfloat16 or float16 matrix;
+* ``mx4_dequantize(Q)``                  its values;
+* ``mx4_gemm_nt(A, B)``                  ``A @ B.T``, as ``gemm_nt``, on the tensor cores' four-bit instructions;
+* ``mx4_grouped_nt(A, B, offsets)``      the same with one matrix for each group of rows, as ``grouped_nt``.
+
+A block's scale is 2^(floor(log2 m) - 2) for its largest magnitude m (at least 2^-127), its values are divided by it and rounded to the
+nearest element, ties to the even code, what is beyond 6 to 6.  A block that holds an infinity or a NaN is NaN as a whole.
+"""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+
+from . import _lib
+from .grouped import TYPES, check_devices, check_offsets, check_out, read_status, result_type, stride_of
+
+BLOCK = 32
+
+
+class Mx4Matrix:
+    """``rows x cols`` values in four bits.
+
+    ``data [rows, 16 ceil(cols / 32)]`` (uint8): value ``2 j`` of a row in the low half of its byte ``j``, value ``2 j + 1`` in the
+    high half, zeros behind the last.  ``scales [ceil(cols / 128), rows, 4]`` (uint8): ``scales[b, r, i]`` is the code of block
+    ``4 b + i`` of row ``r`` (255, which stands for NaN, only where the row has such a block)."""
+
+    __slots__ = ("data", "scales", "cols")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, cols: int):
+        if not 1 <= cols < 1 << 30:
+            raise ValueError(f"cols must be 1 to 2^30 - 1, got {cols}")
+        for t, name in ((data, "data"), (scales, "scales")):
+            if t.dtype != torch.uint8 or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} must be contiguous uint8 that starts at a multiple of 16 bytes")
+        if data.dim() != 2 or data.shape[1] != (cols + 31) // 32 * 16:
+            raise ValueError(f"data must be [rows, {(cols + 31) // 32 * 16}] for {cols} columns, got {tuple(data.shape)}")
+        if tuple(scales.shape) != ((cols + 127) // 128, data.shape[0], 4):
+            raise ValueError(f"scales must be {((cols + 127) // 128, data.shape[0], 4)}, got {tuple(scales.shape)}")
+        if scales.device != data.device:
+            raise ValueError(f"scales must be on {data.device}, got {scales.device}")
+        if data.shape[0] >= (1 << 31) - 512:
+            raise ValueError(f"at most 2^31 - 513 rows, got {data.shape[0]}")
+        self.data, self.scales, self.cols = data, scales, cols
+
+    @property
+    def rows(self) -> int:
+        return self.data.shape[0]
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def nbytes(self) -> int:
+        return self.data.numel() + self.scales.numel()
+
+    def __repr__(self):
+        return f"Mx4Matrix({self.rows} x {self.cols}, {self.device})"
+
+
+def check_status(device=None) -> None:
+    """Raise if a grouped four-bit product on ``device`` met bounds that it had to move, or one of these products gave up on
+    a wait (synchronises the current stream)."""
+    read_status("pcl_mx4_status", device, "four-bit product")
+
+
+def mx4_quantize(X: torch.Tensor) -> Mx4Matrix:
+    """``X [rows, K]`` (float32, bfloat16, float16) in four bits; ``X [E, N, K]``, the matrices of E groups, becomes one
+    of ``E N`` rows."""
+    if X.dtype not in TYPES:
+        raise ValueError(f"X must be float32, bfloat16 or float16, got {X.dtype}")
+    if X.dim() not in (2, 3):
+        raise ValueError(f"X must have 2 or 3 dimensions, got {X.dim()}")
+    K = X.shape[-1]
+    if not 1 <= K < 1 << 30:
+        raise ValueError(f"X must have 1 to 2^30 - 1 columns, got {K}")
+    check_devices(X=X)
+    if X.dim() == 3:
+        X = X.reshape(-1, K)
+    if (K > 1 and X.stride(1) != 1) or (X.shape[0] > 1 and X.stride(0) < 0):
+        X = X.contiguous()
+    rows = X.shape[0]
+    # both parts in one allocation: the data's size is a multiple of 16 bytes
+    words = (K + 127) // 128
+    n = rows * ((K + 31) // 32) * 16
+    buf = torch.empty(n + words * rows * 4, dtype=torch.uint8, device=X.device)
+    q = Mx4Matrix(buf[:n].view(rows, -1) if rows else buf.view(0, (K + 31) // 32 * 16), buf[n:].view(words, rows, 4), K)
+    if rows:
+        _lib.call_on(X.device, "pcl_mx4_quantize", X, stride_of(X, 0, K), TYPES[X.dtype], q.data, q.scales, rows, K)
+    return q
+
+
+def mx4_dequantize(q: Mx4Matrix, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values of ``q`` as ``[rows, cols]``.  float32 and bfloat16 hold every value exactly (but for those beyond 2^127, infinite in
+    either); float16 rounds."""
+    if dtype not in TYPES:
+        raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+    check_out(out, (q.rows, q.cols), dtype)
+    check_devices(q=q, out=out)
+    if out is None:
+        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
+    if q.rows:
+        _lib.call_on(q.device, "pcl_mx4_dequantize", q.data, q.scales, out, stride_of(out, 0, q.cols), TYPES[dtype], q.rows,
+                     q.cols)
+    return out
+
+
+def _product(A, B: Mx4Matrix, offsets, out, out_dtype):
+    if not isinstance(B, Mx4Matrix):
+        raise ValueError("B must be an Mx4Matrix: quantise it once with mx4_quantize")
+    packed = isinstance(A, Mx4Matrix)
+    if not packed and (A.dim() != 2 or A.dtype not in TYPES):
+        raise ValueError(f"A must be an Mx4Matrix or a matrix of float32, bfloat16 or float16, got {A.dtype} {tuple(A.shape)}")
+    T, cols = (A.rows, A.cols) if packed else A.shape
+    if cols != B.cols:
+        raise ValueError(f"A has {cols} columns, B {B.cols}")
+    groups = 1 if offsets is None else check_offsets(offsets)
+    if B.rows == 0 or B.rows % groups:
+        raise ValueError(f"B must have the same number of rows for each of the {groups} groups, at least one, got {B.rows}")
+    N = B.rows // groups
+    dtype = result_type(out, out_dtype, torch.float32 if packed else A.dtype, tuple(TYPES))
+    check_out(out, (T, N), dtype)
+    device = check_devices(A=A, B=B, offsets=offsets, out=out)
+    fill = out is None
+    if fill:
+        out = torch.empty(T, N, dtype=dtype, device=device)
+    if T == 0:
+        return out
+    if not packed:
+        A = mx4_quantize(A)
+    _lib.call_on(device, "pcl_mx4_rows", A.data, A.scales, B.data, B.scales, offsets,
+                 int(offsets is not None and offsets.dtype == torch.int64), out, stride_of(out, 0, N), TYPES[dtype], T, groups, N,
+                 cols, int(fill))
+    return out
+
+
+def mx4_gemm_nt(A: Union[torch.Tensor, Mx4Matrix], B: Mx4Matrix, out: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``A @ B.T`` for ``A [M, K]`` and ``B [N, K]`` in four bits; an ``A`` in float32, bfloat16 or float16 is quantised here.
+    Sums are held in float32.  The result has ``out``'s type, ``out_dtype``, ``A``'s own, or float32 if A is in four bits."""
+    return _product(A, B, None, out, out_dtype)
+
+
+def mx4_grouped_nt(A: Union[torch.Tensor, Mx4Matrix], B: Mx4Matrix, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
+                   out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``Y[t] = B[e] a[t]`` for the rows ``offsets[e] <= t < offsets[e + 1]`` of ``A [T, K]``; ``B`` holds the N rows of every
+    group one after the other (``mx4_quantize`` of an ``[E, N, K]`` tensor).  Offsets and rows that no group has are
+    treated as in ``grouped_nt``."""
+    if offsets is None:
+        raise ValueError("offsets must be a CUDA tensor; a product without groups is mx4_gemm_nt")
+    return _product(A, B, offsets, out, out_dtype)

@@ -1,0 +1,362 @@
+"""Products grouped by expert and their gradients against plain products in 64 bits.
+
+Tolerance of a sum of R products of 16-bit values, each exact in fp32: every one of the at most R additions is off by no more than one
+unit in the last of 24 bits of a partial sum that is at most S = sum |a| |b|, so R 2^-23 S in all; then the rounding into the result's
+type, half a step, eps / 2 of the value.  fp16 results below 2^-14 are 2^-24 apart.  Whole numbers whose sums stay below 2^24 come
+out exactly in fp32.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, FP = torch.bfloat16, torch.float16
+
+
+def _offsets(counts, first=0, dtype=torch.int32):
+    return torch.tensor([first] + counts, device="cuda").cumsum(0).to(dtype)
+
+
+def _bounds(offsets, T):
+    out, at = [], 0
+    for v in offsets.tolist():
+        at = max(at, min(max(v, 0), T))
+        out.append(at)
+    return out
+
+
+def _ref_rows(A, W, offsets):
+    """(values, sums of magnitudes) of a[t] W[e]^T in 64 bits, zero for rows of no group; W [E, columns, reduction]."""
+    y = torch.zeros(A.shape[0], W.shape[1], dtype=torch.float64, device=A.device)
+    s = torch.zeros_like(y)
+    b = _bounds(offsets, A.shape[0])
+    for e in range(W.shape[0]):
+        a, w = A[b[e]:b[e + 1]].double(), W[e].double()
+        y[b[e]:b[e + 1]] = a @ w.T
+        s[b[e]:b[e + 1]] = a.abs() @ w.abs().T
+    return y, s
+
+
+def _ref_tn(dY, X, offsets):
+    b = _bounds(offsets, X.shape[0])
+    E = len(b) - 1
+    d = torch.zeros(E, dY.shape[1], X.shape[1], dtype=torch.float64, device=X.device)
+    s, most = torch.zeros_like(d), 0
+    for e in range(E):
+        y, x = dY[b[e]:b[e + 1]].double(), X[b[e]:b[e + 1]].double()
+        d[e], s[e] = y.T @ x, y.abs().T @ x.abs()
+        most = max(most, b[e + 1] - b[e])
+    return d, s, most
+
+
+def _near(got, ref, mags, R):
+    tol = torch.finfo(got.dtype).eps / 2 * ref.abs() + R * 2.0 ** -23 * mags * (1 + 2.0 ** -8)
+    if got.dtype == FP:
+        tol += 2.0 ** -25
+    off = (got.double() - ref).abs()
+    assert torch.all(off <= tol), f"worst {float((off - tol).max())} beyond, at {int((off - tol).argmax())} of {off.numel()}"
+
+
+def _make(T, E, N, K, dtype, seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(T, K, device="cuda", generator=g).to(dtype), torch.randn(T, N, device="cuda", generator=g).to(dtype),
+            torch.randn(E, N, K, device="cuda", generator=g).to(dtype))
+
+
+def _whole(T, E, N, K, dtype, seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    f = lambda *s: torch.randint(-4, 5, s, device="cuda", generator=g).to(dtype)  # noqa: E731
+    return f(T, K), f(T, N), f(E, N, K)
+
+
+# counts, rows behind the last group, N, K
+SHAPES = [
+    ([1], 0, 1, 1), ([1], 0, 128, 64), ([3], 0, 8, 16), ([0, 1, 0], 0, 33, 7), ([0, 0], 5, 40, 24), ([7, 0, 9], 0, 130, 65),
+    ([16, 31, 33, 1], 3, 72, 200), ([64] * 4, 0, 64, 64), ([128, 256], 0, 256, 128), ([127, 129, 255, 257], 1, 257, 129),
+    ([300, 0, 0, 1, 511], 17, 520, 264), ([1000], 0, 1001, 777), ([5] * 100, 0, 100, 100), ([0] * 63 + [70], 0, 136, 328),
+    ([2, 260, 3], 0, 128, 1032), ([1500, 40], 0, 384, 512), ([600, 17], 0, 900, 2050),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("counts,spare,N,K", SHAPES)
+def test_grouped_products_match(counts, spare, N, K, dtype):
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt, grouped_tn
+    T, E = sum(counts) + spare, len(counts)
+    X, dY, W = _make(T, E, N, K, dtype)
+    off = _offsets(counts)
+    for out_dtype in (dtype, torch.float32):
+        y = grouped_nt(X, W, off, out_dtype=out_dtype)
+        z = grouped_nn(dY, W, off, out_dtype=out_dtype)
+        d = grouped_tn(dY, X, off, out_dtype=out_dtype)
+        check_status()
+        _near(y, *_ref_rows(X, W, off), K)
+        _near(z, *_ref_rows(dY, W.transpose(1, 2), off), N)
+        ref, mags, most = _ref_tn(dY, X, off)
+        _near(d, ref, mags, most)
+        b = _bounds(off, T)
+        assert not y[b[-1]:].any() and not z[b[-1]:].any()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("counts,spare,N,K", SHAPES)
+def test_grouped_products_of_whole_numbers_are_exact(counts, spare, N, K, dtype):
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    T, E = sum(counts) + spare, len(counts)
+    X, dY, W = _whole(T, E, N, K, dtype)
+    off = _offsets(counts, dtype=torch.int64)
+    f = torch.float32
+    assert torch.equal(grouped_nt(X, W, off, out_dtype=f).double(), _ref_rows(X, W, off)[0])
+    assert torch.equal(grouped_nn(dY, W, off, out_dtype=f).double(), _ref_rows(dY, W.transpose(1, 2), off)[0])
+    assert torch.equal(grouped_tn(dY, X, off, out_dtype=f).double(), _ref_tn(dY, X, off)[0])
+
+
+@pytest.mark.parametrize("first,spare", [(0, 9), (4, 0), (37, 30)])
+def test_rows_of_no_group_stay_as_they_were(first, spare):
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt
+    counts, N, K = [20, 0, 150], 72, 40
+    T = first + sum(counts) + spare
+    X, dY, W = _whole(T, 3, N, K, BF)
+    # what rows of no group hold reaches nothing
+    X[:first], X[first + 170:], dY[:first], dY[first + 170:] = float("nan"), float("inf"), float("inf"), float("nan")
+    off = _offsets(counts, first)
+    for call, A, M in ((grouped_nt, X, W), (grouped_nn, dY, W)):
+        ref = _ref_rows(A, M if call is grouped_nt else M.transpose(1, 2), off)[0]
+        wide = torch.full((T, ref.shape[1] + 11), -7.0, device="cuda")
+        call(A, M, off, out=wide[:, 3:-8])
+        want = wide.new_full(wide.shape, -7.0).double()
+        want[first:first + 170, 3:-8] = ref[first:first + 170]
+        assert torch.equal(wide.double(), want)
+        assert torch.equal(call(A, M, off, out_dtype=torch.float32).double(), ref)
+
+
+def test_what_one_group_holds_does_not_reach_another():
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    counts, N, K = [5, 70, 3, 130, 1], 90, 200
+    T = sum(counts)
+    X, dY, W = _whole(T, 5, N, K, FP)
+    off = _offsets(counts)
+    b = off.tolist()
+    bad = [0, 2, 4]
+    X2, dY2, W2 = X.clone(), dY.clone(), W.clone()
+    for e in bad:
+        X2[b[e]:b[e + 1]], dY2[b[e]:b[e + 1]], W2[e] = float("nan"), float("inf"), float("nan")
+    y, z, d = grouped_nt(X2, W2, off), grouped_nn(dY2, W2, off), grouped_tn(dY2, X2, off)
+    ry, rz, rd = grouped_nt(X, W, off), grouped_nn(dY, W, off), grouped_tn(dY, X, off)
+    for e in (1, 3):
+        assert torch.equal(y[b[e]:b[e + 1]], ry[b[e]:b[e + 1]])
+        assert torch.equal(z[b[e]:b[e + 1]], rz[b[e]:b[e + 1]])
+        assert torch.equal(d[e], rd[e])
+    for e in bad:
+        assert not torch.isfinite(y[b[e]:b[e + 1]]).any() and not torch.isfinite(z[b[e]:b[e + 1]]).any()
+        assert not torch.isfinite(d[e]).any()
+
+
+def test_infinities_stay_in_their_place():
+    from paracel_b200.ops.grouped import grouped_nt, grouped_tn
+    X, dY, W = (t.abs() + 1 for t in _whole(200, 2, 64, 96, BF))
+    off = _offsets([90, 110])
+    X[17, 5], W[1, 3, 7] = float("inf"), float("nan")
+    y, ref = grouped_nt(X, W, off, out_dtype=torch.float32).double(), _ref_rows(X, W, off)[0]
+    assert torch.equal(torch.isnan(y), torch.isnan(ref)) and torch.equal(torch.isinf(y), torch.isinf(ref))
+    d, ref = grouped_tn(dY, X, off, out_dtype=torch.float32).double(), _ref_tn(dY, X, off)[0]
+    assert torch.equal(d, ref)
+
+
+@pytest.mark.parametrize("raw,T", [([0, 50, 20, 90], 90), ([-5, 30, 30, 200], 90), ([60, 10, 10, 10], 90),
+                                   ([0, 1 << 40, 5, -(1 << 40)], 90)])
+def test_bad_bounds_are_moved_and_reported(raw, T):
+    from paracel_b200.ops._lib import BadDeviceId
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt, grouped_tn
+    X, dY, W = _whole(T, 3, 40, 24, BF)
+    off = torch.tensor(raw, device="cuda")
+    f = torch.float32
+    for call, got in ((grouped_nt, lambda: _ref_rows(X, W, off)[0]), (grouped_nn, lambda: _ref_rows(dY, W.transpose(1, 2), off)[0])):
+        y = call(X if call is grouped_nt else dY, W, off, out_dtype=f)
+        with pytest.raises(BadDeviceId):
+            check_status()
+        assert torch.equal(y.double(), got())
+        check_status()                                  # reported once
+    d = grouped_tn(dY, X, off, out_dtype=f)
+    with pytest.raises(BadDeviceId):
+        check_status(X.device)
+    assert torch.equal(d.double(), _ref_tn(dY, X, off)[0])
+
+
+def test_strided_operands_and_results():
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    counts, N, K = [33, 100, 7], 104, 80
+    T, E = sum(counts), 3
+    off = _offsets(counts)
+    big, bigy, bigw = _whole(T, E, N, 2 * K, BF)[0], _whole(T, E, 3 * N, K, BF)[1], _whole(T, 2 * E, N + 8, K + 16, BF)[2]
+    f = torch.float32
+    variants = [
+        (big[:, :K], bigy[:, N:2 * N], bigw[::2, :N, 8:K + 8]),          # rows at multiples of 16 bytes: read where they lie
+        (big[:, 1:K + 1], bigy[:, 3:N + 3], bigw[:E, 5:N + 5, 1:K + 1]),  # copied
+        (big[:, ::2], bigy[:, ::3], bigw[:E, :K].transpose(1, 2)[:, :K, :K]),
+        (big[:1, :K].expand(T, K), bigy[:1, :N].expand(T, N), bigw[:1, :N, :K].expand(E, N, K)),
+    ]
+    for X, dY, W in variants:
+        if W.shape[1] != N:
+            dY = dY[:, :W.shape[1]]
+        assert torch.equal(grouped_nt(X, W, off, out_dtype=f).double(), _ref_rows(X, W, off)[0])
+        assert torch.equal(grouped_nn(dY, W, off, out_dtype=f).double(), _ref_rows(dY, W.transpose(1, 2), off)[0])
+        assert torch.equal(grouped_tn(dY, X, off, out_dtype=f).double(), _ref_tn(dY, X, off)[0])
+    X, dY, W = variants[0]
+    # results at every offset of a line, two and four bytes a value
+    for dtype in (BF, f):
+        for shift in (0, 1, 2, 4, 8):
+            wide = torch.full((T, N + 32), 5.0, device="cuda", dtype=dtype)
+            grouped_nt(X, W, off, out=wide[:, shift:shift + N])
+            ref = torch.full_like(wide, 5.0)
+            ref[:, shift:shift + N] = grouped_nt(X, W, off, out_dtype=dtype)
+            assert torch.equal(wide, ref)
+    flat = torch.full((E * N * K + 3,), 5.0, device="cuda", dtype=BF)
+    grouped_tn(dY, X, off, out=flat[1:-2].view(E, N, K))
+    assert torch.equal(flat[1:-2].view(E, N, K), grouped_tn(dY, X, off))
+    assert flat[0] == 5 and torch.all(flat[-2:] == 5)
+
+
+def test_gradients_match_differences():
+    """The product is linear in either operand: with whole numbers its differences are exact."""
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    counts, N, K = [20, 1, 0, 77], 48, 56
+    T, E = sum(counts), 4
+    off = _offsets(counts)
+    X, dY, W = _whole(T, E, N, K, BF)
+    hX, _, hW = _whole(T, E, N, K, BF, seed=9)
+    f = torch.float32
+    loss = lambda x, w: (grouped_nt(x, w, off, out_dtype=f).double() * dY.double()).sum()  # noqa: E731
+    dx, dw = grouped_nn(dY, W, off, out_dtype=f), grouped_tn(dY, X, off, out_dtype=f)
+    assert loss(X + hX, W) - loss(X, W) == (dx.double() * hX.double()).sum()
+    assert loss(X, W + hW) - loss(X, W) == (dw.double() * hW.double()).sum()
+
+
+def test_empty_calls():
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    X, dY, W = _whole(0, 2, 24, 16, BF)
+    off = torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert grouped_nt(X, W, off).shape == (0, 24) and grouped_nn(dY, W, off).shape == (0, 16)
+    assert torch.equal(grouped_tn(dY, X, off), torch.zeros(2, 24, 16, device="cuda", dtype=BF))
+
+
+def test_largest_group_count_and_ties_with_one_group():
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    g = torch.Generator().manual_seed(3)
+    counts = torch.randint(0, 5, (1024,), generator=g).tolist()
+    T = sum(counts)
+    X, dY, W = _whole(T, 1024, 24, 32, FP)
+    off, f = _offsets(counts), torch.float32
+    assert torch.equal(grouped_nt(X, W, off, out_dtype=f).double(), _ref_rows(X, W, off)[0])
+    assert torch.equal(grouped_nn(dY, W, off, out_dtype=f).double(), _ref_rows(dY, W.transpose(1, 2), off)[0])
+    assert torch.equal(grouped_tn(dY, X, off, out_dtype=f).double(), _ref_tn(dY, X, off)[0])
+
+
+@pytest.mark.parametrize("N,K", [(72, 1056), (1056, 72)])
+def test_operands_beyond_two_to_the_31_values(N, K):
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    T = 2_100_007
+    g = torch.Generator(device="cuda").manual_seed(4)
+    X = torch.randint(-2, 3, (T, K), device="cuda", generator=g, dtype=torch.int8).to(BF)
+    W = torch.randint(-2, 3, (3, N, K), device="cuda", generator=g).to(BF)
+    off = torch.tensor([0, 100, T - 300, T], device="cuda")
+    tail = slice(T - 300, T)
+    local = torch.tensor([0, 300], device="cuda")
+    y = grouped_nt(X, W, off)
+    assert torch.equal(y[tail].double(), _ref_rows(X[tail], W[2:], local)[0].to(BF).double())
+    z = grouped_nn(y, W, off)
+    ref, mags = _ref_rows(y[tail], W[2:].transpose(1, 2), local)
+    _near(z[tail], ref, mags, N)
+    d = grouped_tn(y, X, off, out_dtype=torch.float32)
+    ref, mags, most = _ref_tn(y[tail], X[tail], local)
+    _near(d[2:], ref, mags, most)
+
+
+def test_a_captured_step_follows_its_inputs():
+    """Forward and both gradients in one graph; bounds, rows and matrices change between replays.  A second graph and an
+    eager call run in between on another stream."""
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt, grouped_tn
+    T, E, N, K = 400, 6, 136, 96
+    X, dY, W = _whole(T, E, N, K, BF)
+    off = _offsets([100, 50, 0, 150, 60, 40])
+    f = torch.float32
+
+    def step():
+        return (grouped_nt(X, W, off, out_dtype=f), grouped_nn(dY, W, off, out_dtype=f), grouped_tn(dY, X, off, out_dtype=f))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = step()
+        graphs.append((g, got))
+    for seed, counts in ((5, [0, 0, 400, 0, 0, 0]), (6, [1, 2, 3, 4, 5, 6]), (7, [200, 0, 0, 0, 0, 200])):
+        x, y, w = _whole(T, E, N, K, BF, seed)
+        X.copy_(x), dY.copy_(y), W.copy_(w), off.copy_(_offsets(counts))
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+            eager = step()
+        torch.cuda.synchronize()
+        ref = (_ref_rows(X, W, off)[0], _ref_rows(dY, W.transpose(1, 2), off)[0], _ref_tn(dY, X, off)[0])
+        for got in (graphs[0][1], graphs[1][1], eager):
+            for a, b in zip(got, ref):
+                assert torch.equal(a.double(), b)
+    check_status()
+
+
+def test_calls_on_two_streams_at_once():
+    from paracel_b200.ops.grouped import grouped_nt, grouped_tn
+    T, E, N, K = 3000, 8, 520, 512
+    X, dY, W = _whole(T, E, N, K, BF)
+    off = _offsets([375] * 8)
+    ref, rd = _ref_rows(X, W, off)[0], _ref_tn(dY, X, off)[0]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    torch.cuda.synchronize()
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append((grouped_nt(X, W, off, out_dtype=torch.float32), grouped_tn(dY, X, off, out_dtype=torch.float32)))
+    torch.cuda.synchronize()
+    for y, d in got:
+        assert torch.equal(y.double(), ref) and torch.equal(d.double(), rd)
+
+
+def test_the_same_call_gives_the_same_bits():
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    X, dY, W = _make(2000, 5, 264, 1032, BF)
+    off = _offsets([1, 999, 0, 500, 500])
+    first = (grouped_nt(X, W, off), grouped_nn(dY, W, off), grouped_tn(dY, X, off))
+    for _ in range(3):
+        again = (grouped_nt(X, W, off), grouped_nn(dY, W, off), grouped_tn(dY, X, off))
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_training_steps_of_a_grouped_layer():
+    """Rows sorted by cluster, a matrix for each, squared error: every step is what the formulas give from the same weights."""
+    from paracel_b200.ops.grouped import check_status, grouped_nt, grouped_tn
+    T, E, N, K = 900, 4, 40, 56
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cluster = torch.randint(0, E, (T,), device="cuda", generator=g)
+    order = cluster.argsort()
+    off = torch.zeros(E + 1, dtype=torch.int64, device="cuda")
+    off[1:] = torch.bincount(cluster, minlength=E).cumsum(0)
+    X = torch.randn(T, K, device="cuda", generator=g).to(BF)[order]
+    target = torch.randn(T, N, device="cuda", generator=g)
+    W = torch.randn(E, N, K, device="cuda", generator=g) / 8
+    for _ in range(3):
+        Wh = W.to(BF)
+        y = grouped_nt(X, Wh, off, out_dtype=torch.float32)
+        _near(y, *_ref_rows(X, Wh, off), K)
+        dY = ((y - target) / T).to(BF)
+        dW = grouped_tn(dY, X, off, out_dtype=torch.float32)
+        ref, mags, most = _ref_tn(dY, X, off)
+        _near(dW, ref, mags, most)
+        W -= 0.5 * dW
+    check_status()
