@@ -1,175 +1,383 @@
-// Products with one matrix for each group of rows (16-bit storage, fp32 sums).
+// Products with one matrix for each group of rows (16-bit storage, fp32 sums), on tcgen05.mma kind::f16.
 //
-//   rows, nt   Y[t, n] = sum_k X[t, k] W[e, n, k]        t in group e
-//   rows, nn   Z[t, k] = sum_n Y[t, n] W[e, n, k]
-//   tn         D[e, n, k] = sum_{t in group e} Y[t, n] X[t, k]
+//   nt   Y[t, n] = sum_k X[t, k] W[e, n, k]        t in group e
+//   nn   Z[t, k] = sum_n Y[t, n] W[e, n, k]
+//   tn   D[e, n, k] = sum_{t in group e} Y[t, n] X[t, k]
 //
-// One 64 x 64 tile of the output per CTA, 4 x 4 of it per thread, the reduction 16 at a time through shared memory.
-#include "grouped.cuh"
+// All three are D[m, j] = sum_r P[m, r] Q[j, r] (tiles_sm100.cuh), stored at out[j, m]:
+//   nt   P = W[e] as it lies (rows along the reduction), Q = X
+//   nn   P = W[e]^T, read as it lies: its rows run along m ("mn-major" operand tiles), Q = Y
+//   tn   P = X^T, Q = Y^T, both mn-major; the reduction runs over the rows of the group
+//
+// A persistent CTA walks tiles of 128 m x up to 256 j:
+//   warp 0     loads operand stages of 64 reduction steps by TMA (128-byte swizzle)
+//   warp 1     allocates the tensor memory; one lane issues the products
+//   warps 2-9  take the accumulator out of tensor memory and store it; two accumulators alternate, so that this runs under the next tile's
+//              products
+#include "tiles_sm100.cuh"
 
 namespace {
 
 using namespace pcl_group;
+using namespace pcl_tiles;
 
 __device__ PclStatus g_status;
 
-struct RowsArgs {
-  const void* X;
-  const void* W;
+constexpr int NT = 0, NN = 1, TN = 2;
+constexpr int CG = 1;                          // CTAs that work on a tile
+constexpr int BR = 64;                         // reduction steps of a stage
+constexpr int LANES = 128;
+constexpr int P_BYTES = LANES * BR * 2;
+constexpr int Q_BYTES = MAX_COLS / CG * BR * 2;
+constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
+constexpr int STAGES = 4;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int SMALL_BOX = 32;                  // rows of Q that are loaded at a time where a chunk is not full
+
+struct Args {
   void* out;
-  long long ldx, ws_e, ws_n, ldo;
+  long long ldo;
   Offsets off;
-  int N, K, fill;
+  int mdim;            // extent of m: N (nt), K (nn, tn)
+  int jdim;            // tn: extent of j, N
+  int red;             // nt, nn: extent of the reduction
+  uint32_t type;       // operands: 0 fp16, 1 bf16
+  int fill;            // nt, nn: rows of no group become zero
 };
 
-constexpr int T = 64, KB = 16, THREADS = 256;
-
-// acc += P Q^T over one step: ps[r][m], qs[r][j]
-__device__ __forceinline__ void step(const float (*ps)[T], const float (*qs)[T], float (&acc)[4][4]) {
-  const int tm = (threadIdx.x & 15) * 4, tj = (threadIdx.x >> 4) * 4;
-#pragma unroll
-  for (int r = 0; r < KB; ++r) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(ps[r][tm + i], qs[r][tj + j], acc[i][j]);
-  }
-}
-
-template <bool NN, class TI, class TO>
-__global__ void __launch_bounds__(THREADS) rows_kernel(RowsArgs a) {
-  __shared__ int bounds[MAX_GROUPS + 1];
-  __shared__ float ps[KB][T], qs[KB][T];
-  load_bounds(a.off, bounds, &g_status);
-  __syncthreads();
-  const int cols = NN ? a.K : a.N, red = NN ? a.N : a.K;
-  TO* out = static_cast<TO*>(a.out);
-  const int across = (cols + T - 1) / T;
-  int tile = blockIdx.x / across, e = 0;
-  for (; e < a.off.groups; ++e) {
-    const int n = (bounds[e + 1] - bounds[e] + T - 1) / T;
-    if (tile < n) break;
-    tile -= n;
-  }
-  const int c0 = blockIdx.x % across * T;
-  if (e == a.off.groups) {   // rows of no group
-    if (!a.fill || tile != 0) return;
-    for (long long r = threadIdx.x; r < a.off.rows; r += THREADS)
-      if (r < bounds[0] || r >= bounds[a.off.groups])
-        for (int c = c0; c < min(c0 + T, cols); ++c) out[r * a.ldo + c] = to_out<TO>(0.f);
-    return;
-  }
-  const int t0 = bounds[e] + tile * T, t1 = bounds[e + 1];
-  const TI* X = static_cast<const TI*>(a.X);
-  const TI* W = static_cast<const TI*>(a.W) + (long long)e * a.ws_e;
-  float acc[4][4] = {};
-  for (int r0 = 0; r0 < red; r0 += KB) {
-    for (int i = threadIdx.x; i < KB * T; i += THREADS) {
-      const int r = r0 + i % KB, t = t0 + i / KB;
-      qs[i % KB][i / KB] = (r < red && t < t1) ? to_f32(X[(long long)t * a.ldx + r]) : 0.f;
-      const int wr = NN ? r0 + i / T : r, wc = NN ? c0 + i % T : c0 + i / KB;
-      const float w = (wr < red && wc < cols) ? to_f32(NN ? W[(long long)wr * a.ws_n + wc] : W[(long long)wc * a.ws_n + wr]) : 0.f;
-      if (NN) ps[i / T][i % T] = w;
-      else ps[i % KB][i / KB] = w;
-    }
-    __syncthreads();
-    step(ps, qs, acc);
-    __syncthreads();
-  }
-  const int tm = (threadIdx.x & 15) * 4, tj = (threadIdx.x >> 4) * 4;
-  for (int j = 0; j < 4; ++j)
-    for (int i = 0; i < 4; ++i)
-      if (t0 + tj + j < t1 && c0 + tm + i < cols) out[(long long)(t0 + tj + j) * a.ldo + c0 + tm + i] = to_out<TO>(acc[i][j]);
-}
-
-struct TnArgs {
-  const void* Y;
-  const void* X;
-  void* out;
-  long long ldy, ldx;
-  Offsets off;
-  int N, K;
+struct Shared {
+  uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2], tail;
+  uint32_t tmem;
+  int abort_flag;
+  Table table;
 };
 
-template <class TI, class TO>
-__global__ void __launch_bounds__(THREADS) tn_kernel(TnArgs a) {
-  __shared__ int bounds[MAX_GROUPS + 1];
-  __shared__ float ps[KB][T], qs[KB][T];
-  load_bounds(a.off, bounds, &g_status);
-  __syncthreads();
-  const int e = blockIdx.z, k0 = blockIdx.x * T, n0 = blockIdx.y * T;
-  const TI* X = static_cast<const TI*>(a.X);
-  const TI* Y = static_cast<const TI*>(a.Y);
-  float acc[4][4] = {};
-  for (int t0 = bounds[e]; t0 < bounds[e + 1]; t0 += KB) {
-    for (int i = threadIdx.x; i < KB * T; i += THREADS) {
-      const int t = t0 + i / T, c = i % T;
-      const bool in = t < bounds[e + 1];
-      ps[i / T][c] = (in && k0 + c < a.K) ? to_f32(X[(long long)t * a.ldx + k0 + c]) : 0.f;
-      qs[i / T][c] = (in && n0 + c < a.N) ? to_f32(Y[(long long)t * a.ldy + n0 + c]) : 0.f;
+constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + (int)sizeof(Shared);
+
+struct Tile {
+  int e, m0, j0, n, ncol, r0, r1;   // columns: n of them, ncol with those that the product rounds up to
+};
+
+// The tiles of a call, numbered: those that share rows of Q are neighbours.
+template <int MODE>
+struct Walk {
+  const Args& a;
+  const Table& t;
+  int mb, jparts, jsize, e;
+  long long tiles;
+
+  __device__ Walk(const Args& a_, const Table& t_) : a(a_), t(t_), e(0) {
+    mb = (a.mdim + LANES * CG - 1) / (LANES * CG);
+    jparts = jsize = 0;
+    if (MODE == TN) {
+      jparts = (a.jdim + MAX_COLS - 1) / MAX_COLS;
+      jsize = ((a.jdim + jparts - 1) / jparts + 16 * CG - 1) / (16 * CG) * (16 * CG);
+      tiles = (long long)a.off.groups * jparts * mb;
+    } else {
+      tiles = (long long)t.chunks[a.off.groups] * mb;
     }
-    __syncthreads();
-    step(ps, qs, acc);
-    __syncthreads();
   }
-  const int tm = (threadIdx.x & 15) * 4, tj = (threadIdx.x >> 4) * 4;
-  TO* out = static_cast<TO*>(a.out) + (long long)e * a.N * a.K;
-  for (int j = 0; j < 4; ++j)
-    for (int i = 0; i < 4; ++i)
-      if (n0 + tj + j < a.N && k0 + tm + i < a.K) out[(long long)(n0 + tj + j) * a.K + k0 + tm + i] = to_out<TO>(acc[i][j]);
+
+  __device__ Tile at(long long i) {   // rising i
+    Tile w;
+    const long long c = i / mb;
+    w.m0 = (int)(i - c * mb) * LANES * CG;
+    if (MODE == TN) {
+      w.e = (int)(c / jparts);
+      w.j0 = (int)(c - (long long)w.e * jparts) * jsize;
+      w.n = min(jsize, a.jdim - w.j0);
+      w.r0 = t.bounds[w.e];
+      w.r1 = t.bounds[w.e + 1];
+    } else {
+      t.find((int)c, 16 * CG, e, w.j0, w.n);
+      w.e = e;
+      w.r0 = 0;
+      w.r1 = a.red;
+    }
+    w.ncol = (w.n + 16 * CG - 1) / (16 * CG) * (16 * CG);
+    return w;
+  }
+};
+
+template <int MODE, class TO>
+__global__ void __launch_bounds__(THREADS, 1)
+product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
+               const __grid_constant__ CUtensorMap mapQ_small, Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  Shared& s = *reinterpret_cast<Shared*>(stages + STAGES * STAGE_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t me = CG == 2 ? cluster_ctarank() : 0;   // 0 leads the pair
+  volatile int* abort_flag = &s.abort_flag;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < STAGES; ++i) { mbar_init(s.full + i, MODE == TN ? CG : 1); mbar_init(s.empty + i, 1); }
+      for (int i = 0; i < 2; ++i) { mbar_init(s.tfull + i, 1); mbar_init(s.tempty + i, CG * EPI_WARPS); }
+      mbar_init(&s.tail, 1);
+      s.abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    s.table.build(a.off, MAX_COLS, &g_status);
+  }
+  if (warp == 1) tmem_alloc<CG>(&s.tmem, 2 * MAX_COLS);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  sync_cluster_or_block<CG>();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = s.tmem;
+  const int group = blockIdx.x / CG, groups = gridDim.x / CG;
+  Walk<MODE> walk(a, s.table);
+  bool ok = true;
+
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0, tail_phase = 0;
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      const Tile w = walk.at(i);
+      const int steps = (w.r1 - w.r0 + BR - 1) / BR;
+      const int mine = w.ncol / CG;
+      const int j = w.j0 + (int)me * mine;
+      const bool whole = MODE != TN && mine == MAX_COLS / CG;
+      const int boxes = MODE == TN ? (mine + 63) / 64 : whole ? 1 : (mine + SMALL_BOX - 1) / SMALL_BOX;
+      const uint32_t q_bytes = MODE == TN ? boxes * 8192u : whole ? (uint32_t)Q_BYTES : boxes * (uint32_t)(SMALL_BOX * BR * 2);
+      for (int kb = 0; kb < steps; ++kb) {
+        if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) {
+          if (lane == 0) report(&g_status, 0, 41, kb, stage);
+          abort_all<CG>(abort_flag, me ^ 1u);
+          ok = false;
+          break;
+        }
+        uint8_t* st = stages + stage * STAGE_BYTES;
+        const uint32_t sp = smem_u32(st), sq = smem_u32(st + P_BYTES);
+        const int r = w.r0 + kb * BR;
+        // the group's last rows share their stage with the next group's: they are loaded under a barrier of this
+        // CTA's own, and what follows them is cleared, in both operands (zero times infinity is not zero)
+        const bool tail = MODE == TN && r + BR > w.r1;
+        if (lane == 0) {
+          uint32_t bar = smem_u32(s.full + stage);
+          if (tail) {
+            bar = smem_u32(&s.tail);
+            mbar_expect_tx(&s.tail, P_BYTES + q_bytes);
+          } else {
+            if (CG == 2) bar = map_to_cta(bar, 0);
+            if (me == 0) mbar_expect_tx(s.full + stage, CG * (P_BYTES + q_bytes));
+            else if (MODE == TN) arrive_cluster(bar);
+          }
+          const int m = w.m0 + (int)me * LANES;
+          if (MODE == NT) {
+            tma_load_3d<CG>(sp, &mapP, bar, r, m, w.e);
+          } else {
+            for (int h = 0; h < 2; ++h) {
+              if (tail) tma_load_3d<1>(sp + h * 8192, &mapP, bar, m + 64 * h, r, 0);
+              else tma_load_3d<CG>(sp + h * 8192, &mapP, bar, m + 64 * h, r, MODE == TN ? 0 : w.e);
+            }
+          }
+          if (MODE == TN) {
+            for (int b = 0; b < boxes; ++b) {
+              if (tail) tma_load_3d<1>(sq + b * 8192, &mapQ, bar, j + 64 * b, r, 0);
+              else tma_load_3d<CG>(sq + b * 8192, &mapQ, bar, j + 64 * b, r, 0);
+            }
+          } else if (whole) {
+            tma_load_3d<CG>(sq, &mapQ, bar, r, j, 0);
+          } else {
+            for (int b = 0; b < boxes; ++b)
+              tma_load_3d<CG>(sq + b * SMALL_BOX * BR * 2, &mapQ_small, bar, r, j + b * SMALL_BOX, 0);
+          }
+        }
+        if (tail) {
+          if (!mbar_wait(&s.tail, tail_phase, abort_flag)) {
+            if (lane == 0) report(&g_status, 0, 45, kb, stage);
+            abort_all<CG>(abort_flag, me ^ 1u);
+            ok = false;
+            break;
+          }
+          tail_phase ^= 1;
+          // the products stop at the next multiple of 16 steps
+          const int left = w.r1 - r, upto = (left + 15) & ~15;
+          const int chunks = (upto - left) * 8;   // 16-byte pieces of a box
+          for (int c = lane; c < chunks * (2 + boxes); c += 32) {
+            const int b = c / chunks, q = c - b * chunks;
+            *reinterpret_cast<uint4*>(st + (b < 2 ? b * 8192 : P_BYTES + (b - 2) * 8192) + left * 128 + q * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.full + stage), 0) : smem_u32(s.full + stage));
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (!ok)
+      for (int i = 0; i < 2048; ++i) __nanosleep(1000);   // copies in flight land before the shared memory goes away
+  } else if (warp == 1) {
+    if (lane == 0 && me == 0) {
+      const uint32_t idesc0 = (1u << 4) | (a.type << 7) | (a.type << 10) | ((MODE != NT ? 1u : 0u) << 15) |
+                              ((MODE == TN ? 1u : 0u) << 16) | ((uint32_t)(LANES * CG >> 4) << 24);
+      // from one 16-step product to the next: 32 bytes along a row, or 16 rows of 128 bytes
+      constexpr uint64_t STEP_P = MODE == NT ? 2 : 128, STEP_Q = MODE == TN ? 128 : 2;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase[2] = {0, 0};
+      for (long long i = group; i < walk.tiles && ok; i += groups) {
+        const Tile w = walk.at(i);
+        const int len = w.r1 - w.r0;
+        if (len <= 0) continue;
+        const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
+        if (!mbar_wait(s.tempty + acc, acc_phase[acc] ^ 1, abort_flag)) {
+          report(&g_status, 0, 42, acc, 0);
+          abort_all<CG>(abort_flag, me ^ 1u);
+          ok = false;
+          break;
+        }
+        acc_phase[acc] ^= 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem + (uint32_t)(acc * MAX_COLS);
+        for (int r = 0; r < len; r += BR) {
+          if (!wait_full(s.full + stage, phase, abort_flag)) {
+            report(&g_status, 0, 43, r, stage);
+            abort_all<CG>(abort_flag, me ^ 1u);
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          uint8_t* st = stages + stage * STAGE_BYTES;
+          const uint64_t dp = MODE == NT ? desc_k_major(smem_u32(st)) : desc_mn_major(smem_u32(st));
+          const uint64_t dq = MODE == TN ? desc_mn_major(smem_u32(st + P_BYTES)) : desc_k_major(smem_u32(st + P_BYTES));
+#pragma unroll
+          for (int k = 0; k < BR / 16; ++k)
+            if (r + 16 * k < len) umma_f16<CG>(d, dp + k * STEP_P, dq + k * STEP_Q, idesc, (r > 0 || k > 0) ? 1u : 0u);
+          commit<CG>(CG == 2 ? map_to_cta(smem_u32(s.empty + stage), 0) : smem_u32(s.empty + stage));
+          if (CG == 2) commit<CG>(map_to_cta(smem_u32(s.empty + stage), 1));
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        commit<CG>(CG == 2 ? map_to_cta(smem_u32(s.tfull + acc), 0) : smem_u32(s.tfull + acc));
+        if (CG == 2) commit<CG>(map_to_cta(smem_u32(s.tfull + acc), 1));
+        acc ^= 1;
+      }
+    }
+  } else {
+    const int sub = warp & 3;                 // the quarter of the tensor memory's lanes that this warp can read
+    const int half = (warp - 2) >> 2;         // two warps share a quarter: 32 columns in turn
+    TO* out = static_cast<TO*>(a.out);
+    int acc = 0;
+    uint32_t acc_phase[2] = {0, 0};
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      const Tile w = walk.at(i);
+      const int m = w.m0 + (int)me * LANES + sub * 32 + lane;
+      TO* dst = out + (MODE == TN ? ((long long)w.e * a.jdim + w.j0) * a.ldo : (long long)w.j0 * a.ldo) + m;
+      if (w.r1 <= w.r0) {   // a group without rows: its matrix of sums is zero
+        if (m < a.mdim)
+          for (int j = half; j < w.n; j += 2) dst[(long long)j * a.ldo] = to_out<TO>(0.f);
+        continue;
+      }
+      if (!mbar_wait(s.tfull + acc, acc_phase[acc], abort_flag)) {
+        if (lane == 0) report(&g_status, 0, 44, acc, 0);
+        abort_all<CG>(abort_flag, me ^ 1u);
+        ok = false;
+        break;
+      }
+      acc_phase[acc] ^= 1;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * MAX_COLS);
+      for (int c = half * 32; c < w.n; c += 64) {
+        uint32_t v[32];
+        tmem_ld32_issue(t0 + (uint32_t)c, v);
+        tmem_ld_wait(v);
+        if (m < a.mdim) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < w.n) dst[(long long)(c + j) * a.ldo] = to_out<TO>(__uint_as_float(v[j]));
+        }
+        __syncwarp();
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
+      acc ^= 1;
+    }
+    if (MODE != TN && a.fill) {
+      const int first = s.table.bounds[0], last = s.table.bounds[a.off.groups];
+      const int rows = first + a.off.rows - last;
+      for (long long q = (long long)blockIdx.x * EPI_WARPS + warp - 2; q < rows; q += (long long)gridDim.x * EPI_WARPS) {
+        TO* row = out + (q < first ? q : q - first + last) * a.ldo;
+        for (int c = lane; c < a.mdim; c += 32) row[c] = to_out<TO>(0.f);
+      }
+    }
+  }
+
+  // nobody leaves while the pair still reads this CTA's shared memory or signals its barriers
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  sync_cluster_or_block<CG>();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    tmem_free<CG>(tmem, 2 * MAX_COLS);
+  }
 }
 
-template <class TI, class TO>
-int launch_rows(bool nn, const RowsArgs& a, cudaStream_t stream) {
-  const int cols = nn ? a.K : a.N;
-  const long long grid = ((a.off.rows + T - 1ll) / T + a.off.groups + 1) * ((cols + T - 1ll) / T);
-  if (grid >= (1ll << 31)) return (int)cudaErrorInvalidValue;
-  if (nn) rows_kernel<true, TI, TO><<<(unsigned)grid, THREADS, 0, stream>>>(a);
-  else rows_kernel<false, TI, TO><<<(unsigned)grid, THREADS, 0, stream>>>(a);
+template <int MODE, class TO>
+int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
+  auto kernel = product_kernel<MODE, TO>;
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+  if (e != cudaSuccess) return (int)e;
+  const long long mb = (a.mdim + LANES * CG - 1) / (LANES * CG);
+  const long long chunks = MODE == TN ? (long long)a.off.groups * ((a.jdim + MAX_COLS - 1) / MAX_COLS)
+                                      : a.off.rows / MAX_COLS + min(a.off.groups, a.off.rows);
+  const int grid = (int)min((long long)(sms / CG), chunks * mb) * CG;
+  kernel<<<grid, THREADS, SMEM_BYTES, stream>>>(p, q, qs, a);
   return pcl_last_error();
 }
 
-template <class TI, class TO>
-int launch_tn(const TnArgs& a, cudaStream_t stream) {
-  const dim3 grid((a.K + T - 1) / T, (a.N + T - 1) / T, a.off.groups);
-  tn_kernel<TI, TO><<<grid, THREADS, 0, stream>>>(a);
-  return pcl_last_error();
+template <int MODE>
+int launch_as(int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
+  if (out_type == TYPE_F32) return launch<MODE, float>(p, q, qs, a, stream);
+  if (out_type != in_type) return (int)cudaErrorInvalidValue;
+  return in_type == TYPE_BF16 ? launch<MODE, __nv_bfloat16>(p, q, qs, a, stream) : launch<MODE, __half>(p, q, qs, a, stream);
 }
 
-bool sizes_ok(long long rows, int groups, int N, int K) {
-  return rows >= 0 && rows < (1ll << 31) - 512 && groups >= 1 && groups <= MAX_GROUPS && N >= 1 && K >= 1;
+bool sizes_ok(int in_type, long long rows, int groups, int N, int K) {
+  return (in_type == TYPE_BF16 || in_type == TYPE_F16) && rows >= 0 && rows < (1ll << 31) - 512 && groups >= 1 &&
+         groups <= MAX_GROUPS && N >= 1 && N < (1 << 30) && K >= 1 && K < (1 << 30);
 }
 
 }  // namespace
 
-// mode 0: X [rows, K] -> out [rows, N]; mode 1: X [rows, N] -> out [rows, K].  W [groups, N, K] with strides (ws_e, ws_n, 1).
-// in_type 1 / 2 (bf16 / fp16), out_type the same or 0 (fp32).  fill: rows of no group become zero, else they are left.
+// mode 0: X [rows, K] -> out [rows, N]; mode 1: X [rows, N] -> out [rows, K].  W [groups, N, K] with strides (ws_e, ws_n, 1); rows of X and W
+// start at multiples of 16 bytes.  in_type 1 / 2 (bf16 / fp16), out_type the same or 0 (fp32).  fill: rows of no group
+// become zero, else they are left.
 PCL_API int pcl_grouped_rows(int mode, int in_type, int out_type, const void* X, long long ldx, const void* W,
                              long long ws_e, long long ws_n, const void* offsets, int off64, void* out,
                              long long ldo, long long rows, int groups, int N, int K, int fill,
                              cudaStream_t stream) {
-  if (!sizes_ok(rows, groups, N, K) || (mode != 0 && mode != 1)) return (int)cudaErrorInvalidValue;
+  if (!sizes_ok(in_type, rows, groups, N, K) || (mode != 0 && mode != 1)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
-  RowsArgs a{X, W, out, ldx, ws_e, ws_n, ldo, Offsets{offsets, off64, groups, (int)rows}, N, K, fill};
-  const bool nn = mode == 1;
-  if (in_type == TYPE_BF16 && out_type == TYPE_BF16) return launch_rows<__nv_bfloat16, __nv_bfloat16>(nn, a, stream);
-  if (in_type == TYPE_BF16 && out_type == TYPE_F32) return launch_rows<__nv_bfloat16, float>(nn, a, stream);
-  if (in_type == TYPE_F16 && out_type == TYPE_F16) return launch_rows<__half, __half>(nn, a, stream);
-  if (in_type == TYPE_F16 && out_type == TYPE_F32) return launch_rows<__half, float>(nn, a, stream);
-  return (int)cudaErrorInvalidValue;
+  const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const int red = mode == 0 ? K : N;
+  CUtensorMap p, q, qs;
+  int rc = make_map_3d(&p, t, W, K, N, groups, ws_n * 2, ws_e * 2, 64, mode == 0 ? LANES : BR);
+  if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, MAX_COLS / CG);
+  if (rc == 0) rc = make_map_3d(&qs, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SMALL_BOX);
+  if (rc) return rc;
+  Args a{out, ldo, Offsets{offsets, off64, groups, (int)rows}, mode == 0 ? N : K, 0, red, in_type == TYPE_BF16 ? 1u : 0u, fill};
+  return mode == 0 ? launch_as<NT>(in_type, out_type, p, q, qs, a, stream) : launch_as<NN>(in_type, out_type, p, q, qs, a, stream);
 }
 
 // out [groups, N, K] (contiguous): every matrix is written, zeros where a group has no row
 PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long ldy, const void* X, long long ldx,
                            const void* offsets, int off64, void* out, long long rows, int groups, int N, int K,
                            cudaStream_t stream) {
-  if (!sizes_ok(rows, groups, N, K)) return (int)cudaErrorInvalidValue;
-  TnArgs a{Y, X, out, ldy, ldx, Offsets{offsets, off64, groups, (int)rows}, N, K};
-  if (in_type == TYPE_BF16 && out_type == TYPE_BF16) return launch_tn<__nv_bfloat16, __nv_bfloat16>(a, stream);
-  if (in_type == TYPE_BF16 && out_type == TYPE_F32) return launch_tn<__nv_bfloat16, float>(a, stream);
-  if (in_type == TYPE_F16 && out_type == TYPE_F16) return launch_tn<__half, __half>(a, stream);
-  if (in_type == TYPE_F16 && out_type == TYPE_F32) return launch_tn<__half, float>(a, stream);
-  return (int)cudaErrorInvalidValue;
+  if (!sizes_ok(in_type, rows, groups, N, K) || rows == 0) return (int)cudaErrorInvalidValue;
+  const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap p, q;
+  int rc = make_map_3d(&p, t, X, K, rows, 1, ldx * 2, ldx * 2, 64, BR);
+  if (rc == 0) rc = make_map_3d(&q, t, Y, N, rows, 1, ldy * 2, ldy * 2, 64, BR);
+  if (rc) return rc;
+  Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0};
+  return launch_as<TN>(in_type, out_type, p, q, q, a, stream);
 }
 
 // Copies the status block of the grouped products to `host` and clears it (waits for the stream).

@@ -1,0 +1,177 @@
+// Building blocks of the tcgen05 products over groups of rows: the table that turns a tile's number into its group and rows,
+// and the forms of loads, products and commits for one CTA (CG 1) and for a pair (CG 2).
+//
+// Every product here is D[m, j] = sum_r P[m, r] Q[j, r]: the 128 lanes of a CTA's tensor memory are rows m of P, the accumulator's
+// columns rows j of Q.  The matrices of the groups are P and the rows that share them Q, so that a ragged
+// group costs its rows rounded up to 16 columns instead of to 128 lanes, and neighbouring lanes store
+// neighbouring values of a row of the result.
+#pragma once
+#include "gemm_sm100.cuh"
+#include "grouped.cuh"
+
+namespace pcl_tiles {
+
+using namespace pcl_sm100;
+
+constexpr int MAX_COLS = 256;   // columns of an accumulator
+
+// The rows of a group are cut into chunks of at most MAX_COLS, as equal as multiples of `step` allow.
+struct Table {
+  int bounds[pcl_group::MAX_GROUPS + 1];
+  int chunks[pcl_group::MAX_GROUPS + 1];   // chunks of the groups before
+
+  // by the first warp
+  __device__ __forceinline__ void build(const pcl_group::Offsets& o, int most, PclStatus* st) {
+    pcl_group::load_bounds(o, bounds, st);
+    if (threadIdx.x >= 32) return;
+    __syncwarp();
+    int carry = 0;
+    for (int i0 = 0; i0 < o.groups; i0 += 32) {
+      const int i = i0 + (int)threadIdx.x;
+      const int own = i < o.groups ? (bounds[i + 1] - bounds[i] + most - 1) / most : 0;
+      int v = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, d);
+        if ((int)threadIdx.x >= d) v += u;
+      }
+      if (i < o.groups) chunks[i] = carry + v - own;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (threadIdx.x == 0) chunks[o.groups] = carry;
+  }
+
+  // rows [begin, begin + n) of chunk `c`, in group `e` (which only grows: callers ask for rising chunks)
+  __device__ __forceinline__ void find(int c, int step, int& e, int& begin, int& n) const {
+    while (c >= chunks[e + 1]) ++e;
+    const int rows = bounds[e + 1] - bounds[e], parts = chunks[e + 1] - chunks[e];
+    const int size = ((rows + parts - 1) / parts + step - 1) / step * step;
+    begin = bounds[e] + (c - chunks[e]) * size;
+    n = min(size, bounds[e + 1] - begin);   // at least 1: size <= most, and parts - 1 chunks of `most` do not hold all rows
+  }
+};
+
+// as mbar_wait, for a barrier that the other CTA of a pair arrives on
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const uint32_t addr = smem_u32(bar);
+  unsigned long long t0 = 0;
+  for (unsigned it = 0;; ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((it & 31) == 31) {
+      if (*abort_flag) return false;
+      const unsigned long long now = pcl_globaltimer();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > WAIT_NS) return false;
+    }
+  }
+}
+
+// arrive on a barrier given by its cluster address, after this CTA's writes to its shared memory
+__device__ __forceinline__ void arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// raise the abort flag, of both CTAs of a pair
+template <int CG>
+__device__ __forceinline__ void abort_all(volatile int* abort_flag, uint32_t peer) {
+  *abort_flag = 1;
+  if (CG == 2)
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_cta(smem_u32((const void*)abort_flag), peer)), "r"(1) : "memory");
+}
+
+// box of a three-dimensional map into this CTA's shared memory; the bytes count on `bar` (of the pair's leader for CG 2)
+template <int CG>
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  if (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t cluster_addr) {
+  if (CG == 2) umma_commit_pair(cluster_addr);
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  if (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, int cols) {
+  if (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t base, int cols) {
+  if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
+}
+
+template <int CG>
+__device__ __forceinline__ void sync_cluster_or_block() {
+  __syncthreads();
+  if (CG == 2) {
+    __syncwarp();
+    cluster_sync_all();
+  }
+}
+
+// Operand tile whose rows are contiguous along the reduction: 128-byte rows, eight of them swizzled together, groups of eight 1 KB apart.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t saddr) { return make_desc_sw128(saddr); }
+
+// Operand tile whose rows are contiguous along m (or j): boxes of 64 values x 64 steps of the reduction (8 KB) side by side, groups of eight
+// steps 1 KB apart.
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t saddr) {
+  const uint32_t lo = ((saddr >> 4) & 0x3FFFu) | (512u << 16);
+  const uint32_t hi = 64u | (1u << 14) | (2u << 29);
+  return ((uint64_t)hi << 32) | lo;
+}
+
+// map of `depth` matrices [rows x inner]; strides in bytes; box: box_in values x box_rows rows of one matrix.  `inner` and box_in count elements of `type`.
+static inline int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, long long inner, long long rows, long long depth,
+                              long long row_bytes, long long mat_bytes, int box_in, int box_rows) {
+  encode_fn_t enc = get_encode2();
+  if (enc == nullptr) return (int)cudaErrorNotSupported;
+  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)depth};
+  cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)mat_bytes};
+  cuuint32_t box[3] = {(cuuint32_t)box_in, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+}  // namespace pcl_tiles
