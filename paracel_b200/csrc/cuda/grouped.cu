@@ -24,15 +24,23 @@ using namespace pcl_tiles;
 __device__ PclStatus g_status;
 
 constexpr int NT = 0, NN = 1, TN = 2;
-constexpr int CG = 1;                          // CTAs that work on a tile
 constexpr int BR = 64;                         // reduction steps of a stage
 constexpr int LANES = 128;
 constexpr int P_BYTES = LANES * BR * 2;
-constexpr int Q_BYTES = MAX_COLS / CG * BR * 2;
-constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
-constexpr int STAGES = 4;
+constexpr int OPERAND_BYTES = 192 * 1024;
+constexpr int MAX_STAGES = 6;
 constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int FIX_WARP = 2 + EPI_WARPS;
+// tn has a warp more: it clears what a group's last stage holds of the next group
+constexpr int threads_of(int mode) { return 64 + 32 * EPI_WARPS + (mode == 2 ? 32 : 0); }
+// CG: CTAs that work on a tile, one or a pair on neighbouring SMs (tcgen05 cta_group::2); each of a pair holds its 128 m and half the j
+template <int CG>
+struct Form {
+  static constexpr int Q_BYTES = MAX_COLS / CG * BR * 2;
+  static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
+  static constexpr int STAGES = OPERAND_BYTES / STAGE_BYTES;
+  static constexpr int M = LANES * CG;   // m of a tile
+};
 constexpr int SMALL_BOX = 32;                  // rows of Q that are loaded at a time where a chunk is not full
 
 struct Args {
@@ -47,20 +55,20 @@ struct Args {
 };
 
 struct Shared {
-  uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2], tail;
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tail[MAX_STAGES], tfull[2], tempty[2];
   uint32_t tmem;
   int abort_flag;
   Table table;
 };
 
-constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + (int)sizeof(Shared);
+constexpr int SMEM_BYTES = 1024 + OPERAND_BYTES + (int)sizeof(Shared);
 
 struct Tile {
   int e, m0, j0, n, ncol, r0, r1;   // columns: n of them, ncol with those that the product rounds up to
 };
 
 // The tiles of a call, numbered: those that share rows of Q are neighbours.
-template <int MODE>
+template <int MODE, int CG>
 struct Walk {
   const Args& a;
   const Table& t;
@@ -68,7 +76,7 @@ struct Walk {
   long long tiles;
 
   __device__ Walk(const Args& a_, const Table& t_) : a(a_), t(t_), e(0) {
-    mb = (a.mdim + LANES * CG - 1) / (LANES * CG);
+    mb = (a.mdim + Form<CG>::M - 1) / Form<CG>::M;
     jparts = jsize = 0;
     if (MODE == TN) {
       jparts = (a.jdim + MAX_COLS - 1) / MAX_COLS;
@@ -82,7 +90,7 @@ struct Walk {
   __device__ Tile at(long long i) {   // rising i
     Tile w;
     const long long c = i / mb;
-    w.m0 = (int)(i - c * mb) * LANES * CG;
+    w.m0 = (int)(i - c * mb) * Form<CG>::M;
     if (MODE == TN) {
       w.e = (int)(c / jparts);
       w.j0 = (int)(c - (long long)w.e * jparts) * jsize;
@@ -100,22 +108,23 @@ struct Walk {
   }
 };
 
-template <int MODE, class TO>
-__global__ void __launch_bounds__(THREADS, 1)
+template <int MODE, int CG, class TO>
+__global__ void __launch_bounds__(threads_of(MODE), 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                const __grid_constant__ CUtensorMap mapQ_small, Args a) {
+  using F = Form<CG>;
+  constexpr int Q_BYTES = F::Q_BYTES, STAGE_BYTES = F::STAGE_BYTES, STAGES = F::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  Shared& s = *reinterpret_cast<Shared*>(stages + STAGES * STAGE_BYTES);
+  Shared& s = *reinterpret_cast<Shared*>(stages + OPERAND_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t me = CG == 2 ? cluster_ctarank() : 0;   // 0 leads the pair
   volatile int* abort_flag = &s.abort_flag;
 
   if (warp == 0) {
     if (lane == 0) {
-      for (int i = 0; i < STAGES; ++i) { mbar_init(s.full + i, MODE == TN ? CG : 1); mbar_init(s.empty + i, 1); }
+      for (int i = 0; i < STAGES; ++i) { mbar_init(s.full + i, MODE == TN ? CG : 1); mbar_init(s.empty + i, 1); mbar_init(s.tail + i, 1); }
       for (int i = 0; i < 2; ++i) { mbar_init(s.tfull + i, 1); mbar_init(s.tempty + i, CG * EPI_WARPS); }
-      mbar_init(&s.tail, 1);
       s.abort_flag = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -127,12 +136,12 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s.tmem;
   const int group = blockIdx.x / CG, groups = gridDim.x / CG;
-  Walk<MODE> walk(a, s.table);
+  Walk<MODE, CG> walk(a, s.table);
   bool ok = true;
 
   if (warp == 0) {
     int stage = 0;
-    uint32_t phase = 0, tail_phase = 0;
+    uint32_t phase = 0;
     for (long long i = group; i < walk.tiles && ok; i += groups) {
       const Tile w = walk.at(i);
       const int steps = (w.r1 - w.r0 + BR - 1) / BR;
@@ -151,26 +160,27 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         uint8_t* st = stages + stage * STAGE_BYTES;
         const uint32_t sp = smem_u32(st), sq = smem_u32(st + P_BYTES);
         const int r = w.r0 + kb * BR;
-        // the group's last rows share their stage with the next group's: they are loaded under a barrier of this
-        // CTA's own, and what follows them is cleared, in both operands (zero times infinity is not zero)
+        // the group's last rows share their stage with the next group's: they are loaded under a barrier of this CTA's own, and the
+        // warp that waits for it clears what follows them, in both operands (zero times infinity is not zero)
         const bool tail = MODE == TN && r + BR > w.r1;
-        if (lane == 0) {
-          uint32_t bar = smem_u32(s.full + stage);
+        if (elect()) {
+          uint32_t bar = smem_u32((tail ? s.tail : s.full) + stage);
+          const uint32_t bytes = P_BYTES + q_bytes;
           if (tail) {
-            bar = smem_u32(&s.tail);
-            mbar_expect_tx(&s.tail, P_BYTES + q_bytes);
+            mbar_expect_tx(s.tail + stage, bytes);
           } else {
+            if (me == 0) mbar_expect_tx(s.full + stage, CG * bytes);
             if (CG == 2) bar = map_to_cta(bar, 0);
-            if (me == 0) mbar_expect_tx(s.full + stage, CG * (P_BYTES + q_bytes));
-            else if (MODE == TN) arrive_cluster(bar);
+            if (MODE == TN && me != 0) mbar_arrive_cluster(bar);
           }
           const int m = w.m0 + (int)me * LANES;
           if (MODE == NT) {
             tma_load_3d<CG>(sp, &mapP, bar, r, m, w.e);
           } else {
-            for (int h = 0; h < 2; ++h) {
-              if (tail) tma_load_3d<1>(sp + h * 8192, &mapP, bar, m + 64 * h, r, 0);
-              else tma_load_3d<CG>(sp + h * 8192, &mapP, bar, m + 64 * h, r, MODE == TN ? 0 : w.e);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              if (tail) tma_load_3d<1>(sp + b * 8192, &mapP, bar, m + 64 * b, r, 0);
+              else tma_load_3d<CG>(sp + b * 8192, &mapP, bar, m + 64 * b, r, MODE == TN ? 0 : w.e);
             }
           }
           if (MODE == TN) {
@@ -185,25 +195,6 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
               tma_load_3d<CG>(sq + b * SMALL_BOX * BR * 2, &mapQ_small, bar, r, j + b * SMALL_BOX, 0);
           }
         }
-        if (tail) {
-          if (!mbar_wait(&s.tail, tail_phase, abort_flag)) {
-            if (lane == 0) report(&g_status, 0, 45, kb, stage);
-            abort_all<CG>(abort_flag, me ^ 1u);
-            ok = false;
-            break;
-          }
-          tail_phase ^= 1;
-          // the products stop at the next multiple of 16 steps
-          const int left = w.r1 - r, upto = (left + 15) & ~15;
-          const int chunks = (upto - left) * 8;   // 16-byte pieces of a box
-          for (int c = lane; c < chunks * (2 + boxes); c += 32) {
-            const int b = c / chunks, q = c - b * chunks;
-            *reinterpret_cast<uint4*>(st + (b < 2 ? b * 8192 : P_BYTES + (b - 2) * 8192) + left * 128 + q * 16) = make_uint4(0, 0, 0, 0);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.full + stage), 0) : smem_u32(s.full + stage));
-        }
         __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
@@ -211,50 +202,80 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     if (!ok)
       for (int i = 0; i < 2048; ++i) __nanosleep(1000);   // copies in flight land before the shared memory goes away
   } else if (warp == 1) {
-    if (lane == 0 && me == 0) {
+    if (me == 0) {
       const uint32_t idesc0 = (1u << 4) | (a.type << 7) | (a.type << 10) | ((MODE != NT ? 1u : 0u) << 15) |
                               ((MODE == TN ? 1u : 0u) << 16) | ((uint32_t)(LANES * CG >> 4) << 24);
       // from one 16-step product to the next: 32 bytes along a row, or 16 rows of 128 bytes
       constexpr uint64_t STEP_P = MODE == NT ? 2 : 128, STEP_Q = MODE == TN ? 128 : 2;
+      const uint64_t dp0 = MODE == NT ? desc_k_major(smem_u32(stages)) : desc_mn_major(smem_u32(stages));
+      const uint64_t dq0 = MODE == TN ? desc_mn_major(smem_u32(stages + P_BYTES)) : desc_k_major(smem_u32(stages + P_BYTES));
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase[2] = {0, 0};
       for (long long i = group; i < walk.tiles && ok; i += groups) {
         const Tile w = walk.at(i);
-        const int len = w.r1 - w.r0;
+        const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
         if (len <= 0) continue;
-        const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
         if (!mbar_wait(s.tempty + acc, acc_phase[acc] ^ 1, abort_flag)) {
-          report(&g_status, 0, 42, acc, 0);
+          if (lane == 0) report(&g_status, 0, 42, acc, 0);
           abort_all<CG>(abort_flag, me ^ 1u);
           ok = false;
           break;
         }
         acc_phase[acc] ^= 1;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
         const uint32_t d = tmem + (uint32_t)(acc * MAX_COLS);
-        for (int r = 0; r < len; r += BR) {
+        for (int r = 0; r < steps; ++r) {
           if (!wait_full(s.full + stage, phase, abort_flag)) {
-            report(&g_status, 0, 43, r, stage);
+            if (lane == 0) report(&g_status, 0, 43, r, stage);
             abort_all<CG>(abort_flag, me ^ 1u);
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          uint8_t* st = stages + stage * STAGE_BYTES;
-          const uint64_t dp = MODE == NT ? desc_k_major(smem_u32(st)) : desc_mn_major(smem_u32(st));
-          const uint64_t dq = MODE == TN ? desc_mn_major(smem_u32(st + P_BYTES)) : desc_k_major(smem_u32(st + P_BYTES));
+          if (elect()) {
+            const uint64_t dp = dp0 + (uint32_t)(stage * STAGE_BYTES) / 16, dq = dq0 + (uint32_t)(stage * STAGE_BYTES) / 16;
+            if (r * BR + BR <= len) {
 #pragma unroll
-          for (int k = 0; k < BR / 16; ++k)
-            if (r + 16 * k < len) umma_f16<CG>(d, dp + k * STEP_P, dq + k * STEP_Q, idesc, (r > 0 || k > 0) ? 1u : 0u);
-          commit<CG>(CG == 2 ? map_to_cta(smem_u32(s.empty + stage), 0) : smem_u32(s.empty + stage));
-          if (CG == 2) commit<CG>(map_to_cta(smem_u32(s.empty + stage), 1));
+              for (int k = 0; k < BR / 16; ++k) umma_f16<CG>(d, dp + k * STEP_P, dq + k * STEP_Q, idesc, (r > 0 || k > 0) ? 1u : 0u);
+            } else {
+              for (int k = 0; r * BR + 16 * k < len; ++k) umma_f16<CG>(d, dp + k * STEP_P, dq + k * STEP_Q, idesc, (r > 0 || k > 0) ? 1u : 0u);
+            }
+            commit<CG>(smem_u32(s.empty + stage));
+            if (r + 1 == steps) commit<CG>(smem_u32(s.tfull + acc));
+          }
+          __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
-        if (!ok) break;
-        commit<CG>(CG == 2 ? map_to_cta(smem_u32(s.tfull + acc), 0) : smem_u32(s.tfull + acc));
-        if (CG == 2) commit<CG>(map_to_cta(smem_u32(s.tfull + acc), 1));
         acc ^= 1;
       }
+    }
+  } else if (MODE == TN && warp == FIX_WARP) {
+    int stage = 0;
+    uint32_t phases = 0;   // bit i: parity of the next wait on tail[i]
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      const Tile w = walk.at(i);
+      const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
+      const int last = (stage + steps + STAGES - 1) % STAGES;
+      stage = (stage + steps) % STAGES;
+      if (len % BR == 0) continue;
+      if (!mbar_wait(s.tail + last, (phases >> last) & 1u, abort_flag)) {
+        if (lane == 0) report(&g_status, 0, 45, last, 0);
+        abort_all<CG>(abort_flag, me ^ 1u);
+        ok = false;
+        break;
+      }
+      phases ^= 1u << last;
+      // the products stop at the next multiple of 16 steps
+      uint8_t* st = stages + last * STAGE_BYTES;
+      const int left = len % BR, upto = (left + 15) & ~15;
+      const int boxes = 2 + (w.ncol / CG + 63) / 64, pieces = (upto - left) * 8;   // 16-byte pieces of a box
+      for (int b = 0; b < boxes; ++b)                                                 // Q's boxes lie behind P's
+        for (int q = lane; q < pieces; q += 32)
+          *reinterpret_cast<uint4*>(st + b * 8192 + left * 128 + q * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.full + last), 0) : smem_u32(s.full + last));
     }
   } else {
     const int sub = warp & 3;                 // the quarter of the tensor memory's lanes that this warp can read
@@ -293,7 +314,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
+      if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
       acc ^= 1;
     }
     if (MODE != TN && a.fill) {
@@ -316,28 +337,43 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   }
 }
 
-template <int MODE, class TO>
+template <int MODE, int CG, class TO>
 int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
-  auto kernel = product_kernel<MODE, TO>;
+  auto kernel = product_kernel<MODE, CG, TO>;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) return (int)e;
-  const long long mb = (a.mdim + LANES * CG - 1) / (LANES * CG);
+  const long long mb = (a.mdim + Form<CG>::M - 1) / Form<CG>::M;
   const long long chunks = MODE == TN ? (long long)a.off.groups * ((a.jdim + MAX_COLS - 1) / MAX_COLS)
                                       : a.off.rows / MAX_COLS + min(a.off.groups, a.off.rows);
-  const int grid = (int)min((long long)(sms / CG), chunks * mb) * CG;
-  kernel<<<grid, THREADS, SMEM_BYTES, stream>>>(p, q, qs, a);
-  return pcl_last_error();
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)min((long long)(sms / CG), chunks * mb) * CG);
+  cfg.blockDim = dim3(threads_of(MODE));
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, a);
+  return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 
-template <int MODE>
+template <int MODE, int CG>
 int launch_as(int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
-  if (out_type == TYPE_F32) return launch<MODE, float>(p, q, qs, a, stream);
+  if (out_type == TYPE_F32) return launch<MODE, CG, float>(p, q, qs, a, stream);
   if (out_type != in_type) return (int)cudaErrorInvalidValue;
-  return in_type == TYPE_BF16 ? launch<MODE, __nv_bfloat16>(p, q, qs, a, stream) : launch<MODE, __half>(p, q, qs, a, stream);
+  return in_type == TYPE_BF16 ? launch<MODE, CG, __nv_bfloat16>(p, q, qs, a, stream) : launch<MODE, CG, __half>(p, q, qs, a, stream);
 }
+
+// Whether pairs of CTAs take the tiles.  A pair loads a third fewer bytes for its 256 x 256 tile than two CTAs for theirs, but there are half as
+// many tiles: below two for every SM single CTAs spread better.
+bool use_pairs(long long chunks, int mdim) { return chunks * ((mdim + LANES - 1) / LANES) >= 2 * 148; }
 
 bool sizes_ok(int in_type, long long rows, int groups, int N, int K) {
   return (in_type == TYPE_BF16 || in_type == TYPE_F16) && rows >= 0 && rows < (1ll << 31) - 512 && groups >= 1 &&
@@ -357,13 +393,15 @@ PCL_API int pcl_grouped_rows(int mode, int in_type, int out_type, const void* X,
   if (rows == 0) return 0;
   const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int red = mode == 0 ? K : N;
+  const bool pair = use_pairs(rows / MAX_COLS + min((long long)groups, rows) / 2, mode == 0 ? N : K);
   CUtensorMap p, q, qs;
   int rc = make_map_3d(&p, t, W, K, N, groups, ws_n * 2, ws_e * 2, 64, mode == 0 ? LANES : BR);
-  if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, MAX_COLS / CG);
+  if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, pair ? MAX_COLS / 2 : MAX_COLS);
   if (rc == 0) rc = make_map_3d(&qs, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SMALL_BOX);
   if (rc) return rc;
   Args a{out, ldo, Offsets{offsets, off64, groups, (int)rows}, mode == 0 ? N : K, 0, red, in_type == TYPE_BF16 ? 1u : 0u, fill};
-  return mode == 0 ? launch_as<NT>(in_type, out_type, p, q, qs, a, stream) : launch_as<NN>(in_type, out_type, p, q, qs, a, stream);
+  if (mode == 0) return pair ? launch_as<NT, 2>(in_type, out_type, p, q, qs, a, stream) : launch_as<NT, 1>(in_type, out_type, p, q, qs, a, stream);
+  return pair ? launch_as<NN, 2>(in_type, out_type, p, q, qs, a, stream) : launch_as<NN, 1>(in_type, out_type, p, q, qs, a, stream);
 }
 
 // out [groups, N, K] (contiguous): every matrix is written, zeros where a group has no row
@@ -377,7 +415,8 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
   if (rc == 0) rc = make_map_3d(&q, t, Y, N, rows, 1, ldy * 2, ldy * 2, 64, BR);
   if (rc) return rc;
   Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0};
-  return launch_as<TN>(in_type, out_type, p, q, q, a, stream);
+  return use_pairs((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K) ? launch_as<TN, 2>(in_type, out_type, p, q, q, a, stream)
+                                                                            : launch_as<TN, 1>(in_type, out_type, p, q, q, a, stream);
 }
 
 // Copies the status block of the grouped products to `host` and clears it (waits for the stream).

@@ -51,6 +51,15 @@ struct Table {
   }
 };
 
+// One lane of a converged warp.  Loads by the copy engine, products and commits take their operands from the warp's uniform
+// registers: issued under this condition by a warp that runs its loop as a whole they cost a few instructions, under
+// `lane == 0` several times as many.
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // as mbar_wait, for a barrier that the other CTA of a pair arrives on
 __device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   const uint32_t addr = smem_u32(bar);
@@ -102,11 +111,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// arrive on the barrier at this shared-memory address (in both CTAs of a pair) once every product issued so far by this thread has finished
 template <int CG>
-__device__ __forceinline__ void commit(uint32_t cluster_addr) {
-  if (CG == 2) umma_commit_pair(cluster_addr);
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (CG == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                 : "memory");
   else
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 template <int CG>
