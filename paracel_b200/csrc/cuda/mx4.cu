@@ -5,7 +5,8 @@
 // half; scales [ceil(K / 128), rows] words of four codes, byte i of word (b, r) is the code of row r's block 4 b + i.
 // A word holds the scales of 128 values, and the words of neighbouring rows are neighbours: a tile of rows finds its
 // scales in one piece wherever it begins.  A code c stands for 2^(c - 127), 255 for NaN.
-#include "grouped.cuh"
+#include <stdlib.h>
+#include "tiles_sm100.cuh"
 
 namespace {
 
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(QTHREADS) quantize_kernel(QuantArgs a) {
   __shared__ uint32_t words[QROWS];
   const int word = blockIdx.x % a.words;
   const long long r0 = (long long)(blockIdx.x / a.words) * QROWS;
-  const int lane = threadIdx.x & 31, part = threadIdx.x & 15;
+  const int part = threadIdx.x & 15;
   const int c0 = word * 128 + part * 8;
   const int row_bytes4 = (a.K + 31) / 32 * 4;          // 4-byte words of a row of data
 #pragma unroll
@@ -106,7 +107,6 @@ __global__ void __launch_bounds__(QTHREADS) quantize_kernel(QuantArgs a) {
     if (part == 0) words[lr] = w;
   }
   __syncthreads();
-  (void)lane;
   if (threadIdx.x < QROWS && r0 + threadIdx.x < a.rows)
     a.scales[(long long)word * a.rows + r0 + threadIdx.x] = words[threadIdx.x];
 }
@@ -146,80 +146,386 @@ __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
   }
 }
 
-struct RowsArgs {
-  const uint8_t* A;
-  const uint32_t* sa;
-  const uint8_t* B;
-  const uint32_t* sb;
+// ------------------------------------------------------------------------------------------ products
+//
+// D[m, j] = sum_r P[m, r] Q[j, r] (tiles_sm100.cuh) with P = the rows of B, Q = those of A, by tcgen05.mma kind::mxf4: 64
+// values a step, exact products of the four-bit values, scaled by the two blocks' scales, fp32 sums.
+//
+// The instruction takes the scales from tensor memory, for 128 rows in 32 lanes x 4 columns (row r in lane r mod 32, column r / 32), a word of four
+// codes for 128 values of a row; four copies of it stand in the four quarters of the lanes.  A stage of 256 values has two
+// such words of every row.  Three warps fetch them (a word of neighbouring rows is one line), one for P, two for Q, put them
+// into shared memory in that order, and tcgen05.cp spreads them, behind the operands' arrival and ahead of the products.
+//
+// Accumulators have 224 columns, so that two of them leave room for two stages' scales (24 columns each) in the 512 columns of tensor memory.
+// Roles in a CTA: warp 0 loads operands, warp 1 issues products (in the second CTA of a pair it passes on that its scales have come), warps 2-9
+// store, warps 10-12 fetch scales.
+using namespace pcl_tiles;
+
+constexpr int COLS = 224;
+constexpr int LANES = 128;
+constexpr int BR = 256;                        // values of a row in a stage: 128 bytes
+constexpr int P_BYTES = LANES * 128;
+constexpr int SCALE_BYTES = 3 * 1024;          // P, Q rows 0-127, Q rows 128-255: two blocks of 512 bytes each
+constexpr int SCALE_COLS = 24;
+constexpr int TMEM_COLS = 512;
+constexpr int MAX_STAGES = 6;
+constexpr int EPI_WARPS = 8;
+constexpr int SCALE_WARP = 2 + EPI_WARPS;
+constexpr int THREADS = 32 * (SCALE_WARP + 3);
+constexpr int SMALL_BOX = 32;
+static_assert(2 * COLS + 2 * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
+
+template <int CG>
+struct Form {
+  static constexpr int Q_ROWS = COLS / CG;
+  static constexpr int Q_BYTES = (Q_ROWS + 31) / 32 * 32 * 128;
+  static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
+  static constexpr int STAGES = CG == 2 ? 6 : 4;
+  static constexpr int M = LANES * CG;
+};
+
+struct Args {
+  const uint32_t* sp;   // words of B's scales [words, groups * N]
+  const uint32_t* sq;   // of A's [words, rows]
   void* out;
   long long ldo;
   Offsets off;
-  int N, K, fill;
+  int N, steps, words, blocks, fill;
 };
+
+struct Shared {
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], scales[MAX_STAGES], peer_scales[MAX_STAGES], tfull[2], tempty[2];
+  uint32_t tmem;
+  int abort_flag;
+  Table table;
+};
+
+template <int CG>
+constexpr int smem_bytes() { return 1024 + Form<CG>::STAGES * (Form<CG>::STAGE_BYTES + SCALE_BYTES) + (int)sizeof(Shared); }
 
 __device__ PclStatus g_status;
 
-constexpr int T = 64, KB = 32, THREADS = 256;
-
-__device__ __forceinline__ float value_at(const uint8_t* data, const uint32_t* scales, long long rows, int row_bytes, long long r, int k) {
-  const uint32_t c = data[r * row_bytes + (k >> 1)] >> (4 * (k & 1));
-  return mul_keep(code_value(c & 15u), scale_value((scales[(long long)(k >> 7) * rows + r] >> (8 * ((k >> 5) & 3))) & 255u));
+// a block of 32 rows x 16 bytes without swizzle: eight rows are 128 bytes in one piece
+__device__ __forceinline__ uint64_t desc_scales(uint32_t saddr) {
+  return ((uint64_t)(8u | (1u << 14)) << 32) | ((saddr >> 4) & 0x3FFFu) | (8u << 16);
 }
 
-template <class TO>
-__global__ void __launch_bounds__(THREADS) rows_kernel(RowsArgs a) {
-  __shared__ int bounds[MAX_GROUPS + 1];
-  __shared__ float ps[KB][T], qs[KB][T];
-  load_bounds(a.off, bounds, &g_status);
-  __syncthreads();
-  TO* out = static_cast<TO*>(a.out);
-  const int across = (a.N + T - 1) / T;
-  int tile = blockIdx.x / across, e = 0;
-  for (; e < a.off.groups; ++e) {
-    const int n = (bounds[e + 1] - bounds[e] + T - 1) / T;
-    if (tile < n) break;
-    tile -= n;
+template <int CG>
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+  if (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  if (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+
+struct Tile {
+  int e, m0, j0, n, ncol;   // columns: n of them, ncol with those that the product rounds up to
+};
+
+// The tiles of a call, numbered: those that share rows of A are neighbours.
+template <int CG>
+struct Walk {
+  const Table& t;
+  int mb, e;
+  long long tiles;
+
+  __device__ Walk(const Args& a, const Table& t_) : t(t_), e(0) {
+    mb = (a.N + Form<CG>::M - 1) / Form<CG>::M;
+    tiles = (long long)t.chunks[a.off.groups] * mb;
   }
-  const int c0 = blockIdx.x % across * T;
-  if (e == a.off.groups) {   // rows of no group
-    if (!a.fill || tile != 0) return;
-    for (long long r = threadIdx.x; r < a.off.rows; r += THREADS)
-      if (r < bounds[0] || r >= bounds[a.off.groups])
-        for (int c = c0; c < min(c0 + T, a.N); ++c) out[r * a.ldo + c] = to_out<TO>(0.f);
-    return;
+
+  __device__ Tile at(long long i) {   // rising i
+    Tile w;
+    const long long c = i / mb;
+    w.m0 = (int)(i - c * mb) * Form<CG>::M;
+    t.find((int)c, 16 * CG, e, w.j0, w.n);
+    w.e = e;
+    w.ncol = (w.n + 16 * CG - 1) / (16 * CG) * (16 * CG);
+    return w;
   }
-  const int t0 = bounds[e] + tile * T, t1 = bounds[e + 1];
-  const int row_bytes = (a.K + 31) / 32 * 16;
-  const long long b_rows = (long long)a.off.groups * a.N;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += KB) {
-    for (int i = threadIdx.x; i < KB * T; i += THREADS) {
-      const int k = k0 + i % KB, m = i / KB;
-      qs[i % KB][m] = (k < a.K && t0 + m < t1) ? value_at(a.A, a.sa, a.off.rows, row_bytes, t0 + m, k) : 0.f;
-      ps[i % KB][m] = (k < a.K && c0 + m < a.N) ? value_at(a.B, a.sb, b_rows, row_bytes, (long long)e * a.N + c0 + m, k) : 0.f;
+};
+
+template <int CG, class TO>
+__global__ void __launch_bounds__(THREADS, 1)
+product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
+               const __grid_constant__ CUtensorMap mapQ_small, Args a) {
+  using F = Form<CG>;
+  constexpr int STAGES = F::STAGES, STAGE_BYTES = F::STAGE_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* scales = stages + STAGES * STAGE_BYTES;
+  Shared& s = *reinterpret_cast<Shared*>(scales + STAGES * SCALE_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t me = CG == 2 ? cluster_ctarank() : 0;   // 0 leads the pair
+  volatile int* abort_flag = &s.abort_flag;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < STAGES; ++i) {
+        mbar_init(s.full + i, 1);
+        mbar_init(s.empty + i, 1);
+        mbar_init(s.scales + i, 3);
+        mbar_init(s.peer_scales + i, 1);
+      }
+      for (int i = 0; i < 2; ++i) { mbar_init(s.tfull + i, 1); mbar_init(s.tempty + i, CG * EPI_WARPS); }
+      s.abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
-    const int tm = (threadIdx.x & 15) * 4, tj = (threadIdx.x >> 4) * 4;
-#pragma unroll
-    for (int r = 0; r < KB; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(ps[r][tm + i], qs[r][tj + j], acc[i][j]);
-    __syncthreads();
+    s.table.build(a.off, COLS, &g_status);
   }
-  const int tm = (threadIdx.x & 15) * 4, tj = (threadIdx.x >> 4) * 4;
-  for (int j = 0; j < 4; ++j)
-    for (int i = 0; i < 4; ++i)
-      if (t0 + tj + j < t1 && c0 + tm + i < a.N) out[(long long)(t0 + tj + j) * a.ldo + c0 + tm + i] = to_out<TO>(acc[i][j]);
+  if (warp == 1) tmem_alloc<CG>(&s.tmem, TMEM_COLS);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  sync_cluster_or_block<CG>();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = s.tmem;
+  const int group = blockIdx.x / CG, groups = gridDim.x / CG;
+  Walk<CG> walk(a, s.table);
+  bool ok = true;
+  auto gave_up = [&](int where, int x, int y) {
+    if (lane == 0) report(&g_status, 0, where, x, y);
+    abort_all<CG>(abort_flag, me ^ 1u);
+    ok = false;
+  };
+
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      const Tile w = walk.at(i);
+      const int mine = w.ncol / CG;
+      const int j = w.j0 + (int)me * mine, m = w.m0 + (int)me * LANES;
+      const bool whole = mine == F::Q_ROWS;
+      const int boxes = whole ? 1 : (mine + SMALL_BOX - 1) / SMALL_BOX;
+      const uint32_t bytes = P_BYTES + (whole ? F::Q_ROWS * 128 : boxes * SMALL_BOX * 128);
+      for (int kb = 0; kb < a.steps; ++kb) {
+        if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(41, kb, stage); break; }
+        if (elect()) {
+          const uint32_t sp = smem_u32(stages + stage * STAGE_BYTES), sq = sp + P_BYTES;
+          uint32_t bar = smem_u32(s.full + stage);
+          if (CG == 2) bar = map_to_cta(bar, 0);
+          if (me == 0) mbar_expect_tx(s.full + stage, CG * bytes);
+          tma_load_3d<CG>(sp, &mapP, bar, kb * 128, m, w.e);
+          if (whole) {
+            tma_load_3d<CG>(sq, &mapQ, bar, kb * 128, j, 0);
+          } else {
+            for (int b = 0; b < boxes; ++b)
+              tma_load_3d<CG>(sq + b * SMALL_BOX * 128, &mapQ_small, bar, kb * 128, j + b * SMALL_BOX, 0);
+          }
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (!ok)
+      for (int i = 0; i < 2048; ++i) __nanosleep(1000);   // copies in flight land before the shared memory goes away
+  } else if (warp == 1 && me != 0) {
+    // this CTA's scales are in place: tell the leader, whose products read them
+    int stage = 0;
+    uint32_t phase = 0;
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      for (int kb = 0; kb < a.steps; ++kb) {
+        if (!mbar_wait(s.scales + stage, phase, abort_flag)) { gave_up(46, kb, stage); break; }
+        if (lane == 0) arrive_cluster(map_to_cta(smem_u32(s.peer_scales + stage), 0));
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // operands E2M1, scales E8M0
+    const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(F::M >> 4) << 24);
+    const uint64_t dp0 = desc_k_major(smem_u32(stages)), ds0 = desc_scales(smem_u32(scales));
+    int stage = 0, acc = 0, buf = 0;
+    uint32_t phase = 0, acc_phase[2] = {0, 0};
+    int old_stage = 0;                       // the stage before the last: its products use the scales' other half
+    uint32_t old_phase = 0;
+    long long done = 0;
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      const Tile w = walk.at(i);
+      if (!mbar_wait(s.tempty + acc, acc_phase[acc] ^ 1, abort_flag)) { gave_up(42, acc, 0); break; }
+      acc_phase[acc] ^= 1;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
+      const uint32_t d = tmem + (uint32_t)(acc * COLS);
+      const bool wide = w.ncol > 128;
+      for (int kb = 0; kb < a.steps; ++kb) {
+        // the products of two stages ago have read the scales that are overwritten now
+        if (done >= 2) {
+          if (!mbar_wait(s.empty + old_stage, old_phase, abort_flag)) { gave_up(47, kb, old_stage); break; }
+          if (++old_stage == STAGES) { old_stage = 0; old_phase ^= 1; }
+        }
+        if (!wait_full(s.full + stage, phase, abort_flag) || !mbar_wait(s.scales + stage, phase, abort_flag) ||
+            (CG == 2 && !wait_full(s.peer_scales + stage, phase, abort_flag))) {
+          gave_up(43, kb, stage);
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect()) {
+          const uint32_t sf = tmem + (uint32_t)(2 * COLS + buf * SCALE_COLS);
+          const uint64_t ds = ds0 + (uint32_t)(stage * SCALE_BYTES) / 16;
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            copy_scales<CG>(sf + v * 4, ds + v * 32);
+            copy_scales<CG>(sf + 8 + v * 8, ds + 64 + v * 32);
+            if (wide) copy_scales<CG>(sf + 12 + v * 8, ds + 128 + v * 32);
+          }
+          const uint64_t dp = dp0 + (uint32_t)(stage * STAGE_BYTES) / 16;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t id = (uint32_t)(k & 1) * 2;   // codes 0, 1 or 2, 3 of a word
+            umma_mxf4<CG>(d, dp + 2 * k, dp + P_BYTES / 16 + 2 * k, idesc | (id << 4) | (id << 29), sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8,
+                          (kb > 0 || k > 0) ? 1u : 0u);
+          }
+          commit<CG>(smem_u32(s.empty + stage));
+          if (kb + 1 == a.steps) commit<CG>(smem_u32(s.tfull + acc));
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        buf ^= 1;
+        ++done;
+      }
+      acc ^= 1;
+    }
+  } else if (warp >= SCALE_WARP) {
+    const int part = warp - SCALE_WARP;      // 0: P, 1 and 2: Q
+    const uint32_t* src = part == 0 ? a.sp : a.sq;
+    const long long rows = part == 0 ? (long long)a.off.groups * a.N : a.off.rows;
+    // codes of the last word that no block has
+    const int spare = a.words * 4 - a.blocks;
+    const uint32_t last_mask = 0xffffffffu >> (8 * spare);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      const Tile w = walk.at(i);
+      const bool used = part < 2 || w.ncol > 128;
+      const long long r0 = part == 0 ? (long long)w.e * a.N + w.m0 + (long long)me * LANES : (long long)w.j0 + (part - 1) * 128;
+      long long at[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) at[q] = min(r0 + lane + 32 * q, rows - 1);   // rows of no tile: any scales do
+      constexpr int AHEAD = 4;
+      for (int k0 = 0; k0 < a.steps && ok; k0 += AHEAD) {
+        uint32_t v[AHEAD][2][4];
+#pragma unroll
+        for (int b = 0; b < AHEAD; ++b)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const int word = (k0 + b) * 2 + (q >> 2);
+            uint32_t x = 0;
+            if (used && word < a.words) {
+              x = __ldg(src + word * rows + at[q & 3]);
+              if (word == a.words - 1) x &= last_mask;
+            }
+            v[b][q >> 2][q & 3] = x;
+          }
+#pragma unroll
+        for (int b = 0; b < AHEAD; ++b) {
+          if (k0 + b >= a.steps || !ok) continue;
+          if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(48, k0 + b, stage); continue; }
+          if (used) {
+            uint4* dst = reinterpret_cast<uint4*>(scales + stage * SCALE_BYTES + part * 1024) + lane;
+            dst[0] = make_uint4(v[b][0][0], v[b][0][1], v[b][0][2], v[b][0][3]);
+            dst[32] = make_uint4(v[b][1][0], v[b][1][1], v[b][1][2], v[b][1][3]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          __syncwarp();
+          if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(s.scales + stage)) : "memory");
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else {
+    const int sub = warp & 3;                 // the quarter of the tensor memory's lanes that this warp can read
+    const int half = (warp - 2) >> 2;         // two warps share a quarter: 32 columns in turn
+    TO* out = static_cast<TO*>(a.out);
+    int acc = 0;
+    uint32_t acc_phase[2] = {0, 0};
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      const Tile w = walk.at(i);
+      if (!mbar_wait(s.tfull + acc, acc_phase[acc], abort_flag)) { gave_up(44, acc, 0); break; }
+      acc_phase[acc] ^= 1;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int m = w.m0 + (int)me * LANES + sub * 32 + lane;
+      TO* dst = out + (long long)w.j0 * a.ldo + m;
+      const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * COLS);
+      for (int c = half * 32; c < w.n; c += 64) {
+        uint32_t v[32];
+        tmem_ld32_issue(t0 + (uint32_t)c, v);
+        tmem_ld_wait(v);
+        if (m < a.N) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < w.n) dst[(long long)(c + j) * a.ldo] = to_out<TO>(__uint_as_float(v[j]));
+        }
+        __syncwarp();
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
+      acc ^= 1;
+    }
+    if (a.fill) {
+      const int first = s.table.bounds[0], last = s.table.bounds[a.off.groups];
+      const int rows = first + a.off.rows - last;
+      for (long long q = (long long)blockIdx.x * EPI_WARPS + warp - 2; q < rows; q += (long long)gridDim.x * EPI_WARPS) {
+        TO* row = out + (q < first ? q : q - first + last) * a.ldo;
+        for (int c = lane; c < a.N; c += 32) row[c] = to_out<TO>(0.f);
+      }
+    }
+  }
+
+  // nobody leaves while the pair still reads this CTA's shared memory or signals its barriers
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  sync_cluster_or_block<CG>();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    tmem_free<CG>(tmem, TMEM_COLS);
+  }
 }
 
-template <class TO>
-int launch_rows(const RowsArgs& a, cudaStream_t stream) {
-  const long long grid = ((a.off.rows + T - 1ll) / T + a.off.groups + 1) * ((a.N + T - 1ll) / T);
-  if (grid >= (1ll << 31)) return (int)cudaErrorInvalidValue;
-  rows_kernel<TO><<<(unsigned)grid, THREADS, 0, stream>>>(a);
-  return pcl_last_error();
+template <int CG, class TO>
+int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
+  auto kernel = product_kernel<CG, TO>;
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<CG>());
+  if (e != cudaSuccess) return (int)e;
+  const long long mb = (a.N + Form<CG>::M - 1) / Form<CG>::M;
+  const long long chunks = a.off.rows / COLS + min(a.off.groups, a.off.rows);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)min((long long)(sms / CG), chunks * mb) * CG);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem_bytes<CG>();
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, a);
+  return e != cudaSuccess ? (int)e : pcl_last_error();
+}
+
+template <int CG>
+int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
+  if (out_type == TYPE_F32) return launch<CG, float>(p, q, qs, a, stream);
+  if (out_type == TYPE_BF16) return launch<CG, __nv_bfloat16>(p, q, qs, a, stream);
+  return launch<CG, __half>(p, q, qs, a, stream);
 }
 
 bool blocks_of(long long rows, int words, long long* n) {
@@ -266,12 +572,18 @@ PCL_API int pcl_mx4_rows(const void* A, const void* sa, const void* B, const voi
       (long long)groups * N >= (1ll << 31) - 512)
     return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
-  RowsArgs a{static_cast<const uint8_t*>(A), static_cast<const uint32_t*>(sa), static_cast<const uint8_t*>(B),
-             static_cast<const uint32_t*>(sb), out, ldo, Offsets{offsets, off64, groups, (int)rows}, N, K, fill};
-  if (out_type == TYPE_F32) return launch_rows<float>(a, stream);
-  if (out_type == TYPE_BF16) return launch_rows<__nv_bfloat16>(a, stream);
-  if (out_type == TYPE_F16) return launch_rows<__half>(a, stream);
-  return (int)cudaErrorInvalidValue;
+  if (out_type < 0 || out_type > 2) return (int)cudaErrorInvalidValue;
+  const long long row_bytes = (K + 31) / 32 * 16;
+  const bool pair = getenv("PCL_PAIR") ? getenv("PCL_PAIR")[0] == '1' : (rows / COLS + min((long long)groups, rows) / 2) * ((N + LANES - 1) / LANES) >= 2 * 148;
+  CUtensorMap p, q, qs;
+  const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  int rc = make_map_3d(&p, t, B, row_bytes, N, groups, row_bytes, row_bytes * N, 128, LANES);
+  if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, pair ? Form<2>::Q_ROWS : Form<1>::Q_ROWS);
+  if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, SMALL_BOX);
+  if (rc) return rc;
+  Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
+         N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill};
+  return pair ? launch_as<2>(out_type, p, q, qs, a, stream) : launch_as<1>(out_type, p, q, qs, a, stream);
 }
 
 // Copies the status block of these products to `host` and clears it (waits for the stream).
