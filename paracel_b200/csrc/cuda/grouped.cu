@@ -40,6 +40,7 @@ struct Form {
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
   static constexpr int STAGES = OPERAND_BYTES / STAGE_BYTES;
   static constexpr int M = LANES * CG;   // m of a tile
+  static_assert(MAX_COLS % (16 * CG) == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
 };
 constexpr int SMALL_BOX = 32;                  // rows of Q that are loaded at a time where a chunk is not full
 
@@ -52,6 +53,7 @@ struct Args {
   int red;             // nt, nn: extent of the reduction
   uint32_t type;       // operands: 0 fp16, 1 bf16
   int fill;            // nt, nn: rows of no group become zero
+  bool boxed;          // results leave through mapOut
 };
 
 struct Shared {
@@ -61,7 +63,7 @@ struct Shared {
   Table table;
 };
 
-constexpr int SMEM_BYTES = 1024 + OPERAND_BYTES + (int)sizeof(Shared);
+constexpr int SMEM_BYTES = 1024 + OPERAND_BYTES + EPI_WARPS * PIECE_BYTES + (int)sizeof(Shared);
 
 struct Tile {
   int e, m0, j0, n, ncol, r0, r1;   // columns: n of them, ncol with those that the product rounds up to
@@ -111,12 +113,13 @@ struct Walk {
 template <int MODE, int CG, class TO>
 __global__ void __launch_bounds__(threads_of(MODE), 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
-               const __grid_constant__ CUtensorMap mapQ_small, Args a) {
+               const __grid_constant__ CUtensorMap mapQ_small, const __grid_constant__ CUtensorMap mapOut, Args a) {
   using F = Form<CG>;
   constexpr int Q_BYTES = F::Q_BYTES, STAGE_BYTES = F::STAGE_BYTES, STAGES = F::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  Shared& s = *reinterpret_cast<Shared*>(stages + OPERAND_BYTES);
+  uint8_t* pieces = stages + OPERAND_BYTES;
+  Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t me = CG == 2 ? cluster_ctarank() : 0;   // 0 leads the pair
   volatile int* abort_flag = &s.abort_flag;
@@ -285,11 +288,11 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     uint32_t acc_phase[2] = {0, 0};
     for (long long i = group; i < walk.tiles && ok; i += groups) {
       const Tile w = walk.at(i);
-      const int m = w.m0 + (int)me * LANES + sub * 32 + lane;
+      const int m = w.m0 + (int)me * LANES + sub * 32;
       TO* dst = out + (MODE == TN ? ((long long)w.e * a.jdim + w.j0) * a.ldo : (long long)w.j0 * a.ldo) + m;
       if (w.r1 <= w.r0) {   // a group without rows: its matrix of sums is zero
-        if (m < a.mdim)
-          for (int j = half; j < w.n; j += 2) dst[(long long)j * a.ldo] = to_out<TO>(0.f);
+        if (m + lane < a.mdim)
+          for (int j = half; j < w.n; j += 2) dst[(long long)j * a.ldo + lane] = to_out<TO>(0.f);
         continue;
       }
       if (!mbar_wait(s.tfull + acc, acc_phase[acc], abort_flag)) {
@@ -301,22 +304,13 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       acc_phase[acc] ^= 1;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * MAX_COLS);
-      for (int c = half * 32; c < w.n; c += 64) {
-        uint32_t v[32];
-        tmem_ld32_issue(t0 + (uint32_t)c, v);
-        tmem_ld_wait(v);
-        if (m < a.mdim) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < w.n) dst[(long long)(c + j) * a.ldo] = to_out<TO>(__uint_as_float(v[j]));
-        }
-        __syncwarp();
-      }
+      store_columns<TO>(t0, half * 32, w.n, dst, a.ldo, a.mdim - m, a.boxed, pieces + (warp - 2) * PIECE_BYTES, &mapOut, m, w.j0, MODE == TN ? w.e : 0);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
       acc ^= 1;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the copy engine has read and written all boxes
     if (MODE != TN && a.fill) {
       const int first = s.table.bounds[0], last = s.table.bounds[a.off.groups];
       const int rows = first + a.off.rows - last;
@@ -338,7 +332,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
 }
 
 template <int MODE, int CG, class TO>
-int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
+int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
   auto kernel = product_kernel<MODE, CG, TO>;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -360,15 +354,15 @@ int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, co
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = CG > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, a);
+  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, o, a);
   return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 
 template <int MODE, int CG>
-int launch_as(int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
-  if (out_type == TYPE_F32) return launch<MODE, CG, float>(p, q, qs, a, stream);
+int launch_as(int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
+  if (out_type == TYPE_F32) return launch<MODE, CG, float>(p, q, qs, o, a, stream);
   if (out_type != in_type) return (int)cudaErrorInvalidValue;
-  return in_type == TYPE_BF16 ? launch<MODE, CG, __nv_bfloat16>(p, q, qs, a, stream) : launch<MODE, CG, __half>(p, q, qs, a, stream);
+  return in_type == TYPE_BF16 ? launch<MODE, CG, __nv_bfloat16>(p, q, qs, o, a, stream) : launch<MODE, CG, __half>(p, q, qs, o, a, stream);
 }
 
 // Whether pairs of CTAs take the tiles.  A pair loads a third fewer bytes for its 256 x 256 tile than two CTAs for theirs, but there are half as
@@ -394,14 +388,15 @@ PCL_API int pcl_grouped_rows(int mode, int in_type, int out_type, const void* X,
   const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int red = mode == 0 ? K : N;
   const bool pair = use_pairs(rows / MAX_COLS + min((long long)groups, rows) / 2, mode == 0 ? N : K);
-  CUtensorMap p, q, qs;
+  CUtensorMap p, q, qs, o;
   int rc = make_map_3d(&p, t, W, K, N, groups, ws_n * 2, ws_e * 2, 64, mode == 0 ? LANES : BR);
   if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, pair ? MAX_COLS / 2 : MAX_COLS);
   if (rc == 0) rc = make_map_3d(&qs, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SMALL_BOX);
   if (rc) return rc;
-  Args a{out, ldo, Offsets{offsets, off64, groups, (int)rows}, mode == 0 ? N : K, 0, red, in_type == TYPE_BF16 ? 1u : 0u, fill};
-  if (mode == 0) return pair ? launch_as<NT, 2>(in_type, out_type, p, q, qs, a, stream) : launch_as<NT, 1>(in_type, out_type, p, q, qs, a, stream);
-  return pair ? launch_as<NN, 2>(in_type, out_type, p, q, qs, a, stream) : launch_as<NN, 1>(in_type, out_type, p, q, qs, a, stream);
+  Args a{out, ldo, Offsets{offsets, off64, groups, (int)rows}, mode == 0 ? N : K, 0, red, in_type == TYPE_BF16 ? 1u : 0u, fill, false};
+  a.boxed = make_out_map(&o, p, out_type, out, a.mdim, rows, 1, ldo, ldo);
+  if (mode == 0) return pair ? launch_as<NT, 2>(in_type, out_type, p, q, qs, o, a, stream) : launch_as<NT, 1>(in_type, out_type, p, q, qs, o, a, stream);
+  return pair ? launch_as<NN, 2>(in_type, out_type, p, q, qs, o, a, stream) : launch_as<NN, 1>(in_type, out_type, p, q, qs, o, a, stream);
 }
 
 // out [groups, N, K] (contiguous): every matrix is written, zeros where a group has no row
@@ -410,13 +405,14 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
                            cudaStream_t stream) {
   if (!sizes_ok(in_type, rows, groups, N, K) || rows == 0) return (int)cudaErrorInvalidValue;
   const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap p, q;
+  CUtensorMap p, q, o;
   int rc = make_map_3d(&p, t, X, K, rows, 1, ldx * 2, ldx * 2, 64, BR);
   if (rc == 0) rc = make_map_3d(&q, t, Y, N, rows, 1, ldy * 2, ldy * 2, 64, BR);
   if (rc) return rc;
-  Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0};
-  return use_pairs((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K) ? launch_as<TN, 2>(in_type, out_type, p, q, q, a, stream)
-                                                                            : launch_as<TN, 1>(in_type, out_type, p, q, q, a, stream);
+  Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0, false};
+  a.boxed = make_out_map(&o, p, out_type, out, K, N, groups, K, (long long)N * K);
+  return use_pairs((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K) ? launch_as<TN, 2>(in_type, out_type, p, q, q, o, a, stream)
+                                                                            : launch_as<TN, 1>(in_type, out_type, p, q, q, o, a, stream);
 }
 
 // Copies the status block of the grouped products to `host` and clears it (waits for the stream).

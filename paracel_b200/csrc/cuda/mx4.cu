@@ -167,21 +167,25 @@ constexpr int BR = 256;                        // values of a row in a stage: 12
 constexpr int P_BYTES = LANES * 128;
 constexpr int SCALE_BYTES = 3 * 1024;          // P, Q rows 0-127, Q rows 128-255: two blocks of 512 bytes each
 constexpr int SCALE_COLS = 24;
+constexpr int SCALE_BUFS = 2;
 constexpr int TMEM_COLS = 512;
-constexpr int MAX_STAGES = 6;
+constexpr int MAX_STAGES = 5;
 constexpr int EPI_WARPS = 8;
 constexpr int SCALE_WARP = 2 + EPI_WARPS;
-constexpr int THREADS = 32 * (SCALE_WARP + 3);
+constexpr int RELAY_WARP = SCALE_WARP + 3;     // three, of a pair only
+constexpr int RELAYS = 4;                      // with warp 1 of the second CTA
+template <int CG> constexpr int threads_of() { return 32 * (RELAY_WARP + (CG == 2 ? RELAYS - 1 : 0)); }
 constexpr int SMALL_BOX = 32;
-static_assert(2 * COLS + 2 * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
+static_assert(2 * COLS + SCALE_BUFS * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
 
 template <int CG>
 struct Form {
   static constexpr int Q_ROWS = COLS / CG;
   static constexpr int Q_BYTES = (Q_ROWS + 31) / 32 * 32 * 128;
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
-  static constexpr int STAGES = CG == 2 ? 6 : 4;
+  static constexpr int STAGES = CG == 2 ? 5 : 4;
   static constexpr int M = LANES * CG;
+  static_assert(COLS % (16 * CG) == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
 };
 
 struct Args {
@@ -191,6 +195,7 @@ struct Args {
   long long ldo;
   Offsets off;
   int N, steps, words, blocks, fill;
+  bool boxed;   // results leave through mapOut
 };
 
 struct Shared {
@@ -201,7 +206,7 @@ struct Shared {
 };
 
 template <int CG>
-constexpr int smem_bytes() { return 1024 + Form<CG>::STAGES * (Form<CG>::STAGE_BYTES + SCALE_BYTES) + (int)sizeof(Shared); }
+constexpr int smem_bytes() { return 1024 + Form<CG>::STAGES * (Form<CG>::STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (int)sizeof(Shared); }
 
 __device__ PclStatus g_status;
 
@@ -260,15 +265,16 @@ struct Walk {
 };
 
 template <int CG, class TO>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(threads_of<CG>(), 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
-               const __grid_constant__ CUtensorMap mapQ_small, Args a) {
+               const __grid_constant__ CUtensorMap mapQ_small, const __grid_constant__ CUtensorMap mapOut, Args a) {
   using F = Form<CG>;
   constexpr int STAGES = F::STAGES, STAGE_BYTES = F::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* scales = stages + STAGES * STAGE_BYTES;
-  Shared& s = *reinterpret_cast<Shared*>(scales + STAGES * SCALE_BYTES);
+  uint8_t* pieces = scales + STAGES * SCALE_BYTES;
+  Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t me = CG == 2 ? cluster_ctarank() : 0;   // 0 leads the pair
   volatile int* abort_flag = &s.abort_flag;
@@ -332,14 +338,19 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     }
     if (!ok)
       for (int i = 0; i < 2048; ++i) __nanosleep(1000);   // copies in flight land before the shared memory goes away
-  } else if (warp == 1 && me != 0) {
-    // this CTA's scales are in place: tell the leader, whose products read them
-    int stage = 0;
+  } else if (CG == 2 && (warp >= RELAY_WARP || (warp == 1 && me != 0))) {
+    // This CTA's scales are in place: tell the leader, whose products read them.  An arrival that releases to the cluster
+    // takes about a microsecond, two stages' products: four warps take the stages in turn.
+    const int mine = warp == 1 ? 0 : warp - RELAY_WARP + 1;
+    int stage = 0, turn = 0;
     uint32_t phase = 0;
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
+    for (long long i = group; i < walk.tiles && ok && me != 0; i += groups) {
       for (int kb = 0; kb < a.steps; ++kb) {
-        if (!mbar_wait(s.scales + stage, phase, abort_flag)) { gave_up(46, kb, stage); break; }
-        if (lane == 0) arrive_cluster(map_to_cta(smem_u32(s.peer_scales + stage), 0));
+        if (turn == mine) {
+          if (!mbar_wait(s.scales + stage, phase, abort_flag)) { gave_up(46, kb, stage); break; }
+          if (lane == 0) arrive_cluster(map_to_cta(smem_u32(s.peer_scales + stage), 0));
+        }
+        if (++turn == RELAYS) turn = 0;
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
     }
@@ -362,7 +373,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const bool wide = w.ncol > 128;
       for (int kb = 0; kb < a.steps; ++kb) {
         // the products of two stages ago have read the scales that are overwritten now
-        if (done >= 2) {
+        if (done >= SCALE_BUFS) {
           if (!mbar_wait(s.empty + old_stage, old_phase, abort_flag)) { gave_up(47, kb, old_stage); break; }
           if (++old_stage == STAGES) { old_stage = 0; old_phase ^= 1; }
         }
@@ -393,7 +404,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         }
         __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        buf ^= 1;
+        if (++buf == SCALE_BUFS) buf = 0;
         ++done;
       }
       acc ^= 1;
@@ -405,44 +416,56 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     // codes of the last word that no block has
     const int spare = a.words * 4 - a.blocks;
     const uint32_t last_mask = 0xffffffffu >> (8 * spare);
-    int stage = 0;
+    // the words of a stage are asked for DEPTH stages before they are stored
+    constexpr int DEPTH = 3;
+    uint32_t v[DEPTH][8];
+    bool used[DEPTH];
+    long long at[4];
+    long long tile = group;
+    int kb = a.steps;
+    bool in_use = false;
+    auto fetch = [&](int d) {
+      if (kb == a.steps) {
+        if (tile >= walk.tiles) return;
+        const Tile w = walk.at(tile);
+        tile += groups;
+        kb = 0;
+        in_use = part < 2 || w.ncol > 128;
+        const long long r0 = part == 0 ? (long long)w.e * a.N + w.m0 + (long long)me * LANES : (long long)w.j0 + (part - 1) * 128;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) at[q] = min(r0 + lane + 32 * q, rows - 1);   // rows of no tile: any scales do
+      }
+      used[d] = in_use;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int word = kb * 2 + (q >> 2);
+        v[d][q] = in_use && word < a.words ? __ldg(src + word * rows + at[q & 3]) : 0u;
+      }
+      ++kb;
+    };
+    long long left = walk.tiles > group ? ((walk.tiles - group + groups - 1) / groups) * a.steps : 0;
+    int stage = 0, now = 0;
     uint32_t phase = 0;
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
-      const Tile w = walk.at(i);
-      const bool used = part < 2 || w.ncol > 128;
-      const long long r0 = part == 0 ? (long long)w.e * a.N + w.m0 + (long long)me * LANES : (long long)w.j0 + (part - 1) * 128;
-      long long at[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) at[q] = min(r0 + lane + 32 * q, rows - 1);   // rows of no tile: any scales do
-      constexpr int AHEAD = 4;
-      for (int k0 = 0; k0 < a.steps && ok; k0 += AHEAD) {
-        uint32_t v[AHEAD][2][4];
+    for (int d = 0; d < DEPTH; ++d) fetch(d);
+    while (left > 0 && ok) {
 #pragma unroll
-        for (int b = 0; b < AHEAD; ++b)
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int word = (k0 + b) * 2 + (q >> 2);
-            uint32_t x = 0;
-            if (used && word < a.words) {
-              x = __ldg(src + word * rows + at[q & 3]);
-              if (word == a.words - 1) x &= last_mask;
-            }
-            v[b][q >> 2][q & 3] = x;
-          }
-#pragma unroll
-        for (int b = 0; b < AHEAD; ++b) {
-          if (k0 + b >= a.steps || !ok) continue;
-          if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(48, k0 + b, stage); continue; }
-          if (used) {
-            uint4* dst = reinterpret_cast<uint4*>(scales + stage * SCALE_BYTES + part * 1024) + lane;
-            dst[0] = make_uint4(v[b][0][0], v[b][0][1], v[b][0][2], v[b][0][3]);
-            dst[32] = make_uint4(v[b][1][0], v[b][1][1], v[b][1][2], v[b][1][3]);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          }
-          __syncwarp();
-          if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(s.scales + stage)) : "memory");
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      for (int d = 0; d < DEPTH; ++d) {
+        if (left == 0 || !ok) continue;
+        if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(48, now, stage); continue; }
+        if (used[d]) {
+          const uint32_t m0 = now * 2 + 1 == a.words ? last_mask : 0xffffffffu, m1 = now * 2 + 2 == a.words ? last_mask : 0xffffffffu;
+          uint4* dst = reinterpret_cast<uint4*>(scales + stage * SCALE_BYTES + part * 1024) + lane;
+          dst[0] = make_uint4(v[d][0] & m0, v[d][1] & m0, v[d][2] & m0, v[d][3] & m0);
+          dst[32] = make_uint4(v[d][4] & m1, v[d][5] & m1, v[d][6] & m1, v[d][7] & m1);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(s.scales + stage)) : "memory");
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        if (++now == a.steps) now = 0;
+        --left;
+        fetch(d);
       }
     }
   } else {
@@ -456,25 +479,16 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       if (!mbar_wait(s.tfull + acc, acc_phase[acc], abort_flag)) { gave_up(44, acc, 0); break; }
       acc_phase[acc] ^= 1;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int m = w.m0 + (int)me * LANES + sub * 32 + lane;
+      const int m = w.m0 + (int)me * LANES + sub * 32;
       TO* dst = out + (long long)w.j0 * a.ldo + m;
       const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * COLS);
-      for (int c = half * 32; c < w.n; c += 64) {
-        uint32_t v[32];
-        tmem_ld32_issue(t0 + (uint32_t)c, v);
-        tmem_ld_wait(v);
-        if (m < a.N) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < w.n) dst[(long long)(c + j) * a.ldo] = to_out<TO>(__uint_as_float(v[j]));
-        }
-        __syncwarp();
-      }
+      store_columns<TO>(t0, half * 32, w.n, dst, a.ldo, a.N - m, a.boxed, pieces + (warp - 2) * PIECE_BYTES, &mapOut, m, w.j0, 0);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
       acc ^= 1;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the copy engine has read and written all boxes
     if (a.fill) {
       const int first = s.table.bounds[0], last = s.table.bounds[a.off.groups];
       const int rows = first + a.off.rows - last;
@@ -496,7 +510,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
 }
 
 template <int CG, class TO>
-int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
+int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
   auto kernel = product_kernel<CG, TO>;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -512,20 +526,20 @@ int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, co
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)min((long long)(sms / CG), chunks * mb) * CG);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(threads_of<CG>());
   cfg.dynamicSmemBytes = smem_bytes<CG>();
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = CG > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, a);
+  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, o, a);
   return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 
 template <int CG>
-int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const Args& a, cudaStream_t stream) {
-  if (out_type == TYPE_F32) return launch<CG, float>(p, q, qs, a, stream);
-  if (out_type == TYPE_BF16) return launch<CG, __nv_bfloat16>(p, q, qs, a, stream);
-  return launch<CG, __half>(p, q, qs, a, stream);
+int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
+  if (out_type == TYPE_F32) return launch<CG, float>(p, q, qs, o, a, stream);
+  if (out_type == TYPE_BF16) return launch<CG, __nv_bfloat16>(p, q, qs, o, a, stream);
+  return launch<CG, __half>(p, q, qs, o, a, stream);
 }
 
 bool blocks_of(long long rows, int words, long long* n) {
@@ -575,15 +589,16 @@ PCL_API int pcl_mx4_rows(const void* A, const void* sa, const void* B, const voi
   if (out_type < 0 || out_type > 2) return (int)cudaErrorInvalidValue;
   const long long row_bytes = (K + 31) / 32 * 16;
   const bool pair = getenv("PCL_PAIR") ? getenv("PCL_PAIR")[0] == '1' : (rows / COLS + min((long long)groups, rows) / 2) * ((N + LANES - 1) / LANES) >= 2 * 148;
-  CUtensorMap p, q, qs;
+  CUtensorMap p, q, qs, o;
   const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int rc = make_map_3d(&p, t, B, row_bytes, N, groups, row_bytes, row_bytes * N, 128, LANES);
   if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, pair ? Form<2>::Q_ROWS : Form<1>::Q_ROWS);
   if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, SMALL_BOX);
   if (rc) return rc;
   Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
-         N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill};
-  return pair ? launch_as<2>(out_type, p, q, qs, a, stream) : launch_as<1>(out_type, p, q, qs, a, stream);
+         N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false};
+  a.boxed = make_out_map(&o, p, out_type, out, N, rows, 1, ldo, ldo);
+  return pair ? launch_as<2>(out_type, p, q, qs, o, a, stream) : launch_as<1>(out_type, p, q, qs, o, a, stream);
 }
 
 // Copies the status block of these products to `host` and clears it (waits for the stream).

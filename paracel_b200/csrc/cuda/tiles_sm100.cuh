@@ -41,13 +41,14 @@ struct Table {
     if (threadIdx.x == 0) chunks[o.groups] = carry;
   }
 
-  // rows [begin, begin + n) of chunk `c`, in group `e` (which only grows: callers ask for rising chunks)
+  // `step` divides `most`: a chunk is then at most `most` rows, and all but the last of a group's chunks cannot hold all its rows.
+  // Rows [begin, begin + n) of chunk `c`, in group `e` (which only grows: callers ask for rising chunks)
   __device__ __forceinline__ void find(int c, int step, int& e, int& begin, int& n) const {
     while (c >= chunks[e + 1]) ++e;
     const int rows = bounds[e + 1] - bounds[e], parts = chunks[e + 1] - chunks[e];
     const int size = ((rows + parts - 1) / parts + step - 1) / step * step;
     begin = bounds[e] + (c - chunks[e]) * size;
-    n = min(size, bounds[e + 1] - begin);   // at least 1: size <= most, and parts - 1 chunks of `most` do not hold all rows
+    n = min(size, bounds[e + 1] - begin);
   }
 };
 
@@ -172,9 +173,101 @@ __device__ __forceinline__ uint64_t desc_mn_major(uint32_t saddr) {
   return ((uint64_t)hi << 32) | lo;
 }
 
+// 16 lanes x 32 columns of tensor memory: register 4 i + q of thread t holds lane t / 4 + 8 (q / 2), column 8 i + 2 (t mod 4) + q mod 2
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// low half: a, high half: b
+static __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+static __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Where a warp puts 32 columns x 32 lanes of its accumulator for the copy engine: 2 KB, rows of 64 bytes (a column's 32 lanes)
+constexpr int PIECE_BYTES = 2048;
+
+// A warp's part of an accumulator goes to out: column j of [0, n) and the warp's 32 lanes to dst[j * ldo + lane], lanes < `lanes` only.  Columns 32 at a time,
+// first + 0, 64, 128 ..  16-bit results turn around in shared memory (stmatrix) and leave as boxes of 32 rows
+// x 64 bytes, where `boxed` says that the map can take them; what is left of a chunk, and 32-bit results, are stored lane by lane, a row's 32 neighbours at a
+// time.  Stored so throughout, 16-bit results took two thirds as long again as the products of 2048 four-bit values that they came from.
+template <class TO>
+__device__ __forceinline__ void store_columns(uint32_t taddr, int first, int n, TO* dst, long long ldo, int lanes, bool boxed, uint8_t* piece,
+                                              const CUtensorMap* map, int x, int y, int z) {
+  const int lane = threadIdx.x & 31;
+  for (int c = first; c < n; c += 64) {
+    if (sizeof(TO) == 2 && boxed && c + 32 <= n) {
+      uint32_t lo[16], hi[16];
+      tmem_ld_16x32(taddr + (uint32_t)c, lo);
+      tmem_ld_16x32(taddr + (16u << 16) + (uint32_t)c, hi);
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the last box has been read
+      __syncwarp();
+      asm volatile("tcgen05.wait::ld.sync.aligned;"
+                   : "+r"(lo[0]), "+r"(lo[1]), "+r"(lo[2]), "+r"(lo[3]), "+r"(lo[4]), "+r"(lo[5]), "+r"(lo[6]), "+r"(lo[7]),
+                     "+r"(lo[8]), "+r"(lo[9]), "+r"(lo[10]), "+r"(lo[11]), "+r"(lo[12]), "+r"(lo[13]), "+r"(lo[14]), "+r"(lo[15]),
+                     "+r"(hi[0]), "+r"(hi[1]), "+r"(hi[2]), "+r"(hi[3]), "+r"(hi[4]), "+r"(hi[5]), "+r"(hi[6]), "+r"(hi[7]),
+                     "+r"(hi[8]), "+r"(hi[9]), "+r"(hi[10]), "+r"(hi[11]), "+r"(hi[12]), "+r"(hi[13]), "+r"(hi[14]), "+r"(hi[15])
+                   :
+                   : "memory");
+      auto two = [&](const uint32_t* r) { return pack2(__uint_as_float(r[0]), __uint_as_float(r[1]), TO()); };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = 8 * i + (lane & 7);
+        const uint32_t at = smem_u32(piece) + j * 64 + (((lane >> 3) ^ ((j >> 1) & 3)) << 4);
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(two(lo + 4 * i)),
+                     "r"(two(lo + 4 * i + 2)), "r"(two(hi + 4 * i)), "r"(two(hi + 4 * i + 2))
+                     : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && lanes > 0) {
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(piece)),
+                     "r"(x), "r"(y + c), "r"(z)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    } else {
+      uint32_t v[32];
+      tmem_ld32_issue(taddr + (uint32_t)c, v);
+      tmem_ld_wait(v);
+      if (lane < lanes) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c + j < n) dst[(long long)(c + j) * ldo + lane] = pcl_group::to_out<TO>(__uint_as_float(v[j]));
+      }
+    }
+    __syncwarp();
+  }
+}
+template <>
+__device__ __forceinline__ void store_columns<float>(uint32_t taddr, int first, int n, float* dst, long long ldo, int lanes, bool, uint8_t*,
+                                                     const CUtensorMap*, int, int, int) {
+  const int lane = threadIdx.x & 31;
+  for (int c = first; c < n; c += 64) {
+    uint32_t v[32];
+    tmem_ld32_issue(taddr + (uint32_t)c, v);
+    tmem_ld_wait(v);
+    if (lane < lanes) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (c + j < n) dst[(long long)(c + j) * ldo + lane] = __uint_as_float(v[j]);
+    }
+    __syncwarp();
+  }
+}
+
 // map of `depth` matrices [rows x inner]; strides in bytes; box: box_in values x box_rows rows of one matrix.  `inner` and box_in count elements of `type`.
 static inline int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, long long inner, long long rows, long long depth,
-                              long long row_bytes, long long mat_bytes, int box_in, int box_rows) {
+                              long long row_bytes, long long mat_bytes, int box_in, int box_rows,
+                              CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   encode_fn_t enc = get_encode2();
   if (enc == nullptr) return (int)cudaErrorNotSupported;
   cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)depth};
@@ -182,8 +275,18 @@ static inline int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const 
   cuuint32_t box[3] = {(cuuint32_t)box_in, (cuuint32_t)box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(map, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+// The map that store_columns writes through, of `depth` results [rows x inner] of 16 bits; false where its rows do not start at multiples of 16
+// bytes (or the map cannot be made): then `map` becomes a copy of `other`, and is not used.
+static inline bool make_out_map(CUtensorMap* map, const CUtensorMap& other, int out_type, const void* out, long long inner, long long rows, long long depth,
+                                long long ldo, long long ld_mat) {
+  *map = other;
+  if (out_type == pcl_group::TYPE_F32 || ((uintptr_t)out & 15) || (ldo * 2 & 15) || (ld_mat * 2 & 15)) return false;
+  const CUtensorMapDataType t = out_type == pcl_group::TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return make_map_3d(map, t, out, inner, rows, depth, ldo * 2, ld_mat * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B) == 0;
 }
 
 }  // namespace pcl_tiles
