@@ -213,18 +213,18 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const uint64_t dp0 = MODE == NT ? desc_k_major(smem_u32(stages)) : desc_mn_major(smem_u32(stages));
       const uint64_t dq0 = MODE == TN ? desc_mn_major(smem_u32(stages + P_BYTES)) : desc_k_major(smem_u32(stages + P_BYTES));
       int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase[2] = {0, 0};
+      uint32_t phase = 0, acc_phase = 0;   // bit i of acc_phase: accumulator i
       for (long long i = group; i < walk.tiles && ok; i += groups) {
         const Tile w = walk.at(i);
         const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
         if (len <= 0) continue;
-        if (!mbar_wait(s.tempty + acc, acc_phase[acc] ^ 1, abort_flag)) {
+        if (!mbar_wait(s.tempty + acc, (acc_phase >> acc & 1u) ^ 1u, abort_flag)) {
           if (lane == 0) report(&g_status, 0, 42, acc, 0);
           abort_all<CG>(abort_flag, me ^ 1u);
           ok = false;
           break;
         }
-        acc_phase[acc] ^= 1;
+        acc_phase ^= 1u << acc;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
         const uint32_t d = tmem + (uint32_t)(acc * MAX_COLS);
@@ -285,7 +285,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     const int half = (warp - 2) >> 2;         // two warps share a quarter: 32 columns in turn
     TO* out = static_cast<TO*>(a.out);
     int acc = 0;
-    uint32_t acc_phase[2] = {0, 0};
+    uint32_t acc_phase = 0;                   // bit i: accumulator i
     for (long long i = group; i < walk.tiles && ok; i += groups) {
       const Tile w = walk.at(i);
       const int m = w.m0 + (int)me * LANES + sub * 32;
@@ -295,13 +295,13 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
           for (int j = half; j < w.n; j += 2) dst[(long long)j * a.ldo + lane] = to_out<TO>(0.f);
         continue;
       }
-      if (!mbar_wait(s.tfull + acc, acc_phase[acc], abort_flag)) {
+      if (!mbar_wait(s.tfull + acc, acc_phase >> acc & 1u, abort_flag)) {
         if (lane == 0) report(&g_status, 0, 44, acc, 0);
         abort_all<CG>(abort_flag, me ^ 1u);
         ok = false;
         break;
       }
-      acc_phase[acc] ^= 1;
+      acc_phase ^= 1u << acc;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * MAX_COLS);
       store_columns<TO>(t0, half * 32, w.n, dst, a.ldo, a.mdim - m, a.boxed, pieces + (warp - 2) * PIECE_BYTES, &mapOut, m, w.j0, MODE == TN ? w.e : 0);

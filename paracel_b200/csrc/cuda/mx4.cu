@@ -5,7 +5,6 @@
 // half; scales [ceil(K / 128), rows] words of four codes, byte i of word (b, r) is the code of row r's block 4 b + i.
 // A word holds the scales of 128 values, and the words of neighbouring rows are neighbours: a tile of rows finds its
 // scales in one piece wherever it begins.  A code c stands for 2^(c - 127), 255 for NaN.
-#include <stdlib.h>
 #include "tiles_sm100.cuh"
 
 namespace {
@@ -157,11 +156,10 @@ __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
 // into shared memory in that order, and tcgen05.cp spreads them, behind the operands' arrival and ahead of the products.
 //
 // Accumulators have 224 columns, so that two of them leave room for two stages' scales (24 columns each) in the 512 columns of tensor memory.
-// Roles in a CTA: warp 0 loads operands, warp 1 issues products (in the second CTA of a pair it passes on that its scales have come), warps 2-9
-// store, warps 10-12 fetch scales.
+// Roles in a CTA: warp 0 loads operands, warp 1 issues products, warps 2-9 store, warps 10-12 fetch scales.
 using namespace pcl_tiles;
 
-constexpr int COLS = 224;
+constexpr int COLS = 224;                      // of an accumulator
 constexpr int LANES = 128;
 constexpr int BR = 256;                        // values of a row in a stage: 128 bytes
 constexpr int P_BYTES = LANES * 128;
@@ -169,24 +167,15 @@ constexpr int SCALE_BYTES = 3 * 1024;          // P, Q rows 0-127, Q rows 128-25
 constexpr int SCALE_COLS = 24;
 constexpr int SCALE_BUFS = 2;
 constexpr int TMEM_COLS = 512;
-constexpr int MAX_STAGES = 5;
+constexpr int Q_BYTES = COLS * 128;
+constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
+constexpr int STAGES = 4;
 constexpr int EPI_WARPS = 8;
 constexpr int SCALE_WARP = 2 + EPI_WARPS;
-constexpr int RELAY_WARP = SCALE_WARP + 3;     // three, of a pair only
-constexpr int RELAYS = 4;                      // with warp 1 of the second CTA
-template <int CG> constexpr int threads_of() { return 32 * (RELAY_WARP + (CG == 2 ? RELAYS - 1 : 0)); }
+constexpr int THREADS = 32 * (SCALE_WARP + 3);
 constexpr int SMALL_BOX = 32;
 static_assert(2 * COLS + SCALE_BUFS * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
-
-template <int CG>
-struct Form {
-  static constexpr int Q_ROWS = COLS / CG;
-  static constexpr int Q_BYTES = (Q_ROWS + 31) / 32 * 32 * 128;
-  static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
-  static constexpr int STAGES = CG == 2 ? 5 : 4;
-  static constexpr int M = LANES * CG;
-  static_assert(COLS % (16 * CG) == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
-};
+static_assert(COLS % 16 == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
 
 struct Args {
   const uint32_t* sp;   // words of B's scales [words, groups * N]
@@ -199,14 +188,13 @@ struct Args {
 };
 
 struct Shared {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], scales[MAX_STAGES], peer_scales[MAX_STAGES], tfull[2], tempty[2];
+  uint64_t full[STAGES], empty[STAGES], scales[STAGES], tfull[2], tempty[2];
   uint32_t tmem;
   int abort_flag;
   Table table;
 };
 
-template <int CG>
-constexpr int smem_bytes() { return 1024 + Form<CG>::STAGES * (Form<CG>::STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (int)sizeof(Shared); }
+constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (int)sizeof(Shared);
 
 __device__ PclStatus g_status;
 
@@ -215,26 +203,16 @@ __device__ __forceinline__ uint64_t desc_scales(uint32_t saddr) {
   return ((uint64_t)(8u | (1u << 14)) << 32) | ((saddr >> 4) & 0x3FFFu) | (8u << 16);
 }
 
-template <int CG>
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
-  if (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-template <int CG>
 __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
-  if (CG == 2)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
 }
 
 struct Tile {
@@ -242,41 +220,37 @@ struct Tile {
 };
 
 // The tiles of a call, numbered: those that share rows of A are neighbours.
-template <int CG>
 struct Walk {
   const Table& t;
   int mb, e;
   long long tiles;
 
   __device__ Walk(const Args& a, const Table& t_) : t(t_), e(0) {
-    mb = (a.N + Form<CG>::M - 1) / Form<CG>::M;
+    mb = (a.N + LANES - 1) / LANES;
     tiles = (long long)t.chunks[a.off.groups] * mb;
   }
 
   __device__ Tile at(long long i) {   // rising i
     Tile w;
     const long long c = i / mb;
-    w.m0 = (int)(i - c * mb) * Form<CG>::M;
-    t.find((int)c, 16 * CG, e, w.j0, w.n);
+    w.m0 = (int)(i - c * mb) * LANES;
+    t.find((int)c, 16, e, w.j0, w.n);
     w.e = e;
-    w.ncol = (w.n + 16 * CG - 1) / (16 * CG) * (16 * CG);
+    w.ncol = (w.n + 16 - 1) / (16) * (16);
     return w;
   }
 };
 
-template <int CG, class TO>
-__global__ void __launch_bounds__(threads_of<CG>(), 1)
+template <class TO>
+__global__ void __launch_bounds__(THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                const __grid_constant__ CUtensorMap mapQ_small, const __grid_constant__ CUtensorMap mapOut, Args a) {
-  using F = Form<CG>;
-  constexpr int STAGES = F::STAGES, STAGE_BYTES = F::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* scales = stages + STAGES * STAGE_BYTES;
   uint8_t* pieces = scales + STAGES * SCALE_BYTES;
   Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t me = CG == 2 ? cluster_ctarank() : 0;   // 0 leads the pair
   volatile int* abort_flag = &s.abort_flag;
 
   if (warp == 0) {
@@ -284,26 +258,25 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       for (int i = 0; i < STAGES; ++i) {
         mbar_init(s.full + i, 1);
         mbar_init(s.empty + i, 1);
-        mbar_init(s.scales + i, 3);
-        mbar_init(s.peer_scales + i, 1);
+        mbar_init(s.scales + i, 3 * 32);
       }
-      for (int i = 0; i < 2; ++i) { mbar_init(s.tfull + i, 1); mbar_init(s.tempty + i, CG * EPI_WARPS); }
+      for (int i = 0; i < 2; ++i) { mbar_init(s.tfull + i, 1); mbar_init(s.tempty + i, EPI_WARPS); }
       s.abort_flag = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     s.table.build(a.off, COLS, &g_status);
   }
-  if (warp == 1) tmem_alloc<CG>(&s.tmem, TMEM_COLS);
+  if (warp == 1) tmem_alloc<1>(&s.tmem, TMEM_COLS);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  sync_cluster_or_block<CG>();
+  __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s.tmem;
-  const int group = blockIdx.x / CG, groups = gridDim.x / CG;
-  Walk<CG> walk(a, s.table);
+  const int group = blockIdx.x, groups = gridDim.x;
+  Walk walk(a, s.table);
   bool ok = true;
   auto gave_up = [&](int where, int x, int y) {
     if (lane == 0) report(&g_status, 0, where, x, y);
-    abort_all<CG>(abort_flag, me ^ 1u);
+    *abort_flag = 1;
     ok = false;
   };
 
@@ -312,24 +285,21 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     uint32_t phase = 0;
     for (long long i = group; i < walk.tiles && ok; i += groups) {
       const Tile w = walk.at(i);
-      const int mine = w.ncol / CG;
-      const int j = w.j0 + (int)me * mine, m = w.m0 + (int)me * LANES;
-      const bool whole = mine == F::Q_ROWS;
-      const int boxes = whole ? 1 : (mine + SMALL_BOX - 1) / SMALL_BOX;
-      const uint32_t bytes = P_BYTES + (whole ? F::Q_ROWS * 128 : boxes * SMALL_BOX * 128);
+      const bool whole = w.ncol == COLS;
+      const int boxes = whole ? 1 : (w.ncol + SMALL_BOX - 1) / SMALL_BOX;
+      const uint32_t bytes = P_BYTES + (whole ? COLS * 128 : boxes * SMALL_BOX * 128);
       for (int kb = 0; kb < a.steps; ++kb) {
         if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(41, kb, stage); break; }
         if (elect()) {
           const uint32_t sp = smem_u32(stages + stage * STAGE_BYTES), sq = sp + P_BYTES;
-          uint32_t bar = smem_u32(s.full + stage);
-          if (CG == 2) bar = map_to_cta(bar, 0);
-          if (me == 0) mbar_expect_tx(s.full + stage, CG * bytes);
-          tma_load_3d<CG>(sp, &mapP, bar, kb * 128, m, w.e);
+          const uint32_t bar = smem_u32(s.full + stage);
+          mbar_expect_tx(s.full + stage, bytes);
+          tma_load_3d<1>(sp, &mapP, bar, kb * 128, w.m0, w.e);
           if (whole) {
-            tma_load_3d<CG>(sq, &mapQ, bar, kb * 128, j, 0);
+            tma_load_3d<1>(sq, &mapQ, bar, kb * 128, w.j0, 0);
           } else {
             for (int b = 0; b < boxes; ++b)
-              tma_load_3d<CG>(sq + b * SMALL_BOX * 128, &mapQ_small, bar, kb * 128, j + b * SMALL_BOX, 0);
+              tma_load_3d<1>(sq + b * SMALL_BOX * 128, &mapQ_small, bar, kb * 128, w.j0 + b * SMALL_BOX, 0);
           }
         }
         __syncwarp();
@@ -338,35 +308,19 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     }
     if (!ok)
       for (int i = 0; i < 2048; ++i) __nanosleep(1000);   // copies in flight land before the shared memory goes away
-  } else if (CG == 2 && (warp >= RELAY_WARP || (warp == 1 && me != 0))) {
-    // This CTA's scales are in place: tell the leader, whose products read them.  An arrival that releases to the cluster
-    // takes about a microsecond, two stages' products: four warps take the stages in turn.
-    const int mine = warp == 1 ? 0 : warp - RELAY_WARP + 1;
-    int stage = 0, turn = 0;
-    uint32_t phase = 0;
-    for (long long i = group; i < walk.tiles && ok && me != 0; i += groups) {
-      for (int kb = 0; kb < a.steps; ++kb) {
-        if (turn == mine) {
-          if (!mbar_wait(s.scales + stage, phase, abort_flag)) { gave_up(46, kb, stage); break; }
-          if (lane == 0) arrive_cluster(map_to_cta(smem_u32(s.peer_scales + stage), 0));
-        }
-        if (++turn == RELAYS) turn = 0;
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
-      }
-    }
   } else if (warp == 1) {
     // operands E2M1, scales E8M0
-    const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(F::M >> 4) << 24);
+    const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(LANES >> 4) << 24);
     const uint64_t dp0 = desc_k_major(smem_u32(stages)), ds0 = desc_scales(smem_u32(scales));
     int stage = 0, acc = 0, buf = 0;
-    uint32_t phase = 0, acc_phase[2] = {0, 0};
+    uint32_t phase = 0, acc_phase = 0;   // bit i of acc_phase: accumulator i
     int old_stage = 0;                       // the stage before the last: its products use the scales' other half
     uint32_t old_phase = 0;
     long long done = 0;
     for (long long i = group; i < walk.tiles && ok; i += groups) {
       const Tile w = walk.at(i);
-      if (!mbar_wait(s.tempty + acc, acc_phase[acc] ^ 1, abort_flag)) { gave_up(42, acc, 0); break; }
-      acc_phase[acc] ^= 1;
+      if (!mbar_wait(s.tempty + acc, (acc_phase >> acc & 1u) ^ 1u, abort_flag)) { gave_up(42, acc, 0); break; }
+      acc_phase ^= 1u << acc;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
       const uint32_t d = tmem + (uint32_t)(acc * COLS);
@@ -377,30 +331,31 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
           if (!mbar_wait(s.empty + old_stage, old_phase, abort_flag)) { gave_up(47, kb, old_stage); break; }
           if (++old_stage == STAGES) { old_stage = 0; old_phase ^= 1; }
         }
-        if (!wait_full(s.full + stage, phase, abort_flag) || !mbar_wait(s.scales + stage, phase, abort_flag) ||
-            (CG == 2 && !wait_full(s.peer_scales + stage, phase, abort_flag))) {
+        if (!mbar_wait(s.full + stage, phase, abort_flag) || !mbar_wait(s.scales + stage, phase, abort_flag)) {
           gave_up(43, kb, stage);
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (elect()) {
+          // the scales were copied for other threads, and have arrived
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           const uint32_t sf = tmem + (uint32_t)(2 * COLS + buf * SCALE_COLS);
           const uint64_t ds = ds0 + (uint32_t)(stage * SCALE_BYTES) / 16;
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
-            copy_scales<CG>(sf + v * 4, ds + v * 32);
-            copy_scales<CG>(sf + 8 + v * 8, ds + 64 + v * 32);
-            if (wide) copy_scales<CG>(sf + 12 + v * 8, ds + 128 + v * 32);
+            copy_scales(sf + v * 4, ds + v * 32);
+            copy_scales(sf + 8 + v * 8, ds + 64 + v * 32);
+            if (wide) copy_scales(sf + 12 + v * 8, ds + 128 + v * 32);
           }
           const uint64_t dp = dp0 + (uint32_t)(stage * STAGE_BYTES) / 16;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t id = (uint32_t)(k & 1) * 2;   // codes 0, 1 or 2, 3 of a word
-            umma_mxf4<CG>(d, dp + 2 * k, dp + P_BYTES / 16 + 2 * k, idesc | (id << 4) | (id << 29), sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8,
+            umma_mxf4(d, dp + 2 * k, dp + P_BYTES / 16 + 2 * k, idesc | (id << 4) | (id << 29), sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8,
                           (kb > 0 || k > 0) ? 1u : 0u);
           }
-          commit<CG>(smem_u32(s.empty + stage));
-          if (kb + 1 == a.steps) commit<CG>(smem_u32(s.tfull + acc));
+          commit<1>(smem_u32(s.empty + stage));
+          if (kb + 1 == a.steps) commit<1>(smem_u32(s.tfull + acc));
         }
         __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -411,81 +366,60 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     }
   } else if (warp >= SCALE_WARP) {
     const int part = warp - SCALE_WARP;      // 0: P, 1 and 2: Q
-    const uint32_t* src = part == 0 ? a.sp : a.sq;
     const long long rows = part == 0 ? (long long)a.off.groups * a.N : a.off.rows;
-    // codes of the last word that no block has
-    const int spare = a.words * 4 - a.blocks;
-    const uint32_t last_mask = 0xffffffffu >> (8 * spare);
-    // the words of a stage are asked for DEPTH stages before they are stored
-    constexpr int DEPTH = 3;
-    uint32_t v[DEPTH][8];
-    bool used[DEPTH];
-    long long at[4];
-    long long tile = group;
-    int kb = a.steps;
-    bool in_use = false;
-    auto fetch = [&](int d) {
-      if (kb == a.steps) {
-        if (tile >= walk.tiles) return;
-        const Tile w = walk.at(tile);
-        tile += groups;
-        kb = 0;
-        in_use = part < 2 || w.ncol > 128;
-        const long long r0 = part == 0 ? (long long)w.e * a.N + w.m0 + (long long)me * LANES : (long long)w.j0 + (part - 1) * 128;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) at[q] = min(r0 + lane + 32 * q, rows - 1);   // rows of no tile: any scales do
-      }
-      used[d] = in_use;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int word = kb * 2 + (q >> 2);
-        v[d][q] = in_use && word < a.words ? __ldg(src + word * rows + at[q & 3]) : 0u;
-      }
-      ++kb;
-    };
-    long long left = walk.tiles > group ? ((walk.tiles - group + groups - 1) / groups) * a.steps : 0;
-    int stage = 0, now = 0;
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(part == 0 ? a.sp : a.sq);
+    // Of 128 rows a lane copies 8 q + lane mod 8 + 32 (lane / 8), q = 0 .. 3: together the lanes read whole sectors and write
+    // different banks.  (Words that went through registers took 73 of 311 thousand cycles of 4096 x 8192^2, more the further ahead they were
+    // read: the copies are neither waited for nor unrolled.)
+    const int row = (lane & 7) + 32 * (lane >> 3);
+    const uint32_t dst0 = smem_u32(scales) + part * 1024 + (lane & 7) * 16 + (lane >> 3) * 4;
+    const int last_bytes = 4 - (a.words * 4 - a.blocks);   // codes of the last word; those that no block has become zero
+    int stage = 0;
     uint32_t phase = 0;
+    for (long long i = group; i < walk.tiles && ok; i += groups) {
+      const Tile w = walk.at(i);
+      const bool used = part < 2 || w.ncol > 128;
+      const long long r0 = part == 0 ? (long long)w.e * a.N + w.m0 : (long long)w.j0 + (part - 1) * 128;
+      const uint8_t* at[4];
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) fetch(d);
-    while (left > 0 && ok) {
+      for (int q = 0; q < 4; ++q) at[q] = src + 4 * min(r0 + row + 8 * q, rows - 1);   // rows of no tile: any scales do
+      for (int kb = 0; kb < a.steps; ++kb) {
+        if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(48, kb, stage); break; }
+        if (used) {
+          const uint32_t dst = dst0 + stage * SCALE_BYTES;
 #pragma unroll
-      for (int d = 0; d < DEPTH; ++d) {
-        if (left == 0 || !ok) continue;
-        if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(48, now, stage); continue; }
-        if (used[d]) {
-          const uint32_t m0 = now * 2 + 1 == a.words ? last_mask : 0xffffffffu, m1 = now * 2 + 2 == a.words ? last_mask : 0xffffffffu;
-          uint4* dst = reinterpret_cast<uint4*>(scales + stage * SCALE_BYTES + part * 1024) + lane;
-          dst[0] = make_uint4(v[d][0] & m0, v[d][1] & m0, v[d][2] & m0, v[d][3] & m0);
-          dst[32] = make_uint4(v[d][4] & m1, v[d][5] & m1, v[d][6] & m1, v[d][7] & m1);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          for (int v = 0; v < 2; ++v) {
+            const int word = kb * 2 + v;
+            const int bytes = word + 1 < a.words ? 4 : word + 1 == a.words ? last_bytes : 0;
+            const long long off = word < a.words ? word * rows * 4 : 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + v * 512 + q * 128), "l"(at[q] + off), "r"(bytes) : "memory");
+          }
         }
-        __syncwarp();
-        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(s.scales + stage)) : "memory");
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(s.scales + stage)) : "memory");
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        if (++now == a.steps) now = 0;
-        --left;
-        fetch(d);
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     const int sub = warp & 3;                 // the quarter of the tensor memory's lanes that this warp can read
     const int half = (warp - 2) >> 2;         // two warps share a quarter: 32 columns in turn
     TO* out = static_cast<TO*>(a.out);
     int acc = 0;
-    uint32_t acc_phase[2] = {0, 0};
+    uint32_t acc_phase = 0;                   // bit i: accumulator i
     for (long long i = group; i < walk.tiles && ok; i += groups) {
       const Tile w = walk.at(i);
-      if (!mbar_wait(s.tfull + acc, acc_phase[acc], abort_flag)) { gave_up(44, acc, 0); break; }
-      acc_phase[acc] ^= 1;
+      if (!mbar_wait(s.tfull + acc, acc_phase >> acc & 1u, abort_flag)) { gave_up(44, acc, 0); break; }
+      acc_phase ^= 1u << acc;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int m = w.m0 + (int)me * LANES + sub * 32;
+      const int m = w.m0 + sub * 32;
       TO* dst = out + (long long)w.j0 * a.ldo + m;
       const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * COLS);
       store_columns<TO>(t0, half * 32, w.n, dst, a.ldo, a.N - m, a.boxed, pieces + (warp - 2) * PIECE_BYTES, &mapOut, m, w.j0, 0);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
+      if (lane == 0) mbar_arrive_cluster(smem_u32(s.tempty + acc));
       acc ^= 1;
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the copy engine has read and written all boxes
@@ -499,47 +433,27 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     }
   }
 
-  // nobody leaves while the pair still reads this CTA's shared memory or signals its barriers
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncwarp();
-  sync_cluster_or_block<CG>();
+  __syncthreads();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    tmem_free<CG>(tmem, TMEM_COLS);
+    tmem_free<1>(tmem, TMEM_COLS);
   }
 }
 
-template <int CG, class TO>
+template <class TO>
 int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  auto kernel = product_kernel<CG, TO>;
+  auto kernel = product_kernel<TO>;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<CG>());
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) return (int)e;
-  const long long mb = (a.N + Form<CG>::M - 1) / Form<CG>::M;
+  const long long mb = (a.N + LANES - 1) / LANES;
   const long long chunks = a.off.rows / COLS + min(a.off.groups, a.off.rows);
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)min((long long)(sms / CG), chunks * mb) * CG);
-  cfg.blockDim = dim3(threads_of<CG>());
-  cfg.dynamicSmemBytes = smem_bytes<CG>();
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, o, a);
-  return e != cudaSuccess ? (int)e : pcl_last_error();
-}
-
-template <int CG>
-int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  if (out_type == TYPE_F32) return launch<CG, float>(p, q, qs, o, a, stream);
-  if (out_type == TYPE_BF16) return launch<CG, __nv_bfloat16>(p, q, qs, o, a, stream);
-  return launch<CG, __half>(p, q, qs, o, a, stream);
+  kernel<<<(unsigned)min((long long)sms, chunks * mb), THREADS, SMEM_BYTES, stream>>>(p, q, qs, o, a);
+  return pcl_last_error();
 }
 
 bool blocks_of(long long rows, int words, long long* n) {
@@ -588,17 +502,18 @@ PCL_API int pcl_mx4_rows(const void* A, const void* sa, const void* B, const voi
   if (rows == 0) return 0;
   if (out_type < 0 || out_type > 2) return (int)cudaErrorInvalidValue;
   const long long row_bytes = (K + 31) / 32 * 16;
-  const bool pair = getenv("PCL_PAIR") ? getenv("PCL_PAIR")[0] == '1' : (rows / COLS + min((long long)groups, rows) / 2) * ((N + LANES - 1) / LANES) >= 2 * 148;
   CUtensorMap p, q, qs, o;
   const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int rc = make_map_3d(&p, t, B, row_bytes, N, groups, row_bytes, row_bytes * N, 128, LANES);
-  if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, pair ? Form<2>::Q_ROWS : Form<1>::Q_ROWS);
+  if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, COLS);
   if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, SMALL_BOX);
   if (rc) return rc;
   Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
          N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false};
   a.boxed = make_out_map(&o, p, out_type, out, N, rows, 1, ldo, ldo);
-  return pair ? launch_as<2>(out_type, p, q, qs, o, a, stream) : launch_as<1>(out_type, p, q, qs, o, a, stream);
+  if (out_type == TYPE_F32) return launch<float>(p, q, qs, o, a, stream);
+  if (out_type == TYPE_BF16) return launch<__nv_bfloat16>(p, q, qs, o, a, stream);
+  return launch<__half>(p, q, qs, o, a, stream);
 }
 
 // Copies the status block of these products to `host` and clears it (waits for the stream).
