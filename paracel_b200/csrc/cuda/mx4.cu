@@ -463,9 +463,7 @@ bool blocks_of(long long rows, int words, long long* n) {
 
 }  // namespace
 
-// x [rows, K] of in_type (0 fp32, 1 bf16, 2 fp16), rows ldx values apart
-PCL_API int pcl_mx4_quantize(const void* x, long long ldx, int in_type, void* data, void* scales, long long rows, int K,
-                             cudaStream_t stream) {
+static int quantize(const void* x, long long ldx, int in_type, void* data, void* scales, long long rows, int K, cudaStream_t stream) {
   QuantArgs a{x, ldx, static_cast<uint32_t*>(data), static_cast<uint32_t*>(scales), rows, K, (K + 127) / 128, 0};
   const int size = in_type == TYPE_F32 ? 4 : 2;
   a.vec = ((uintptr_t)x & 15) == 0 && (ldx * size & 15) == 0;
@@ -476,6 +474,12 @@ PCL_API int pcl_mx4_quantize(const void* x, long long ldx, int in_type, void* da
   else if (in_type == TYPE_BF16) quantize_kernel<__nv_bfloat16><<<(unsigned)n, QTHREADS, 0, stream>>>(a);
   else quantize_kernel<__half><<<(unsigned)n, QTHREADS, 0, stream>>>(a);
   return pcl_last_error();
+}
+
+// x [rows, K] of in_type (0 fp32, 1 bf16, 2 fp16), rows ldx values apart
+PCL_API int pcl_mx4_quantize(const void* x, long long ldx, int in_type, void* data, void* scales, long long rows, int K,
+                             cudaStream_t stream) {
+  return quantize(x, ldx, in_type, data, scales, rows, K, stream);
 }
 
 PCL_API int pcl_mx4_dequantize(const void* data, const void* scales, void* out, long long ldo, int out_type, long long rows,
@@ -492,15 +496,20 @@ PCL_API int pcl_mx4_dequantize(const void* data, const void* scales, void* out, 
   return pcl_last_error();
 }
 
-// A [rows, K], B [groups * N, K], both in four bits -> out [rows, N] of out_type; offsets null: one group of all rows
-PCL_API int pcl_mx4_rows(const void* A, const void* sa, const void* B, const void* sb, const void* offsets, int off64, void* out,
-                         long long ldo, int out_type, long long rows, int groups, int N, int K, int fill,
+// A [rows, K], B [groups * N, K], both in four bits -> out [rows, N] of out_type; offsets null: one group of all rows.  x_type 0, 1, 2: A and
+// sa are room for x [rows, K] (fp32, bf16, fp16, rows ldx values apart), which is quantised into them first; -1: they are the operand.
+PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void* sa, const void* B, const void* sb, const void* offsets,
+                         int off64, void* out, long long ldo, int out_type, long long rows, int groups, int N, int K, int fill,
                          cudaStream_t stream) {
   if (rows < 0 || rows >= (1ll << 31) - 512 || groups < 1 || groups > MAX_GROUPS || N < 1 || K < 1 ||
       (long long)groups * N >= (1ll << 31) - 512)
     return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   if (out_type < 0 || out_type > 2) return (int)cudaErrorInvalidValue;
+  if (x_type >= 0) {
+    const int rc = quantize(x, ldx, x_type, A, sa, rows, K, stream);
+    if (rc) return rc;
+  }
   const long long row_bytes = (K + 31) / 32 * 16;
   CUtensorMap p, q, qs, o;
   const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;

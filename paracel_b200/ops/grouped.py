@@ -26,6 +26,7 @@ from . import _lib
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_GROUPS = 1024
+MAX_ROWS = (1 << 31) - 512
 
 
 def check_status(device=None) -> None:
@@ -35,11 +36,9 @@ def check_status(device=None) -> None:
 
 
 def read_status(entry: str, device, what: str) -> None:
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    if dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
+    index = None if device is None else torch.device(device).index
     host = torch.zeros(4, dtype=torch.int64)
-    _lib.call_on(dev, entry, host)
+    _lib.call_on(torch.cuda.current_device() if index is None else index, entry, host.data_ptr())
     _lib.raise_status(host, what)
 
 
@@ -120,11 +119,12 @@ def _check_sizes(rows: int, **sizes) -> None:
     for name, v in sizes.items():
         if not 1 <= v < 1 << 30:
             raise ValueError(f"{name} must be 1 to 2^30 - 1, got {v}")
-    if rows >= (1 << 31) - 512:
+    if rows >= MAX_ROWS:
         raise ValueError(f"at most 2^31 - 513 rows, got {rows}")
 
 
-def _rows(mode: int, X, W, offsets, out, out_dtype):
+def _check_rows(mode: int, X, W, offsets, out, dtype) -> None:
+    """Raise for what is wrong with the operands of ``_rows``."""
     name = "X" if mode == 0 else "dY"
     check_operand(X, name, 2)
     check_operand(W, "W", 3, X.dtype)
@@ -135,23 +135,54 @@ def _rows(mode: int, X, W, offsets, out, out_dtype):
     given, cols = (K, N) if mode == 0 else (N, K)
     if X.shape[1] != given:
         raise ValueError(f"{name} must have {given} columns, got {X.shape[1]}")
-    T = X.shape[0]
-    _check_sizes(T, N=N, K=K)
-    dtype = result_type(out, out_dtype, X.dtype, (X.dtype, torch.float32))
-    check_out(out, (T, cols), dtype)
-    device = check_devices(**{name: X, "W": W, "offsets": offsets, "out": out})
+    _check_sizes(X.shape[0], N=N, K=K)
+    dtype = result_type(out, dtype, X.dtype, (X.dtype, torch.float32))
+    check_out(out, (X.shape[0], cols), dtype)
+    check_devices(**{name: X, "W": W, "offsets": offsets, "out": out})
+
+
+def _rows(mode: int, X, W, offsets, out, out_dtype):
+    # a call is a few microseconds on the device: everything is looked at once here, and what is wrong is found out above
+    xs, ws, dtype, device = X.shape, W.shape, X.dtype, X.get_device()
+    if not (len(xs) == 2 and len(ws) == 3 and (dtype == torch.bfloat16 or dtype == torch.float16) and W.dtype == dtype
+            and xs[1] == ws[2 - mode] and 0 < ws[1] < 1 << 30 and 0 < ws[2] < 1 << 30 and xs[0] < MAX_ROWS
+            and offsets.dim() == 1 and offsets.shape[0] == ws[0] + 1 and 0 < ws[0] <= MAX_GROUPS
+            and (offsets.dtype == torch.int32 or offsets.dtype == torch.int64) and offsets.is_contiguous()
+            and device >= 0 and W.get_device() == device and offsets.get_device() == device
+            and out is None and (out_dtype is None or out_dtype == dtype or out_dtype == torch.float32)):
+        _check_rows(mode, X, W, offsets, out, out_dtype)
+    T, (E, N, K) = xs[0], ws
+    cols = ws[1 + mode]
     fill = out is None
     if fill:
-        out = torch.empty(T, cols, dtype=dtype, device=device)
+        out = torch.empty((T, cols), dtype=dtype if out_dtype is None else out_dtype, device=X.device)
     if T == 0:
         return out
-    X, W = aligned(X), aligned(W)
-    ldx = stride_of(X, 0, (given + 7) // 8 * 8)
-    ws_n = stride_of(W, 1, (K + 7) // 8 * 8)
-    ws_e = stride_of(W, 0, ws_n * N)
-    _lib.call_on(device, "pcl_grouped_rows", mode, TYPES[X.dtype], TYPES[dtype], X, ldx, W, ws_e, ws_n, offsets,
-                 int(offsets.dtype == torch.int64), out, stride_of(out, 0, cols), T, E, N, K, int(fill))
+    x, w = X.data_ptr(), W.data_ptr()
+    ldx, unit = X.stride()
+    ws_e, ws_n, w_unit = W.stride()
+    if x & 15 or w & 15 or unit != 1 or w_unit != 1 or ldx & 7 or ws_n & 7 or ws_e & 7 or not (ldx and ws_n and ws_e):
+        X, W = aligned(X), aligned(W)
+        x, w = X.data_ptr(), W.data_ptr()
+        ldx = stride_of(X, 0, (xs[1] + 7) // 8 * 8)
+        ws_n = stride_of(W, 1, (K + 7) // 8 * 8)
+        ws_e = stride_of(W, 0, ws_n * N)
+    _lib.call_on(device, "pcl_grouped_rows", mode, TYPES[dtype], TYPES[out.dtype], x, ldx, w, ws_e, ws_n, offsets.data_ptr(),
+                 offsets.dtype == torch.int64, out.data_ptr(), out.stride(0), T, E, N, K, fill)
     return out
+
+
+def _check_tn(dY, X, offsets, out, dtype) -> None:
+    """Raise for what is wrong with the operands of ``grouped_tn``."""
+    check_operand(X, "X", 2)
+    check_operand(dY, "dY", 2, X.dtype)
+    E = check_offsets(offsets)
+    if dY.shape[0] != X.shape[0]:
+        raise ValueError(f"dY has {dY.shape[0]} rows, X {X.shape[0]}")
+    _check_sizes(X.shape[0], N=dY.shape[1], K=X.shape[1])
+    dtype = result_type(out, dtype, X.dtype, (X.dtype, torch.float32))
+    check_out(out, (E, dY.shape[1], X.shape[1]), dtype)
+    check_devices(dY=dY, X=X, offsets=offsets, out=out)
 
 
 def grouped_nt(X: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -175,21 +206,26 @@ def grouped_tn(dY: torch.Tensor, X: torch.Tensor, offsets: torch.Tensor, out: Op
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``dW [E, N, K]``, ``dW[e]`` the sum of ``dy[t] x[t]^T`` over the rows of group ``e`` (zero where it has none): the
     gradient of ``grouped_nt`` with respect to ``W``.  ``dY [T, N]``, ``X [T, K]``; ``out`` must be contiguous."""
-    check_operand(X, "X", 2)
-    check_operand(dY, "dY", 2, X.dtype)
-    E = check_offsets(offsets)
-    if dY.shape[0] != X.shape[0]:
-        raise ValueError(f"dY has {dY.shape[0]} rows, X {X.shape[0]}")
-    T, N, K = X.shape[0], dY.shape[1], X.shape[1]
-    _check_sizes(T, N=N, K=K)
-    dtype = result_type(out, out_dtype, X.dtype, (X.dtype, torch.float32))
-    check_out(out, (E, N, K), dtype)
-    device = check_devices(dY=dY, X=X, offsets=offsets, out=out)
+    xs, ys, dtype, device = X.shape, dY.shape, X.dtype, X.get_device()
+    if not (len(xs) == 2 and len(ys) == 2 and (dtype == torch.bfloat16 or dtype == torch.float16) and dY.dtype == dtype
+            and xs[0] == ys[0] and xs[0] < MAX_ROWS and 0 < xs[1] < 1 << 30 and 0 < ys[1] < 1 << 30
+            and offsets.dim() == 1 and 1 < offsets.shape[0] <= MAX_GROUPS + 1
+            and (offsets.dtype == torch.int32 or offsets.dtype == torch.int64) and offsets.is_contiguous()
+            and device >= 0 and dY.get_device() == device and offsets.get_device() == device
+            and out is None and (out_dtype is None or out_dtype == dtype or out_dtype == torch.float32)):
+        _check_tn(dY, X, offsets, out, out_dtype)
+    T, K, N, E = xs[0], xs[1], ys[1], offsets.shape[0] - 1
     if out is None:
-        out = torch.empty(E, N, K, dtype=dtype, device=device)
+        out = torch.empty((E, N, K), dtype=dtype if out_dtype is None else out_dtype, device=X.device)
     if T == 0:
         return out.zero_()
-    X, dY = aligned(X), aligned(dY)
-    _lib.call_on(device, "pcl_grouped_tn", TYPES[X.dtype], TYPES[dtype], dY, stride_of(dY, 0, (N + 7) // 8 * 8), X,
-                 stride_of(X, 0, (K + 7) // 8 * 8), offsets, int(offsets.dtype == torch.int64), out, T, E, N, K)
+    x, y = X.data_ptr(), dY.data_ptr()
+    ldx, unit = X.stride()
+    ldy, y_unit = dY.stride()
+    if x & 15 or y & 15 or unit != 1 or y_unit != 1 or ldx & 7 or ldy & 7 or not (ldx and ldy):
+        X, dY = aligned(X), aligned(dY)
+        x, y = X.data_ptr(), dY.data_ptr()
+        ldx, ldy = stride_of(X, 0, (K + 7) // 8 * 8), stride_of(dY, 0, (N + 7) // 8 * 8)
+    _lib.call_on(device, "pcl_grouped_tn", TYPES[dtype], TYPES[out.dtype], y, ldy, x, ldx, offsets.data_ptr(),
+                 offsets.dtype == torch.int64, out.data_ptr(), T, E, N, K)
     return out

@@ -18,7 +18,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .grouped import TYPES, check_devices, check_offsets, check_out, read_status, result_type, stride_of
+from .grouped import MAX_GROUPS, MAX_ROWS, TYPES, check_devices, check_offsets, check_out, read_status, result_type
 
 BLOCK = 32
 
@@ -33,6 +33,16 @@ class Mx4Matrix:
     __slots__ = ("data", "scales", "cols")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, cols: int):
+        ds, ss = data.shape, scales.shape
+        if not (0 < cols < 1 << 30 and data.dtype == torch.uint8 and scales.dtype == torch.uint8 and len(ds) == 2 and len(ss) == 3
+                and ds[1] == (cols + 31) // 32 * 16 and ss[0] == (cols + 127) // 128 and ss[1] == ds[0] and ss[2] == 4
+                and ds[0] < MAX_ROWS and data.is_contiguous() and scales.is_contiguous()
+                and not (data.data_ptr() | scales.data_ptr()) & 15 and data.get_device() == scales.get_device()):
+            self._refuse(data, scales, cols)
+        self.data, self.scales, self.cols = data, scales, cols
+
+    @staticmethod
+    def _refuse(data, scales, cols):
         if not 1 <= cols < 1 << 30:
             raise ValueError(f"cols must be 1 to 2^30 - 1, got {cols}")
         for t, name in ((data, "data"), (scales, "scales")):
@@ -44,9 +54,7 @@ class Mx4Matrix:
             raise ValueError(f"scales must be {((cols + 127) // 128, data.shape[0], 4)}, got {tuple(scales.shape)}")
         if scales.device != data.device:
             raise ValueError(f"scales must be on {data.device}, got {scales.device}")
-        if data.shape[0] >= (1 << 31) - 512:
-            raise ValueError(f"at most 2^31 - 513 rows, got {data.shape[0]}")
-        self.data, self.scales, self.cols = data, scales, cols
+        raise ValueError(f"at most 2^31 - 513 rows, got {data.shape[0]}")
 
     @property
     def rows(self) -> int:
@@ -79,20 +87,28 @@ def mx4_quantize(X: torch.Tensor) -> Mx4Matrix:
     K = X.shape[-1]
     if not 1 <= K < 1 << 30:
         raise ValueError(f"X must have 1 to 2^30 - 1 columns, got {K}")
-    check_devices(X=X)
+    device = X.get_device()
+    if device < 0:
+        check_devices(X=X)
     if X.dim() == 3:
         X = X.reshape(-1, K)
-    if (K > 1 and X.stride(1) != 1) or (X.shape[0] > 1 and X.stride(0) < 0):
-        X = X.contiguous()
+    X, ldx = _row_stride(X)
     rows = X.shape[0]
-    # both parts in one allocation: the data's size is a multiple of 16 bytes
-    words = (K + 127) // 128
-    n = rows * ((K + 31) // 32) * 16
-    buf = torch.empty(n + words * rows * 4, dtype=torch.uint8, device=X.device)
-    q = Mx4Matrix(buf[:n].view(rows, -1) if rows else buf.view(0, (K + 31) // 32 * 16), buf[n:].view(words, rows, 4), K)
+    data = torch.empty((rows, (K + 31) // 32 * 16), dtype=torch.uint8, device=X.device)
+    scales = torch.empty(((K + 127) // 128, rows, 4), dtype=torch.uint8, device=X.device)
+    q = Mx4Matrix(data, scales, K)
     if rows:
-        _lib.call_on(X.device, "pcl_mx4_quantize", X, stride_of(X, 0, K), TYPES[X.dtype], q.data, q.scales, rows, K)
+        _lib.call_on(device, "pcl_mx4_quantize", X.data_ptr(), ldx, TYPES[X.dtype], data.data_ptr(), scales.data_ptr(), rows, K)
     return q
+
+
+def _row_stride(X: torch.Tensor):
+    """(``X``, or a copy of it, with contiguous rows; values from one row to the next)"""
+    ldx, unit = X.stride()
+    if unit != 1 and X.shape[1] > 1:
+        X = X.contiguous()
+        ldx = X.shape[1]
+    return X, ldx
 
 
 def mx4_dequantize(q: Mx4Matrix, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -100,17 +116,19 @@ def mx4_dequantize(q: Mx4Matrix, dtype: torch.dtype = torch.float32, out: Option
     either); float16 rounds."""
     if dtype not in TYPES:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
-    check_out(out, (q.rows, q.cols), dtype)
-    check_devices(q=q, out=out)
+    if out is not None or not q.data.is_cuda:
+        check_out(out, (q.rows, q.cols), dtype)
+        check_devices(q=q, out=out)
     if out is None:
-        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
+        out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.data.device)
     if q.rows:
-        _lib.call_on(q.device, "pcl_mx4_dequantize", q.data, q.scales, out, stride_of(out, 0, q.cols), TYPES[dtype], q.rows,
-                     q.cols)
+        _lib.call_on(q.data.get_device(), "pcl_mx4_dequantize", q.data.data_ptr(), q.scales.data_ptr(), out.data_ptr(), out.stride(0),
+                     TYPES[dtype], q.rows, q.cols)
     return out
 
 
-def _product(A, B: Mx4Matrix, offsets, out, out_dtype):
+def _check_product(A, B, offsets, out, dtype) -> None:
+    """Raise for what is wrong with the operands of ``_product``."""
     if not isinstance(B, Mx4Matrix):
         raise ValueError("B must be an Mx4Matrix: quantise it once with mx4_quantize")
     packed = isinstance(A, Mx4Matrix)
@@ -122,20 +140,45 @@ def _product(A, B: Mx4Matrix, offsets, out, out_dtype):
     groups = 1 if offsets is None else check_offsets(offsets)
     if B.rows == 0 or B.rows % groups:
         raise ValueError(f"B must have the same number of rows for each of the {groups} groups, at least one, got {B.rows}")
-    N = B.rows // groups
-    dtype = result_type(out, out_dtype, torch.float32 if packed else A.dtype, tuple(TYPES))
-    check_out(out, (T, N), dtype)
-    device = check_devices(A=A, B=B, offsets=offsets, out=out)
+    if T >= MAX_ROWS:
+        raise ValueError(f"at most 2^31 - 513 rows, got {T}")
+    dtype = result_type(out, dtype, torch.float32 if packed else A.dtype, tuple(TYPES))
+    check_out(out, (T, B.rows // groups), dtype)
+    check_devices(A=A, B=B, offsets=offsets, out=out)
+
+
+def _product(A, B: Mx4Matrix, offsets, out, out_dtype):
+    packed = isinstance(A, Mx4Matrix)
+    if not isinstance(B, Mx4Matrix):
+        _check_product(A, B, offsets, out, out_dtype)
+    data = B.data
+    K, rows, device = B.cols, data.shape[0], data.get_device()
+    shape = (A.data.shape[0], A.cols) if packed else A.shape
+    dtype = out_dtype if out_dtype is not None else out.dtype if out is not None else torch.float32 if packed else A.dtype
+    groups = 1 if offsets is None else offsets.numel() - 1
+    if not (len(shape) == 2 and shape[1] == K and (packed or A.dtype in TYPES) and dtype in TYPES and out is None and shape[0] < MAX_ROWS
+            and 0 < groups <= rows and rows % groups == 0 and device >= 0 and (A.data if packed else A).get_device() == device
+            and (offsets is None or offsets.dim() == 1 and groups <= MAX_GROUPS and offsets.get_device() == device
+                 and (offsets.dtype == torch.int32 or offsets.dtype == torch.int64) and offsets.is_contiguous())):
+        _check_product(A, B, offsets, out, out_dtype)
+    T, N = shape[0], rows // groups
     fill = out is None
     if fill:
-        out = torch.empty(T, N, dtype=dtype, device=device)
+        out = torch.empty((T, N), dtype=dtype, device=data.device)
     if T == 0:
         return out
-    if not packed:
-        A = mx4_quantize(A)
-    _lib.call_on(device, "pcl_mx4_rows", A.data, A.scales, B.data, B.scales, offsets,
-                 int(offsets is not None and offsets.dtype == torch.int64), out, stride_of(out, 0, N), TYPES[dtype], T, groups, N,
-                 cols, int(fill))
+    if packed:
+        x, ldx, kind, a, sa = 0, 0, -1, A.data.data_ptr(), A.scales.data_ptr()
+    else:
+        # A in four bits, for the length of the call
+        A, ldx = _row_stride(A)
+        size = T * ((K + 31) // 32 * 16)
+        work = torch.empty(size + T * ((K + 127) // 128 * 4), dtype=torch.uint8, device=data.device)
+        x, kind, a = A.data_ptr(), TYPES[A.dtype], work.data_ptr()
+        sa = a + size
+    _lib.call_on(device, "pcl_mx4_rows", x, ldx, kind, a, sa, data.data_ptr(), B.scales.data_ptr(),
+                 None if offsets is None else offsets.data_ptr(), offsets is not None and offsets.dtype == torch.int64, out.data_ptr(),
+                 out.stride(0), TYPES[dtype], T, groups, N, K, fill)
     return out
 
 
