@@ -28,19 +28,21 @@ constexpr int BR = 64;                         // reduction steps of a stage
 constexpr int LANES = 128;
 constexpr int P_BYTES = LANES * BR * 2;
 constexpr int OPERAND_BYTES = 192 * 1024;
-constexpr int MAX_STAGES = 6;
+constexpr int MAX_STAGES = 8;
 constexpr int EPI_WARPS = 8;
 constexpr int FIX_WARP = 2 + EPI_WARPS;
 // tn has a warp more: it clears what a group's last stage holds of the next group
 constexpr int threads_of(int mode) { return 64 + 32 * EPI_WARPS + (mode == 2 ? 32 : 0); }
 // CG: CTAs that work on a tile, one or a pair on neighbouring SMs (tcgen05 cta_group::2); each of a pair holds its 128 m and half the j
-template <int CG>
+// COLS: columns of an accumulator, the most j of a tile
+template <int CG, int COLS>
 struct Form {
-  static constexpr int Q_BYTES = MAX_COLS / CG * BR * 2;
+  static constexpr int Q_BYTES = COLS / CG * BR * 2;
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
   static constexpr int STAGES = OPERAND_BYTES / STAGE_BYTES;
   static constexpr int M = LANES * CG;   // m of a tile
-  static_assert(MAX_COLS % (16 * CG) == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
+  static_assert(STAGES <= MAX_STAGES, "barriers");
+  static_assert(COLS % (16 * CG) == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
 };
 constexpr int SMALL_BOX = 32;                  // rows of Q that are loaded at a time where a chunk is not full
 
@@ -70,7 +72,7 @@ struct Tile {
 };
 
 // The tiles of a call, numbered: those that share rows of Q are neighbours.
-template <int MODE, int CG>
+template <int MODE, int CG, int COLS>
 struct Walk {
   const Args& a;
   const Table& t;
@@ -78,10 +80,10 @@ struct Walk {
   long long tiles;
 
   __device__ Walk(const Args& a_, const Table& t_) : a(a_), t(t_), e(0) {
-    mb = (a.mdim + Form<CG>::M - 1) / Form<CG>::M;
+    mb = (a.mdim + Form<CG, COLS>::M - 1) / Form<CG, COLS>::M;
     jparts = jsize = 0;
     if (MODE == TN) {
-      jparts = (a.jdim + MAX_COLS - 1) / MAX_COLS;
+      jparts = (a.jdim + COLS - 1) / COLS;
       jsize = ((a.jdim + jparts - 1) / jparts + 16 * CG - 1) / (16 * CG) * (16 * CG);
       tiles = (long long)a.off.groups * jparts * mb;
     } else {
@@ -92,7 +94,7 @@ struct Walk {
   __device__ Tile at(long long i) {   // rising i
     Tile w;
     const long long c = i / mb;
-    w.m0 = (int)(i - c * mb) * Form<CG>::M;
+    w.m0 = (int)(i - c * mb) * Form<CG, COLS>::M;
     if (MODE == TN) {
       w.e = (int)(c / jparts);
       w.j0 = (int)(c - (long long)w.e * jparts) * jsize;
@@ -110,11 +112,11 @@ struct Walk {
   }
 };
 
-template <int MODE, int CG, class TO>
+template <int MODE, int CG, int COLS, class TO>
 __global__ void __launch_bounds__(threads_of(MODE), 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                const __grid_constant__ CUtensorMap mapQ_small, const __grid_constant__ CUtensorMap mapOut, Args a) {
-  using F = Form<CG>;
+  using F = Form<CG, COLS>;
   constexpr int Q_BYTES = F::Q_BYTES, STAGE_BYTES = F::STAGE_BYTES, STAGES = F::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -131,15 +133,15 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       s.abort_flag = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    s.table.build(a.off, MAX_COLS, &g_status);
+    s.table.build(a.off, COLS, &g_status);
   }
-  if (warp == 1) tmem_alloc<CG>(&s.tmem, 2 * MAX_COLS);
+  if (warp == 1) tmem_alloc<CG>(&s.tmem, 2 * COLS);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   sync_cluster_or_block<CG>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s.tmem;
   const int group = blockIdx.x / CG, groups = gridDim.x / CG;
-  Walk<MODE, CG> walk(a, s.table);
+  Walk<MODE, CG, COLS> walk(a, s.table);
   bool ok = true;
 
   if (warp == 0) {
@@ -150,7 +152,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const int steps = (w.r1 - w.r0 + BR - 1) / BR;
       const int mine = w.ncol / CG;
       const int j = w.j0 + (int)me * mine;
-      const bool whole = MODE != TN && mine == MAX_COLS / CG;
+      const bool whole = MODE != TN && mine == COLS / CG;
       const int boxes = MODE == TN ? (mine + 63) / 64 : whole ? 1 : (mine + SMALL_BOX - 1) / SMALL_BOX;
       const uint32_t q_bytes = MODE == TN ? boxes * 8192u : whole ? (uint32_t)Q_BYTES : boxes * (uint32_t)(SMALL_BOX * BR * 2);
       for (int kb = 0; kb < steps; ++kb) {
@@ -227,7 +229,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         acc_phase ^= 1u << acc;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
-        const uint32_t d = tmem + (uint32_t)(acc * MAX_COLS);
+        const uint32_t d = tmem + (uint32_t)(acc * COLS);
         for (int r = 0; r < steps; ++r) {
           if (!wait_full(s.full + stage, phase, abort_flag)) {
             if (lane == 0) report(&g_status, 0, 43, r, stage);
@@ -303,7 +305,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       }
       acc_phase ^= 1u << acc;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * MAX_COLS);
+      const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * COLS);
       store_columns<TO>(t0, half * 32, w.n, dst, a.ldo, a.mdim - m, a.boxed, pieces + (warp - 2) * PIECE_BYTES, &mapOut, m, w.j0, MODE == TN ? w.e : 0);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -327,21 +329,21 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   sync_cluster_or_block<CG>();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    tmem_free<CG>(tmem, 2 * MAX_COLS);
+    tmem_free<CG>(tmem, 2 * COLS);
   }
 }
 
-template <int MODE, int CG, class TO>
+template <int MODE, int CG, int COLS, class TO>
 int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  auto kernel = product_kernel<MODE, CG, TO>;
+  auto kernel = product_kernel<MODE, CG, COLS, TO>;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) return (int)e;
-  const long long mb = (a.mdim + Form<CG>::M - 1) / Form<CG>::M;
-  const long long chunks = MODE == TN ? (long long)a.off.groups * ((a.jdim + MAX_COLS - 1) / MAX_COLS)
-                                      : a.off.rows / MAX_COLS + min(a.off.groups, a.off.rows);
+  const long long mb = (a.mdim + Form<CG, COLS>::M - 1) / Form<CG, COLS>::M;
+  const long long chunks = MODE == TN ? (long long)a.off.groups * ((a.jdim + COLS - 1) / COLS)
+                                      : a.off.rows / COLS + min(a.off.groups, a.off.rows);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -358,16 +360,34 @@ int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, co
   return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 
-template <int MODE, int CG>
+template <int MODE, int CG, int COLS>
 int launch_as(int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  if (out_type == TYPE_F32) return launch<MODE, CG, float>(p, q, qs, o, a, stream);
+  if (out_type == TYPE_F32) return launch<MODE, CG, COLS, float>(p, q, qs, o, a, stream);
   if (out_type != in_type) return (int)cudaErrorInvalidValue;
-  return in_type == TYPE_BF16 ? launch<MODE, CG, __nv_bfloat16>(p, q, qs, o, a, stream) : launch<MODE, CG, __half>(p, q, qs, o, a, stream);
+  return in_type == TYPE_BF16 ? launch<MODE, CG, COLS, __nv_bfloat16>(p, q, qs, o, a, stream) : launch<MODE, CG, COLS, __half>(p, q, qs, o, a, stream);
 }
 
 // Whether pairs of CTAs take the tiles.  A pair loads a third fewer bytes for its 256 x 256 tile than two CTAs for theirs, but there are half as
 // many tiles: below two for every SM single CTAs spread better.
 bool use_pairs(long long chunks, int mdim) { return chunks * ((mdim + LANES - 1) / LANES) >= 2 * 148; }
+
+// The forms of nt and nn.  FEW: groups of few rows stream their matrices once, and what counts is how many bytes are on their way: a stage
+// without room for 256 rows of Q is 24 KB instead of 48, and there are eight instead of four.
+enum RowsForm { FEW, SINGLE, PAIR };
+constexpr int FEW_COLS = 64;
+
+RowsForm rows_form(long long rows, int groups, int mdim) {
+  if (rows <= FEW_COLS || rows / groups <= FEW_COLS / 4) return FEW;
+  return use_pairs(rows / MAX_COLS + min((long long)groups, rows) / 2, mdim) ? PAIR : SINGLE;
+}
+
+template <int MODE>
+int launch_form(RowsForm form, int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o,
+                const Args& a, cudaStream_t stream) {
+  if (form == FEW) return launch_as<MODE, 1, FEW_COLS>(in_type, out_type, p, q, qs, o, a, stream);
+  if (form == SINGLE) return launch_as<MODE, 1, MAX_COLS>(in_type, out_type, p, q, qs, o, a, stream);
+  return launch_as<MODE, 2, MAX_COLS>(in_type, out_type, p, q, qs, o, a, stream);
+}
 
 bool sizes_ok(int in_type, long long rows, int groups, int N, int K) {
   return (in_type == TYPE_BF16 || in_type == TYPE_F16) && rows >= 0 && rows < (1ll << 31) - 512 && groups >= 1 &&
@@ -387,16 +407,16 @@ PCL_API int pcl_grouped_rows(int mode, int in_type, int out_type, const void* X,
   if (rows == 0) return 0;
   const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int red = mode == 0 ? K : N;
-  const bool pair = use_pairs(rows / MAX_COLS + min((long long)groups, rows) / 2, mode == 0 ? N : K);
+  const RowsForm form = rows_form(rows, groups, mode == 0 ? N : K);
   CUtensorMap p, q, qs, o;
   int rc = make_map_3d(&p, t, W, K, N, groups, ws_n * 2, ws_e * 2, 64, mode == 0 ? LANES : BR);
-  if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, pair ? MAX_COLS / 2 : MAX_COLS);
+  if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, form == FEW ? FEW_COLS : form == PAIR ? MAX_COLS / 2 : MAX_COLS);
   if (rc == 0) rc = make_map_3d(&qs, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SMALL_BOX);
   if (rc) return rc;
   Args a{out, ldo, Offsets{offsets, off64, groups, (int)rows}, mode == 0 ? N : K, 0, red, in_type == TYPE_BF16 ? 1u : 0u, fill, false};
   a.boxed = make_out_map(&o, p, out_type, out, a.mdim, rows, 1, ldo, ldo);
-  if (mode == 0) return pair ? launch_as<NT, 2>(in_type, out_type, p, q, qs, o, a, stream) : launch_as<NT, 1>(in_type, out_type, p, q, qs, o, a, stream);
-  return pair ? launch_as<NN, 2>(in_type, out_type, p, q, qs, o, a, stream) : launch_as<NN, 1>(in_type, out_type, p, q, qs, o, a, stream);
+  if (mode == 0) return launch_form<NT>(form, in_type, out_type, p, q, qs, o, a, stream);
+  return launch_form<NN>(form, in_type, out_type, p, q, qs, o, a, stream);
 }
 
 // out [groups, N, K] (contiguous): every matrix is written, zeros where a group has no row
@@ -411,8 +431,8 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
   if (rc) return rc;
   Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0, false};
   a.boxed = make_out_map(&o, p, out_type, out, K, N, groups, K, (long long)N * K);
-  return use_pairs((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K) ? launch_as<TN, 2>(in_type, out_type, p, q, q, o, a, stream)
-                                                                            : launch_as<TN, 1>(in_type, out_type, p, q, q, o, a, stream);
+  return use_pairs((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K) ? launch_as<TN, 2, 256>(in_type, out_type, p, q, q, o, a, stream)
+                                                                            : launch_as<TN, 1, 256>(in_type, out_type, p, q, q, o, a, stream);
 }
 
 // Copies the status block of the grouped products to `host` and clears it (waits for the stream).

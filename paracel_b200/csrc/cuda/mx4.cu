@@ -155,27 +155,35 @@ __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
 // such words of every row.  Three warps fetch them (a word of neighbouring rows is one line), one for P, two for Q, put them
 // into shared memory in that order, and tcgen05.cp spreads them, behind the operands' arrival and ahead of the products.
 //
-// Accumulators have 224 columns, so that two of them leave room for two stages' scales (24 columns each) in the 512 columns of tensor memory.
+// Every stage has 24 columns of tensor memory for its scales, which are free when the stage is; two accumulators of at most 208 columns and
+// four stages fill the 512.  (224 columns and scales for two stages: a stage's copy then waits for the products of the stage before the last,
+// and 1000 cycles go by per stage, 270 us for 8192^3.)
 // Roles in a CTA: warp 0 loads operands, warp 1 issues products, warps 2-9 store, warps 10-12 fetch scales.
 using namespace pcl_tiles;
 
-constexpr int COLS = 224;                      // of an accumulator
 constexpr int LANES = 128;
 constexpr int BR = 256;                        // values of a row in a stage: 128 bytes
 constexpr int P_BYTES = LANES * 128;
 constexpr int SCALE_BYTES = 3 * 1024;          // P, Q rows 0-127, Q rows 128-255: two blocks of 512 bytes each
 constexpr int SCALE_COLS = 24;
-constexpr int SCALE_BUFS = 2;
 constexpr int TMEM_COLS = 512;
-constexpr int Q_BYTES = COLS * 128;
-constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
-constexpr int STAGES = 4;
+constexpr int MAX_STAGES = 7;
 constexpr int EPI_WARPS = 8;
 constexpr int SCALE_WARP = 2 + EPI_WARPS;
 constexpr int THREADS = 32 * (SCALE_WARP + 3);
 constexpr int SMALL_BOX = 32;
-static_assert(2 * COLS + SCALE_BUFS * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
-static_assert(COLS % 16 == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
+
+// COLS: columns of an accumulator, the most rows of A in a tile.  64 of them leave room for seven stages of 27 KB, 208 for four of 45.
+template <int COLS>
+struct Form {
+  static constexpr int STAGE_BYTES = P_BYTES + COLS * 128;
+  static constexpr int STAGES = 192 * 1024 / (STAGE_BYTES + SCALE_BYTES);
+  static constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES;   // and Shared
+  static_assert(STAGES <= MAX_STAGES, "barriers");
+  static_assert(2 * COLS + STAGES * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
+  static_assert(COLS % 16 == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
+};
+constexpr int FEW_COLS = 64, MANY_COLS = 208;
 
 struct Args {
   const uint32_t* sp;   // words of B's scales [words, groups * N]
@@ -188,13 +196,12 @@ struct Args {
 };
 
 struct Shared {
-  uint64_t full[STAGES], empty[STAGES], scales[STAGES], tfull[2], tempty[2];
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], scales[MAX_STAGES], tfull[2], tempty[2];
   uint32_t tmem;
   int abort_flag;
   Table table;
 };
 
-constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (int)sizeof(Shared);
 
 __device__ PclStatus g_status;
 
@@ -241,10 +248,11 @@ struct Walk {
   }
 };
 
-template <class TO>
+template <int COLS, class TO>
 __global__ void __launch_bounds__(THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                const __grid_constant__ CUtensorMap mapQ_small, const __grid_constant__ CUtensorMap mapOut, Args a) {
+  constexpr int STAGES = Form<COLS>::STAGES, STAGE_BYTES = Form<COLS>::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* scales = stages + STAGES * STAGE_BYTES;
@@ -312,11 +320,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     // operands E2M1, scales E8M0
     const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(LANES >> 4) << 24);
     const uint64_t dp0 = desc_k_major(smem_u32(stages)), ds0 = desc_scales(smem_u32(scales));
-    int stage = 0, acc = 0, buf = 0;
+    int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;   // bit i of acc_phase: accumulator i
-    int old_stage = 0;                       // the stage before the last: its products use the scales' other half
-    uint32_t old_phase = 0;
-    long long done = 0;
     for (long long i = group; i < walk.tiles && ok; i += groups) {
       const Tile w = walk.at(i);
       if (!mbar_wait(s.tempty + acc, (acc_phase >> acc & 1u) ^ 1u, abort_flag)) { gave_up(42, acc, 0); break; }
@@ -326,11 +331,6 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const uint32_t d = tmem + (uint32_t)(acc * COLS);
       const bool wide = w.ncol > 128;
       for (int kb = 0; kb < a.steps; ++kb) {
-        // the products of two stages ago have read the scales that are overwritten now
-        if (done >= SCALE_BUFS) {
-          if (!mbar_wait(s.empty + old_stage, old_phase, abort_flag)) { gave_up(47, kb, old_stage); break; }
-          if (++old_stage == STAGES) { old_stage = 0; old_phase ^= 1; }
-        }
         if (!mbar_wait(s.full + stage, phase, abort_flag) || !mbar_wait(s.scales + stage, phase, abort_flag)) {
           gave_up(43, kb, stage);
           break;
@@ -339,7 +339,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         if (elect()) {
           // the scales were copied for other threads, and have arrived
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          const uint32_t sf = tmem + (uint32_t)(2 * COLS + buf * SCALE_COLS);
+          const uint32_t sf = tmem + (uint32_t)(2 * COLS + stage * SCALE_COLS);
           const uint64_t ds = ds0 + (uint32_t)(stage * SCALE_BYTES) / 16;
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
@@ -359,8 +359,6 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         }
         __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        if (++buf == SCALE_BUFS) buf = 0;
-        ++done;
       }
       acc ^= 1;
     }
@@ -442,18 +440,26 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   }
 }
 
-template <class TO>
+template <int COLS, class TO>
 int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  auto kernel = product_kernel<TO>;
+  auto kernel = product_kernel<COLS, TO>;
+  constexpr int smem = Form<COLS>::SMEM_BYTES + (int)sizeof(Shared);
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
   const long long mb = (a.N + LANES - 1) / LANES;
   const long long chunks = a.off.rows / COLS + min(a.off.groups, a.off.rows);
-  kernel<<<(unsigned)min((long long)sms, chunks * mb), THREADS, SMEM_BYTES, stream>>>(p, q, qs, o, a);
+  kernel<<<(unsigned)min((long long)sms, chunks * mb), THREADS, smem, stream>>>(p, q, qs, o, a);
   return pcl_last_error();
+}
+
+template <int COLS>
+int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
+  if (out_type == TYPE_F32) return launch<COLS, float>(p, q, qs, o, a, stream);
+  if (out_type == TYPE_BF16) return launch<COLS, __nv_bfloat16>(p, q, qs, o, a, stream);
+  return launch<COLS, __half>(p, q, qs, o, a, stream);
 }
 
 bool blocks_of(long long rows, int words, long long* n) {
@@ -511,18 +517,18 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
     if (rc) return rc;
   }
   const long long row_bytes = (K + 31) / 32 * 16;
+  // groups of few rows stream their matrices, and what counts is how many bytes are on their way
+  const bool few = rows <= FEW_COLS || rows / groups <= FEW_COLS / 4;
   CUtensorMap p, q, qs, o;
   const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int rc = make_map_3d(&p, t, B, row_bytes, N, groups, row_bytes, row_bytes * N, 128, LANES);
-  if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, COLS);
+  if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, few ? FEW_COLS : MANY_COLS);
   if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, SMALL_BOX);
   if (rc) return rc;
   Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
          N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false};
   a.boxed = make_out_map(&o, p, out_type, out, N, rows, 1, ldo, ldo);
-  if (out_type == TYPE_F32) return launch<float>(p, q, qs, o, a, stream);
-  if (out_type == TYPE_BF16) return launch<__nv_bfloat16>(p, q, qs, o, a, stream);
-  return launch<__half>(p, q, qs, o, a, stream);
+  return few ? launch_as<FEW_COLS>(out_type, p, q, qs, o, a, stream) : launch_as<MANY_COLS>(out_type, p, q, qs, o, a, stream);
 }
 
 // Copies the status block of these products to `host` and clears it (waits for the stream).
