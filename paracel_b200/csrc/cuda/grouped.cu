@@ -377,8 +377,9 @@ enum RowsForm { FEW, SINGLE, PAIR };
 constexpr int FEW_COLS = 64;
 
 RowsForm rows_form(long long rows, int groups, int mdim) {
-  if (rows <= FEW_COLS || rows / groups <= FEW_COLS / 4) return FEW;
-  return use_pairs(rows / MAX_COLS + min((long long)groups, rows) / 2, mdim) ? PAIR : SINGLE;
+  const long long chunks = rows / MAX_COLS + min((long long)groups, rows) / 2;
+  if (rows <= FEW_COLS || rows / groups <= FEW_COLS / 4 || chunks * ((mdim + LANES - 1) / LANES) < 148) return FEW;
+  return use_pairs(chunks, mdim) ? PAIR : SINGLE;
 }
 
 template <int MODE>

@@ -518,7 +518,8 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
   }
   const long long row_bytes = (K + 31) / 32 * 16;
   // groups of few rows stream their matrices, and what counts is how many bytes are on their way
-  const bool few = rows <= FEW_COLS || rows / groups <= FEW_COLS / 4;
+  const bool few = rows <= FEW_COLS || rows / groups <= FEW_COLS / 4 ||
+                   (rows / MANY_COLS + min((long long)groups, rows) / 2) * ((N + LANES - 1) / LANES) < 148;
   CUtensorMap p, q, qs, o;
   const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int rc = make_map_3d(&p, t, B, row_bytes, N, groups, row_bytes, row_bytes * N, 128, LANES);
