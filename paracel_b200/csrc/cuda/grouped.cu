@@ -35,11 +35,12 @@ constexpr int FIX_WARP = 2 + EPI_WARPS;
 constexpr int threads_of(int mode) { return 64 + 32 * EPI_WARPS + (mode == 2 ? 32 : 0); }
 // CG: CTAs that work on a tile, one or a pair on neighbouring SMs (tcgen05 cta_group::2); each of a pair holds its 128 m and half the j
 // COLS: columns of an accumulator, the most j of a tile
-template <int CG, int COLS>
+// SPLIT: a cluster shares a tile's reduction (COLS 64 only)
+template <int CG, int COLS, bool SPLIT>
 struct Form {
   static constexpr int Q_BYTES = COLS / CG * BR * 2;
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
-  static constexpr int STAGES = OPERAND_BYTES / STAGE_BYTES;
+  static constexpr int STAGES = (OPERAND_BYTES - (SPLIT ? INBOX_BYTES : 0)) / STAGE_BYTES;
   static constexpr int M = LANES * CG;   // m of a tile
   static_assert(STAGES <= MAX_STAGES, "barriers");
   static_assert(COLS % (16 * CG) == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
@@ -72,82 +73,96 @@ struct Tile {
 };
 
 // The tiles of a call, numbered: those that share rows of Q are neighbours.
-template <int MODE, int CG, int COLS>
+template <int MODE, int CG, int COLS, bool SPLIT>
 struct Walk {
   const Args& a;
   const Table& t;
-  int mb, jparts, jsize, e;
-  long long tiles;
+  int mb, jparts, jsize, chunks;
 
-  __device__ Walk(const Args& a_, const Table& t_) : a(a_), t(t_), e(0) {
-    mb = (a.mdim + Form<CG, COLS>::M - 1) / Form<CG, COLS>::M;
+  __device__ Walk(const Args& a_, const Table& t_) : a(a_), t(t_) {
+    mb = (a.mdim + Form<CG, COLS, SPLIT>::M - 1) / Form<CG, COLS, SPLIT>::M;
     jparts = jsize = 0;
     if (MODE == TN) {
       jparts = (a.jdim + COLS - 1) / COLS;
       jsize = ((a.jdim + jparts - 1) / jparts + 16 * CG - 1) / (16 * CG) * (16 * CG);
-      tiles = (long long)a.off.groups * jparts * mb;
+      chunks = a.off.groups * jparts;
     } else {
-      tiles = (long long)t.chunks[a.off.groups] * mb;
+      chunks = t.chunks[a.off.groups];
     }
   }
 
-  __device__ Tile at(long long i) {   // rising i
+  __device__ Counter start(int first, int step) const { return Counter(first, step, mb); }
+  __device__ bool has(const Counter& i) const { return i.c < chunks; }
+
+  __device__ Tile at(const Counter& i) const {
     Tile w;
-    const long long c = i / mb;
-    w.m0 = (int)(i - c * mb) * Form<CG, COLS>::M;
+    w.m0 = i.m * Form<CG, COLS, SPLIT>::M;
     if (MODE == TN) {
-      w.e = (int)(c / jparts);
-      w.j0 = (int)(c - (long long)w.e * jparts) * jsize;
+      w.e = i.c / jparts;
+      w.j0 = (i.c - w.e * jparts) * jsize;
       w.n = min(jsize, a.jdim - w.j0);
       w.r0 = t.bounds[w.e];
       w.r1 = t.bounds[w.e + 1];
     } else {
-      t.find((int)c, 16 * CG, e, w.j0, w.n);
-      w.e = e;
+      t.find(a.off.groups, i.c, 16 * CG, w.e, w.j0, w.n);
       w.r0 = 0;
       w.r1 = a.red;
+      if (SPLIT) {   // this CTA's stages
+        const int steps = (a.red + BR - 1) / BR, rank = (int)cluster_ctarank(), parts = (int)cluster_size();
+        w.r0 = rank * steps / parts * BR;
+        w.r1 = min(a.red, (rank + 1) * steps / parts * BR);
+      }
     }
     w.ncol = (w.n + 16 * CG - 1) / (16 * CG) * (16 * CG);
     return w;
   }
 };
 
-template <int MODE, int CG, int COLS, class TO>
+template <int MODE, int CG, int COLS, bool SPLIT, class TO>
 __global__ void __launch_bounds__(threads_of(MODE), 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                const __grid_constant__ CUtensorMap mapQ_small, const __grid_constant__ CUtensorMap mapOut, Args a) {
-  using F = Form<CG, COLS>;
+  using F = Form<CG, COLS, SPLIT>;
   constexpr int Q_BYTES = F::Q_BYTES, STAGE_BYTES = F::STAGE_BYTES, STAGES = F::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* pieces = stages + OPERAND_BYTES;
   Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES);
+  float* inbox = reinterpret_cast<float*>(stages + STAGES * STAGE_BYTES);   // SPLIT
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t me = CG == 2 ? cluster_ctarank() : 0;   // 0 leads the pair
   volatile int* abort_flag = &s.abort_flag;
 
   if (warp == 0) {
-    if (lane == 0) {
-      for (int i = 0; i < STAGES; ++i) { mbar_init(s.full + i, MODE == TN ? CG : 1); mbar_init(s.empty + i, 1); mbar_init(s.tail + i, 1); }
-      for (int i = 0; i < 2; ++i) { mbar_init(s.tfull + i, 1); mbar_init(s.tempty + i, CG * EPI_WARPS); }
-      s.abort_flag = 0;
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (lane < STAGES) {
+      mbar_init(s.full + lane, MODE == TN ? CG : 1);
+      mbar_init(s.empty + lane, 1);
+      mbar_init(s.tail + lane, 1);
     }
-    s.table.build(a.off, COLS, &g_status);
+    if (lane < 2) { mbar_init(s.tfull + lane, 1); mbar_init(s.tempty + lane, CG * EPI_WARPS); }
+    if (lane == 0) s.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == 2 && lane == 0) {
+    for (const CUtensorMap* m : {&mapP, &mapQ, &mapQ_small, &mapOut}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+  }
+  load_bounds(a.off, s.table.bounds, &g_status);
+  __syncthreads();
+  if (warp == 0) s.table.build(a.off.groups, COLS, &g_status);
   if (warp == 1) tmem_alloc<CG>(&s.tmem, 2 * COLS);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  sync_cluster_or_block<CG>();
+  sync_cluster_or_block<CG == 2 || SPLIT>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s.tmem;
-  const int group = blockIdx.x / CG, groups = gridDim.x / CG;
-  Walk<MODE, CG, COLS> walk(a, s.table);
+  const int share = SPLIT ? (int)cluster_size() : CG;
+  const int group = blockIdx.x / share, groups = gridDim.x / share;
+  const Walk<MODE, CG, COLS, SPLIT> walk(a, s.table);
   bool ok = true;
 
   if (warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
+    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
       const int steps = (w.r1 - w.r0 + BR - 1) / BR;
       const int mine = w.ncol / CG;
@@ -216,7 +231,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const uint64_t dq0 = MODE == TN ? desc_mn_major(smem_u32(stages + P_BYTES)) : desc_k_major(smem_u32(stages + P_BYTES));
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;   // bit i of acc_phase: accumulator i
-      for (long long i = group; i < walk.tiles && ok; i += groups) {
+      bool ready = false;                  // the next stage has arrived
+      for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
         const Tile w = walk.at(i);
         const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
         if (len <= 0) continue;
@@ -231,12 +247,14 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
         const uint32_t d = tmem + (uint32_t)(acc * COLS);
         for (int r = 0; r < steps; ++r) {
-          if (!wait_full(s.full + stage, phase, abort_flag)) {
+          if (!ready && !wait_full(s.full + stage, phase, abort_flag)) {
             if (lane == 0) report(&g_status, 0, 43, r, stage);
             abort_all<CG>(abort_flag, me ^ 1u);
             ok = false;
             break;
           }
+          const int next = stage + 1 == STAGES ? 0 : stage + 1;
+          ready = has_passed(s.full + next, phase ^ (uint32_t)(next == 0));
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (elect()) {
             const uint64_t dp = dp0 + (uint32_t)(stage * STAGE_BYTES) / 16, dq = dq0 + (uint32_t)(stage * STAGE_BYTES) / 16;
@@ -258,7 +276,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   } else if (MODE == TN && warp == FIX_WARP) {
     int stage = 0;
     uint32_t phases = 0;   // bit i: parity of the next wait on tail[i]
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
+    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
       const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
       const int last = (stage + steps + STAGES - 1) % STAGES;
@@ -288,7 +306,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     TO* out = static_cast<TO*>(a.out);
     int acc = 0;
     uint32_t acc_phase = 0;                   // bit i: accumulator i
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
+    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
       const int m = w.m0 + (int)me * LANES + sub * 32;
       TO* dst = out + (MODE == TN ? ((long long)w.e * a.jdim + w.j0) * a.ldo : (long long)w.j0 * a.ldo) + m;
@@ -306,6 +324,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       acc_phase ^= 1u << acc;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * COLS);
+      if (SPLIT) {   // the cluster has this one tile
+        send_columns(t0, sub, half * 32, w.n, inbox, cluster_ctarank(), columns_of_part(w.n, share));
+        continue;
+      }
       store_columns<TO>(t0, half * 32, w.n, dst, a.ldo, a.mdim - m, a.boxed, pieces + (warp - 2) * PIECE_BYTES, &mapOut, m, w.j0, MODE == TN ? w.e : 0);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -323,48 +345,55 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     }
   }
 
-  // nobody leaves while the pair still reads this CTA's shared memory or signals its barriers
+  // Nobody leaves while the pair still reads this CTA's shared memory or signals its barriers; the parts of a split tile are in their inboxes
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncwarp();
-  sync_cluster_or_block<CG>();
+  sync_cluster_or_block<CG == 2 || SPLIT>();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     tmem_free<CG>(tmem, 2 * COLS);
   }
+  if (SPLIT && warp >= 2 && walk.has(walk.start(group, groups))) {
+    const Tile w = walk.at(walk.start(group, groups));
+    add_up<TO>(inbox, w.n, columns_of_part(w.n, share), cluster_ctarank(), share, 64, 32 * EPI_WARPS, static_cast<TO*>(a.out) + (long long)w.j0 * a.ldo + w.m0,
+               a.ldo, a.mdim - w.m0);
+  }
 }
 
-template <int MODE, int CG, int COLS, class TO>
-int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  auto kernel = product_kernel<MODE, CG, COLS, TO>;
+template <int MODE, int CG, int COLS, bool SPLIT, class TO>
+int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, int parts, cudaStream_t stream) {
+  auto kernel = product_kernel<MODE, CG, COLS, SPLIT, TO>;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) return (int)e;
-  const long long mb = (a.mdim + Form<CG, COLS>::M - 1) / Form<CG, COLS>::M;
+  const long long mb = (a.mdim + Form<CG, COLS, SPLIT>::M - 1) / Form<CG, COLS, SPLIT>::M;
   const long long chunks = MODE == TN ? (long long)a.off.groups * ((a.jdim + COLS - 1) / COLS)
-                                      : a.off.rows / COLS + min(a.off.groups, a.off.rows);
+                                      : most_chunks(a.off.rows, a.off.groups, COLS);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.x = SPLIT ? parts : CG;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)min((long long)(sms / CG), chunks * mb) * CG);
+  // a cluster that shares a tile has no other
+  cfg.gridDim = dim3(SPLIT ? (unsigned)(chunks * mb) * parts : (unsigned)min((long long)(sms / CG), chunks * mb) * CG);
   cfg.blockDim = dim3(threads_of(MODE));
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
+  cfg.numAttrs = CG > 1 || SPLIT ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, o, a);
   return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 
-template <int MODE, int CG, int COLS>
-int launch_as(int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  if (out_type == TYPE_F32) return launch<MODE, CG, COLS, float>(p, q, qs, o, a, stream);
+template <int MODE, int CG, int COLS, bool SPLIT>
+int launch_as(int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, int parts,
+              cudaStream_t stream) {
+  if (out_type == TYPE_F32) return launch<MODE, CG, COLS, SPLIT, float>(p, q, qs, o, a, parts, stream);
   if (out_type != in_type) return (int)cudaErrorInvalidValue;
-  return in_type == TYPE_BF16 ? launch<MODE, CG, COLS, __nv_bfloat16>(p, q, qs, o, a, stream) : launch<MODE, CG, COLS, __half>(p, q, qs, o, a, stream);
+  return in_type == TYPE_BF16 ? launch<MODE, CG, COLS, SPLIT, __nv_bfloat16>(p, q, qs, o, a, parts, stream) : launch<MODE, CG, COLS, SPLIT, __half>(p, q, qs, o, a, parts, stream);
 }
 
 // Whether pairs of CTAs take the tiles.  A pair loads a third fewer bytes for its 256 x 256 tile than two CTAs for theirs, but there are half as
@@ -385,9 +414,12 @@ RowsForm rows_form(long long rows, int groups, int mdim) {
 template <int MODE>
 int launch_form(RowsForm form, int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o,
                 const Args& a, cudaStream_t stream) {
-  if (form == FEW) return launch_as<MODE, 1, FEW_COLS>(in_type, out_type, p, q, qs, o, a, stream);
-  if (form == SINGLE) return launch_as<MODE, 1, MAX_COLS>(in_type, out_type, p, q, qs, o, a, stream);
-  return launch_as<MODE, 2, MAX_COLS>(in_type, out_type, p, q, qs, o, a, stream);
+  if (form == SINGLE) return launch_as<MODE, 1, MAX_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
+  if (form == PAIR) return launch_as<MODE, 2, MAX_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
+  const long long tiles = most_chunks(a.off.rows, a.off.groups, FEW_COLS) * ((a.mdim + LANES - 1) / LANES);
+  const int parts = parts_of(tiles, (a.red + BR - 1) / BR, 148);
+  return parts > 1 ? launch_as<MODE, 1, FEW_COLS, true>(in_type, out_type, p, q, qs, o, a, parts, stream)
+                   : launch_as<MODE, 1, FEW_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
 }
 
 bool sizes_ok(int in_type, long long rows, int groups, int N, int K) {
@@ -432,8 +464,8 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
   if (rc) return rc;
   Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0, false};
   a.boxed = make_out_map(&o, p, out_type, out, K, N, groups, K, (long long)N * K);
-  return use_pairs((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K) ? launch_as<TN, 2, 256>(in_type, out_type, p, q, q, o, a, stream)
-                                                                            : launch_as<TN, 1, 256>(in_type, out_type, p, q, q, o, a, stream);
+  return use_pairs((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K) ? launch_as<TN, 2, MAX_COLS, false>(in_type, out_type, p, q, q, o, a, 1, stream)
+                                                                            : launch_as<TN, 1, MAX_COLS, false>(in_type, out_type, p, q, q, o, a, 1, stream);
 }
 
 // Copies the status block of the grouped products to `host` and clears it (waits for the stream).

@@ -25,28 +25,13 @@ struct Offsets {
   }
 };
 
-// bounds[0..groups] in shared memory, by the first warp; every thread of the block calls this and
-// synchronises behind it.  Bounds are taken ascending and inside the tensor whatever the array holds
-// (each is at least the one before it), so that no row is outside or in two groups; the first one that had to be moved
-// goes into the status block.
+// bounds[0..groups] in shared memory as they come, inside the tensor; every thread of the block calls this, and synchronises behind it
 static __device__ __forceinline__ void load_bounds(const Offsets& o, int* bounds, PclStatus* st) {
-  if (threadIdx.x >= 32) return;
-  int carry = 0;
-  for (int i0 = 0; i0 <= o.groups; i0 += 32) {
-    const int i = i0 + (int)threadIdx.x;
-    const long long raw = i <= o.groups ? o.raw(i) : 0;
-    int v = (int)min(max(raw, 0ll), (long long)o.rows);
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, d);
-      if ((int)threadIdx.x >= d) v = max(v, u);
-    }
-    v = max(v, carry);
-    if (i <= o.groups) {
-      bounds[i] = v;
-      if (v != raw) pcl_report_bad_id(st, 0, 110, i, raw);
-    }
-    carry = __shfl_sync(0xffffffffu, v, 31);
+  for (int i = threadIdx.x; i <= o.groups; i += blockDim.x) {
+    const long long raw = o.raw(i);
+    const int v = (int)min(max(raw, 0ll), (long long)o.rows);
+    bounds[i] = v;
+    if (v != raw) pcl_report_bad_id(st, 0, 110, i, raw);
   }
 }
 

@@ -174,11 +174,12 @@ constexpr int THREADS = 32 * (SCALE_WARP + 3);
 constexpr int SMALL_BOX = 32;
 
 // COLS: columns of an accumulator, the most rows of A in a tile.  64 of them leave room for seven stages of 27 KB, 208 for four of 45.
-template <int COLS>
+// SPLIT: a cluster shares a tile's reduction (COLS 64 only)
+template <int COLS, bool SPLIT>
 struct Form {
   static constexpr int STAGE_BYTES = P_BYTES + COLS * 128;
-  static constexpr int STAGES = 192 * 1024 / (STAGE_BYTES + SCALE_BYTES);
-  static constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES;   // and Shared
+  static constexpr int STAGES = (192 * 1024 - (SPLIT ? INBOX_BYTES : 0)) / (STAGE_BYTES + SCALE_BYTES);
+  static constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (SPLIT ? INBOX_BYTES : 0);   // and Shared
   static_assert(STAGES <= MAX_STAGES, "barriers");
   static_assert(2 * COLS + STAGES * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
   static_assert(COLS % 16 == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
@@ -196,7 +197,7 @@ struct Args {
 };
 
 struct Shared {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], scales[MAX_STAGES], tfull[2], tempty[2];
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2];
   uint32_t tmem;
   int abort_flag;
   Table table;
@@ -224,63 +225,77 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t da, uint64_t db, 
 
 struct Tile {
   int e, m0, j0, n, ncol;   // columns: n of them, ncol with those that the product rounds up to
+  int k0, k1;               // stages
 };
 
 // The tiles of a call, numbered: those that share rows of A are neighbours.
+template <bool SPLIT>
 struct Walk {
+  const Args& a;
   const Table& t;
-  int mb, e;
-  long long tiles;
+  int mb, chunks;
 
-  __device__ Walk(const Args& a, const Table& t_) : t(t_), e(0) {
+  __device__ Walk(const Args& a_, const Table& t_) : a(a_), t(t_) {
     mb = (a.N + LANES - 1) / LANES;
-    tiles = (long long)t.chunks[a.off.groups] * mb;
+    chunks = t.chunks[a.off.groups];
   }
 
-  __device__ Tile at(long long i) {   // rising i
+  __device__ Counter start(int first, int step) const { return Counter(first, step, mb); }
+  __device__ bool has(const Counter& i) const { return i.c < chunks; }
+
+  __device__ Tile at(const Counter& i) const {
     Tile w;
-    const long long c = i / mb;
-    w.m0 = (int)(i - c * mb) * LANES;
-    t.find((int)c, 16, e, w.j0, w.n);
-    w.e = e;
+    w.m0 = i.m * LANES;
+    t.find(a.off.groups, i.c, 16, w.e, w.j0, w.n);
+    w.k0 = 0;
+    w.k1 = a.steps;
+    if (SPLIT) {
+      const int rank = (int)cluster_ctarank(), parts = (int)cluster_size();
+      w.k0 = rank * a.steps / parts;
+      w.k1 = (rank + 1) * a.steps / parts;
+    }
     w.ncol = (w.n + 16 - 1) / (16) * (16);
     return w;
   }
 };
 
-template <int COLS, class TO>
+template <int COLS, bool SPLIT, class TO>
 __global__ void __launch_bounds__(THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                const __grid_constant__ CUtensorMap mapQ_small, const __grid_constant__ CUtensorMap mapOut, Args a) {
-  constexpr int STAGES = Form<COLS>::STAGES, STAGE_BYTES = Form<COLS>::STAGE_BYTES;
+  constexpr int STAGES = Form<COLS, SPLIT>::STAGES, STAGE_BYTES = Form<COLS, SPLIT>::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* scales = stages + STAGES * STAGE_BYTES;
   uint8_t* pieces = scales + STAGES * SCALE_BYTES;
-  Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES);
+  float* inbox = reinterpret_cast<float*>(pieces + EPI_WARPS * PIECE_BYTES);   // SPLIT
+  Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES + (SPLIT ? INBOX_BYTES : 0));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
 
   if (warp == 0) {
-    if (lane == 0) {
-      for (int i = 0; i < STAGES; ++i) {
-        mbar_init(s.full + i, 1);
-        mbar_init(s.empty + i, 1);
-        mbar_init(s.scales + i, 3 * 32);
-      }
-      for (int i = 0; i < 2; ++i) { mbar_init(s.tfull + i, 1); mbar_init(s.tempty + i, EPI_WARPS); }
-      s.abort_flag = 0;
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (lane < STAGES) {
+      mbar_init(s.full + lane, 1 + 3 * 32);   // the loads, and every lane that copies scales
+      mbar_init(s.empty + lane, 1);
     }
-    s.table.build(a.off, COLS, &g_status);
+    if (lane < 2) { mbar_init(s.tfull + lane, 1); mbar_init(s.tempty + lane, EPI_WARPS); }
+    if (lane == 0) s.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (warp == 2 && lane == 0) {
+    for (const CUtensorMap* m : {&mapP, &mapQ, &mapQ_small, &mapOut}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+  }
+  load_bounds(a.off, s.table.bounds, &g_status);
+  __syncthreads();
+  if (warp == 0) s.table.build(a.off.groups, COLS, &g_status);
   if (warp == 1) tmem_alloc<1>(&s.tmem, TMEM_COLS);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  sync_cluster_or_block<SPLIT>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s.tmem;
-  const int group = blockIdx.x, groups = gridDim.x;
-  Walk walk(a, s.table);
+  const int share = SPLIT ? (int)cluster_size() : 1;
+  const int group = blockIdx.x / share, groups = gridDim.x / share;
+  const Walk<SPLIT> walk(a, s.table);
   bool ok = true;
   auto gave_up = [&](int where, int x, int y) {
     if (lane == 0) report(&g_status, 0, where, x, y);
@@ -291,12 +306,12 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   if (warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
+    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
       const bool whole = w.ncol == COLS;
       const int boxes = whole ? 1 : (w.ncol + SMALL_BOX - 1) / SMALL_BOX;
       const uint32_t bytes = P_BYTES + (whole ? COLS * 128 : boxes * SMALL_BOX * 128);
-      for (int kb = 0; kb < a.steps; ++kb) {
+      for (int kb = w.k0; kb < w.k1; ++kb) {
         if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(41, kb, stage); break; }
         if (elect()) {
           const uint32_t sp = smem_u32(stages + stage * STAGE_BYTES), sq = sp + P_BYTES;
@@ -322,7 +337,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     const uint64_t dp0 = desc_k_major(smem_u32(stages)), ds0 = desc_scales(smem_u32(scales));
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;   // bit i of acc_phase: accumulator i
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
+    bool ready = false;                  // the next stage has arrived
+    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
       if (!mbar_wait(s.tempty + acc, (acc_phase >> acc & 1u) ^ 1u, abort_flag)) { gave_up(42, acc, 0); break; }
       acc_phase ^= 1u << acc;
@@ -330,11 +346,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
       const uint32_t d = tmem + (uint32_t)(acc * COLS);
       const bool wide = w.ncol > 128;
-      for (int kb = 0; kb < a.steps; ++kb) {
-        if (!mbar_wait(s.full + stage, phase, abort_flag) || !mbar_wait(s.scales + stage, phase, abort_flag)) {
-          gave_up(43, kb, stage);
-          break;
-        }
+      for (int kb = w.k0; kb < w.k1; ++kb) {
+        if (!ready && !mbar_wait(s.full + stage, phase, abort_flag)) { gave_up(43, kb, stage); break; }
+        const int next = stage + 1 == STAGES ? 0 : stage + 1;
+        ready = has_passed(s.full + next, phase ^ (uint32_t)(next == 0));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (elect()) {
           // the scales were copied for other threads, and have arrived
@@ -352,10 +367,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
           for (int k = 0; k < 4; ++k) {
             const uint32_t id = (uint32_t)(k & 1) * 2;   // codes 0, 1 or 2, 3 of a word
             umma_mxf4(d, dp + 2 * k, dp + P_BYTES / 16 + 2 * k, idesc | (id << 4) | (id << 29), sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8,
-                          (kb > 0 || k > 0) ? 1u : 0u);
+                          (kb > w.k0 || k > 0) ? 1u : 0u);
           }
           commit<1>(smem_u32(s.empty + stage));
-          if (kb + 1 == a.steps) commit<1>(smem_u32(s.tfull + acc));
+          if (kb + 1 == w.k1) commit<1>(smem_u32(s.tfull + acc));
         }
         __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -374,14 +389,14 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     const int last_bytes = 4 - (a.words * 4 - a.blocks);   // codes of the last word; those that no block has become zero
     int stage = 0;
     uint32_t phase = 0;
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
+    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
       const bool used = part < 2 || w.ncol > 128;
       const long long r0 = part == 0 ? (long long)w.e * a.N + w.m0 : (long long)w.j0 + (part - 1) * 128;
       const uint8_t* at[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) at[q] = src + 4 * min(r0 + row + 8 * q, rows - 1);   // rows of no tile: any scales do
-      for (int kb = 0; kb < a.steps; ++kb) {
+      for (int kb = w.k0; kb < w.k1; ++kb) {
         if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(48, kb, stage); break; }
         if (used) {
           const uint32_t dst = dst0 + stage * SCALE_BYTES;
@@ -395,7 +410,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
               asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + v * 512 + q * 128), "l"(at[q] + off), "r"(bytes) : "memory");
           }
         }
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(s.scales + stage)) : "memory");
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(s.full + stage)) : "memory");
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
     }
@@ -406,7 +421,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     TO* out = static_cast<TO*>(a.out);
     int acc = 0;
     uint32_t acc_phase = 0;                   // bit i: accumulator i
-    for (long long i = group; i < walk.tiles && ok; i += groups) {
+    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
       if (!mbar_wait(s.tfull + acc, acc_phase >> acc & 1u, abort_flag)) { gave_up(44, acc, 0); break; }
       acc_phase ^= 1u << acc;
@@ -414,6 +429,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const int m = w.m0 + sub * 32;
       TO* dst = out + (long long)w.j0 * a.ldo + m;
       const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * COLS);
+      if (SPLIT) {   // the cluster has this one tile
+        send_columns(t0, sub, half * 32, w.n, inbox, cluster_ctarank(), columns_of_part(w.n, share));
+        continue;
+      }
       store_columns<TO>(t0, half * 32, w.n, dst, a.ldo, a.N - m, a.boxed, pieces + (warp - 2) * PIECE_BYTES, &mapOut, m, w.j0, 0);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -433,33 +452,52 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncwarp();
-  __syncthreads();
+  sync_cluster_or_block<SPLIT>();   // the parts of a split tile are in their inboxes
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     tmem_free<1>(tmem, TMEM_COLS);
   }
+  if (SPLIT && warp >= 2 && warp < SCALE_WARP && walk.has(walk.start(group, groups))) {
+    const Tile w = walk.at(walk.start(group, groups));
+    add_up<TO>(inbox, w.n, columns_of_part(w.n, share), cluster_ctarank(), share, 64, 32 * EPI_WARPS, static_cast<TO*>(a.out) + (long long)w.j0 * a.ldo + w.m0,
+               a.ldo, a.N - w.m0);
+  }
 }
 
-template <int COLS, class TO>
-int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  auto kernel = product_kernel<COLS, TO>;
-  constexpr int smem = Form<COLS>::SMEM_BYTES + (int)sizeof(Shared);
+template <int COLS, bool SPLIT, class TO>
+int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, int parts, cudaStream_t stream) {
+  auto kernel = product_kernel<COLS, SPLIT, TO>;
+  constexpr int smem = Form<COLS, SPLIT>::SMEM_BYTES + (int)sizeof(Shared);
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
   const long long mb = (a.N + LANES - 1) / LANES;
-  const long long chunks = a.off.rows / COLS + min(a.off.groups, a.off.rows);
-  kernel<<<(unsigned)min((long long)sms, chunks * mb), THREADS, smem, stream>>>(p, q, qs, o, a);
-  return pcl_last_error();
+  const long long chunks = most_chunks(a.off.rows, a.off.groups, COLS);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  // a cluster that shares a tile has no other
+  cfg.gridDim = dim3(SPLIT ? (unsigned)(chunks * mb) * parts : (unsigned)min((long long)sms, chunks * mb));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = SPLIT ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, o, a);
+  return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 
-template <int COLS>
-int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, cudaStream_t stream) {
-  if (out_type == TYPE_F32) return launch<COLS, float>(p, q, qs, o, a, stream);
-  if (out_type == TYPE_BF16) return launch<COLS, __nv_bfloat16>(p, q, qs, o, a, stream);
-  return launch<COLS, __half>(p, q, qs, o, a, stream);
+template <int COLS, bool SPLIT>
+int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, int parts,
+              cudaStream_t stream) {
+  if (out_type == TYPE_F32) return launch<COLS, SPLIT, float>(p, q, qs, o, a, parts, stream);
+  if (out_type == TYPE_BF16) return launch<COLS, SPLIT, __nv_bfloat16>(p, q, qs, o, a, parts, stream);
+  return launch<COLS, SPLIT, __half>(p, q, qs, o, a, parts, stream);
 }
 
 bool blocks_of(long long rows, int words, long long* n) {
@@ -529,7 +567,10 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
   Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
          N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false};
   a.boxed = make_out_map(&o, p, out_type, out, N, rows, 1, ldo, ldo);
-  return few ? launch_as<FEW_COLS>(out_type, p, q, qs, o, a, stream) : launch_as<MANY_COLS>(out_type, p, q, qs, o, a, stream);
+  if (!few) return launch_as<MANY_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
+  const long long tiles = most_chunks(rows, groups, FEW_COLS) * ((N + LANES - 1) / LANES);
+  const int parts = parts_of(tiles, a.steps, 148);
+  return parts > 1 ? launch_as<FEW_COLS, true>(out_type, p, q, qs, o, a, parts, stream) : launch_as<FEW_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
 }
 
 // Copies the status block of these products to `host` and clears it (waits for the stream).

@@ -20,31 +20,50 @@ struct Table {
   int bounds[pcl_group::MAX_GROUPS + 1];
   int chunks[pcl_group::MAX_GROUPS + 1];   // chunks of the groups before
 
-  // by the first warp
-  __device__ __forceinline__ void build(const pcl_group::Offsets& o, int most, PclStatus* st) {
-    pcl_group::load_bounds(o, bounds, st);
-    if (threadIdx.x >= 32) return;
-    __syncwarp();
-    int carry = 0;
-    for (int i0 = 0; i0 < o.groups; i0 += 32) {
-      const int i = i0 + (int)threadIdx.x;
-      const int own = i < o.groups ? (bounds[i + 1] - bounds[i] + most - 1) / most : 0;
-      int v = own;
+  // By the first warp, behind load_bounds and a barrier.  Bounds are made ascending (each at least the one before it) whatever the array
+  // holds, so that no row is in two groups; the first one that had to be moved goes into the status block.
+  __device__ __forceinline__ void build(int groups, int most, PclStatus* st) {
+    const int lane = threadIdx.x;
+    int top = bounds[0], carry = 0;
+    for (int i0 = 0; i0 < groups; i0 += 32) {
+      const int i = i0 + lane + 1;
+      const int own = i <= groups ? bounds[i] : 0;
+      int v = max(own, top);
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, d);
-        if ((int)threadIdx.x >= d) v += u;
+        if (lane >= d) v = max(v, u);
       }
-      if (i < o.groups) chunks[i] = carry + v - own;
-      carry += __shfl_sync(0xffffffffu, v, 31);
+      int before = __shfl_up_sync(0xffffffffu, v, 1);
+      if (lane == 0) before = top;
+      top = __shfl_sync(0xffffffffu, v, 31);
+      if (i <= groups) {
+        bounds[i] = v;
+        if (v != own) pcl_report_bad_id(st, 0, 110, i, own);
+      }
+      const int parts = i <= groups ? (v - before + most - 1) / most : 0;
+      int sum = parts;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += u;
+      }
+      if (i <= groups) chunks[i - 1] = carry + sum - parts;
+      carry += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (threadIdx.x == 0) chunks[o.groups] = carry;
+    if (lane == 0) chunks[groups] = carry;
   }
 
   // `step` divides `most`: a chunk is then at most `most` rows, and all but the last of a group's chunks cannot hold all its rows.
-  // Rows [begin, begin + n) of chunk `c`, in group `e` (which only grows: callers ask for rising chunks)
-  __device__ __forceinline__ void find(int c, int step, int& e, int& begin, int& n) const {
-    while (c >= chunks[e + 1]) ++e;
+  // Rows [begin, begin + n) of chunk `c`, in group `e`, the last whose chunks begin at or before `c`
+  __device__ __forceinline__ void find(int groups, int c, int step, int& e, int& begin, int& n) const {
+    int hi = groups;   // chunks[e] <= c < chunks[hi]
+    e = 0;
+    while (hi - e > 1) {
+      const int mid = (e + hi) >> 1;
+      if (chunks[mid] <= c) e = mid;
+      else hi = mid;
+    }
     const int rows = bounds[e + 1] - bounds[e], parts = chunks[e + 1] - chunks[e];
     const int size = ((rows + parts - 1) / parts + step - 1) / step * step;
     begin = bounds[e] + (c - chunks[e]) * size;
@@ -59,6 +78,20 @@ __device__ __forceinline__ bool elect() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
+}
+
+// Whether the phase has passed, without waiting.  The answer takes 85 cycles: asked for the next stage while the products of this one are issued, it
+// costs nothing where the stage has arrived.
+__device__ __forceinline__ bool has_passed(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
 }
 
 // as mbar_wait, for a barrier that the other CTA of a pair arrives on
@@ -153,10 +186,27 @@ __device__ __forceinline__ void tmem_free(uint32_t base, int cols) {
   else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
 }
 
-template <int CG>
+// A CTA's (or cluster's) tiles, first, first + step, ..: tile c * across + m is block m of chunk c.  No division but at the start, and that in 32 bits: one in
+// 64 takes longer than a short tile.
+struct Counter {
+  int c, m, dc, dm, across;
+  __device__ Counter(int first, int step, int across_) : across(across_) {
+    c = first / across;
+    m = first - c * across;
+    dc = step / across;
+    dm = step - dc * across;
+  }
+  __device__ __forceinline__ void next() {
+    c += dc;
+    m += dm;
+    if (m >= across) { m -= across; ++c; }
+  }
+};
+
+template <bool CLUSTER>
 __device__ __forceinline__ void sync_cluster_or_block() {
   __syncthreads();
-  if (CG == 2) {
+  if (CLUSTER) {
     __syncwarp();
     cluster_sync_all();
   }
@@ -194,6 +244,34 @@ static __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
 
 // Where a warp puts 32 columns x 32 lanes of its accumulator for the copy engine: 2 KB, rows of 64 bytes (a column's 32 lanes)
 constexpr int PIECE_BYTES = 2048;
+
+// 8 columns of the warp's 32 lanes
+static __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+
+// n columns lane by lane, a row's 32 neighbours at a time: short code, for the few columns of short calls
+template <class TO>
+__device__ __forceinline__ void store_singly(uint32_t taddr, int n, TO* dst, long long ldo, int lanes) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int c = 0; c < n; c += 8) {
+    uint32_t v[8];
+    tmem_ld8(taddr + (uint32_t)c, v);
+    if (lane < lanes) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < n) dst[(c + j) * ldo + lane] = pcl_group::to_out<TO>(__uint_as_float(v[j]));
+    }
+    __syncwarp();
+  }
+}
 
 // A warp's part of an accumulator goes to out: column j of [0, n) and the warp's 32 lanes to dst[j * ldo + lane], lanes < `lanes` only.  Columns 32 at a time,
 // first + 0, 64, 128 ..  16-bit results turn around in shared memory (stmatrix) and leave as boxes of 32 rows
@@ -235,14 +313,7 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, int first, int n, 
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     } else {
-      uint32_t v[32];
-      tmem_ld32_issue(taddr + (uint32_t)c, v);
-      tmem_ld_wait(v);
-      if (lane < lanes) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j < n) dst[(long long)(c + j) * ldo + lane] = pcl_group::to_out<TO>(__uint_as_float(v[j]));
-      }
+      store_singly(taddr + (uint32_t)c, min(32, n - c), dst + (long long)c * ldo, ldo, lanes);
     }
     __syncwarp();
   }
@@ -250,18 +321,64 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, int first, int n, 
 template <>
 __device__ __forceinline__ void store_columns<float>(uint32_t taddr, int first, int n, float* dst, long long ldo, int lanes, bool, uint8_t*,
                                                      const CUtensorMap*, int, int, int) {
+  for (int c = first; c < n; c += 64) store_singly(taddr + (uint32_t)c, min(32, n - c), dst + (long long)c * ldo, ldo, lanes);
+}
+
+// ---- one tile by a cluster: every CTA has a part of the reduction, and adds up the parts of some of the columns
+
+static __device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+
+constexpr int INBOX_BYTES = (64 + 8) * 128 * 4;   // up to 64 columns, rounded up to 8 parts
+__device__ __forceinline__ int columns_of_part(int n, int parts) { return (n + parts - 1) / parts; }
+
+// This warp's quarter of the accumulator to the CTAs that add it up: columns [o * each, (o + 1) * each) go to CTA o, there into inbox[rank][column][lane]
+static __device__ __forceinline__ void send_columns(uint32_t taddr, int sub, int first, int n, const float* inbox, uint32_t rank, int each) {
   const int lane = threadIdx.x & 31;
-  for (int c = first; c < n; c += 64) {
-    uint32_t v[32];
-    tmem_ld32_issue(taddr + (uint32_t)c, v);
-    tmem_ld_wait(v);
-    if (lane < lanes) {
+#pragma unroll 1
+  for (int c = first; c < n; c += ((c & 31) == 24 ? 40 : 8)) {   // 32 columns of every 64, eight at a time
+    uint32_t v[8];
+    tmem_ld8(taddr + (uint32_t)c, v);
+    int owner = c / each, col = c - owner * each;
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (c + j < n) dst[(long long)(c + j) * ldo + lane] = __uint_as_float(v[j]);
+    for (int j = 0; j < 8; ++j) {
+      if (c + j < n) {
+        const uint32_t at = map_to_cta(smem_u32(inbox + ((int)rank * each + col) * 128 + sub * 32 + lane), (uint32_t)owner);
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v[j]) : "memory");
+      }
+      if (++col == each) { col = 0; ++owner; }
     }
     __syncwarp();
   }
+}
+
+// Behind the cluster's barrier: this CTA's columns, added up in the order of the parts, to dst[column * ldo + lane]; by `threads` threads from `first` on
+template <class TO>
+__device__ __forceinline__ void add_up(const float* inbox, int n, int each, uint32_t rank, int parts, int first, int threads, TO* dst, long long ldo, int lanes) {
+  const int mine = min(each, n - (int)rank * each);
+  for (int i = (int)threadIdx.x - first; i < mine * 128; i += threads) {
+    const int col = i >> 7, l = i & 127;
+    float v = 0.f;
+    for (int p = 0; p < parts; ++p) v += inbox[(p * each + col) * 128 + l];
+    if (l < lanes) dst[((long long)rank * each + col) * ldo + l] = pcl_group::to_out<TO>(v);
+  }
+}
+
+// the most chunks of at most `cols` rows that `rows` rows of `groups` groups can make
+static inline long long most_chunks(long long rows, int groups, int cols) {
+  const long long taken = rows < groups ? rows : groups;   // groups with a row
+  return (rows - taken) / cols + taken;
+}
+
+// Parts that a tile's reduction of `steps` stages is cut into where `tiles` of them leave more than half the SMs idle: as many as fill these, at most
+// eight (the largest portable cluster), and two stages at least for each.  1: not cut.
+static inline int parts_of(long long tiles, int steps, int sms) {
+  int parts = 1;
+  while (parts < 8 && tiles * parts * 2 <= sms && steps >= max(8, parts * 4)) parts *= 2;
+  return parts;
 }
 
 // map of `depth` matrices [rows x inner]; strides in bytes; box: box_in values x box_rows rows of one matrix.  `inner` and box_in count elements of `type`.
