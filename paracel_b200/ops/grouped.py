@@ -142,7 +142,8 @@ def _check_rows(mode: int, X, W, offsets, out, dtype) -> None:
 
 
 def _rows(mode: int, X, W, offsets, out, out_dtype):
-    # a call is a few microseconds on the device: everything is looked at once here, and what is wrong is found out above
+    # A call is a few microseconds on the device: everything is looked at once here, and what is wrong is found out above.  (A
+    # size given as a tuple costs torch.empty 0.8 us.)
     xs, ws, dtype, device = X.shape, W.shape, X.dtype, X.get_device()
     if not (len(xs) == 2 and len(ws) == 3 and (dtype == torch.bfloat16 or dtype == torch.float16) and W.dtype == dtype
             and xs[1] == ws[2 - mode] and 0 < ws[1] < 1 << 30 and 0 < ws[2] < 1 << 30 and xs[0] < MAX_ROWS
@@ -155,7 +156,7 @@ def _rows(mode: int, X, W, offsets, out, out_dtype):
     cols = ws[1 + mode]
     fill = out is None
     if fill:
-        out = torch.empty((T, cols), dtype=dtype if out_dtype is None else out_dtype, device=X.device)
+        out = torch.empty(T, cols, dtype=dtype if out_dtype is None else out_dtype, device=X.device)
     if T == 0:
         return out
     x, w = X.data_ptr(), W.data_ptr()
@@ -216,7 +217,7 @@ def grouped_tn(dY: torch.Tensor, X: torch.Tensor, offsets: torch.Tensor, out: Op
         _check_tn(dY, X, offsets, out, out_dtype)
     T, K, N, E = xs[0], xs[1], ys[1], offsets.shape[0] - 1
     if out is None:
-        out = torch.empty((E, N, K), dtype=dtype if out_dtype is None else out_dtype, device=X.device)
+        out = torch.empty(E, N, K, dtype=dtype if out_dtype is None else out_dtype, device=X.device)
     if T == 0:
         return out.zero_()
     x, y = X.data_ptr(), dY.data_ptr()

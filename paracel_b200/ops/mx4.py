@@ -30,16 +30,43 @@ class Mx4Matrix:
     high half, zeros behind the last.  ``scales [ceil(cols / 128), rows, 4]`` (uint8): ``scales[b, r, i]`` is the code of block
     ``4 b + i`` of row ``r`` (255, which stands for NaN, only where the row has such a block)."""
 
-    __slots__ = ("data", "scales", "cols")
+    # _data and _scales are None where both lie in _buf, until they are asked for
+    __slots__ = ("_data", "_scales", "_buf", "_device", "rows", "cols", "_data_ptr", "_scales_ptr")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, cols: int):
         ds, ss = data.shape, scales.shape
+        data_ptr, scales_ptr, device = data.data_ptr(), scales.data_ptr(), data.get_device()
         if not (0 < cols < 1 << 30 and data.dtype == torch.uint8 and scales.dtype == torch.uint8 and len(ds) == 2 and len(ss) == 3
                 and ds[1] == (cols + 31) // 32 * 16 and ss[0] == (cols + 127) // 128 and ss[1] == ds[0] and ss[2] == 4
                 and ds[0] < MAX_ROWS and data.is_contiguous() and scales.is_contiguous()
-                and not (data.data_ptr() | scales.data_ptr()) & 15 and data.get_device() == scales.get_device()):
+                and not (data_ptr | scales_ptr) & 15 and scales.get_device() == device):
             self._refuse(data, scales, cols)
-        self.data, self.scales, self.cols = data, scales, cols
+        self._data, self._scales, self._buf, self._device = data, scales, None, device
+        self.rows, self.cols, self._data_ptr, self._scales_ptr = ds[0], cols, data_ptr, scales_ptr
+
+    @classmethod
+    def _empty(cls, rows: int, cols: int, device: torch.device) -> "Mx4Matrix":
+        """One whose values are not set: both parts in one allocation (two and their checks take 3 us more)."""
+        q = cls.__new__(cls)
+        size = rows * ((cols + 31) // 32 * 16)           # a multiple of 16
+        buf = torch.empty(size + (cols + 127) // 128 * rows * 4, dtype=torch.uint8, device=device)
+        q._data, q._scales, q._buf, q._device, q.rows, q.cols = None, None, buf, buf.get_device(), rows, cols
+        q._data_ptr = buf.data_ptr()
+        q._scales_ptr = q._data_ptr + size
+        return q
+
+    @property
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            width = (self.cols + 31) // 32 * 16
+            self._data = self._buf[:self.rows * width].view(self.rows, width)
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._buf[self.rows * ((self.cols + 31) // 32 * 16):].view((self.cols + 127) // 128, self.rows, 4)
+        return self._scales
 
     @staticmethod
     def _refuse(data, scales, cols):
@@ -57,12 +84,8 @@ class Mx4Matrix:
         raise ValueError(f"at most 2^31 - 513 rows, got {data.shape[0]}")
 
     @property
-    def rows(self) -> int:
-        return self.data.shape[0]
-
-    @property
     def device(self) -> torch.device:
-        return self.data.device
+        return (self._data if self._buf is None else self._buf).device
 
     def nbytes(self) -> int:
         return self.data.numel() + self.scales.numel()
@@ -80,25 +103,25 @@ def check_status(device=None) -> None:
 def mx4_quantize(X: torch.Tensor) -> Mx4Matrix:
     """``X [rows, K]`` (float32, bfloat16, float16) in four bits; ``X [E, N, K]``, the matrices of E groups, becomes one
     of ``E N`` rows."""
-    if X.dtype not in TYPES:
+    shape, kind, device = X.shape, TYPES.get(X.dtype), X.get_device()
+    if kind is None:
         raise ValueError(f"X must be float32, bfloat16 or float16, got {X.dtype}")
-    if X.dim() not in (2, 3):
-        raise ValueError(f"X must have 2 or 3 dimensions, got {X.dim()}")
-    K = X.shape[-1]
+    if len(shape) != 2 and len(shape) != 3:
+        raise ValueError(f"X must have 2 or 3 dimensions, got {len(shape)}")
+    K = shape[-1]
     if not 1 <= K < 1 << 30:
         raise ValueError(f"X must have 1 to 2^30 - 1 columns, got {K}")
-    device = X.get_device()
     if device < 0:
         check_devices(X=X)
-    if X.dim() == 3:
+    if len(shape) == 3:
         X = X.reshape(-1, K)
     X, ldx = _row_stride(X)
     rows = X.shape[0]
-    data = torch.empty((rows, (K + 31) // 32 * 16), dtype=torch.uint8, device=X.device)
-    scales = torch.empty(((K + 127) // 128, rows, 4), dtype=torch.uint8, device=X.device)
-    q = Mx4Matrix(data, scales, K)
+    if rows >= MAX_ROWS:
+        raise ValueError(f"at most 2^31 - 513 rows, got {rows}")
+    q = Mx4Matrix._empty(rows, K, X.device)
     if rows:
-        _lib.call_on(device, "pcl_mx4_quantize", X.data_ptr(), ldx, TYPES[X.dtype], data.data_ptr(), scales.data_ptr(), rows, K)
+        _lib.call_on(device, "pcl_mx4_quantize", X.data_ptr(), ldx, kind, q._data_ptr, q._scales_ptr, rows, K)
     return q
 
 
@@ -116,14 +139,14 @@ def mx4_dequantize(q: Mx4Matrix, dtype: torch.dtype = torch.float32, out: Option
     either); float16 rounds."""
     if dtype not in TYPES:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
-    if out is not None or not q.data.is_cuda:
+    if out is not None or q._device < 0:
         check_out(out, (q.rows, q.cols), dtype)
         check_devices(q=q, out=out)
     if out is None:
-        out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.data.device)
+        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
     if q.rows:
-        _lib.call_on(q.data.get_device(), "pcl_mx4_dequantize", q.data.data_ptr(), q.scales.data_ptr(), out.data_ptr(), out.stride(0),
-                     TYPES[dtype], q.rows, q.cols)
+        _lib.call_on(q._device, "pcl_mx4_dequantize", q._data_ptr, q._scales_ptr, out.data_ptr(), out.stride(0), TYPES[dtype], q.rows,
+                     q.cols)
     return out
 
 
@@ -151,34 +174,37 @@ def _product(A, B: Mx4Matrix, offsets, out, out_dtype):
     packed = isinstance(A, Mx4Matrix)
     if not isinstance(B, Mx4Matrix):
         _check_product(A, B, offsets, out, out_dtype)
-    data = B.data
-    K, rows, device = B.cols, data.shape[0], data.get_device()
-    shape = (A.data.shape[0], A.cols) if packed else A.shape
-    dtype = out_dtype if out_dtype is not None else out.dtype if out is not None else torch.float32 if packed else A.dtype
+    K, rows, device = B.cols, B.rows, B._device
+    if packed:
+        T, cols, kind, place, own = A.rows, A.cols, -1, A._device, torch.float32
+    else:
+        T, cols = A.shape if A.dim() == 2 else (0, 0)
+        own = A.dtype
+        kind, place = TYPES.get(own), A.get_device()
+    dtype = out_dtype if out_dtype is not None else out.dtype if out is not None else own
     groups = 1 if offsets is None else offsets.numel() - 1
-    if not (len(shape) == 2 and shape[1] == K and (packed or A.dtype in TYPES) and dtype in TYPES and out is None and shape[0] < MAX_ROWS
-            and 0 < groups <= rows and rows % groups == 0 and device >= 0 and (A.data if packed else A).get_device() == device
+    if not (cols == K and kind is not None and dtype in TYPES and out is None and T < MAX_ROWS
+            and 0 < groups <= rows and rows % groups == 0 and device >= 0 and place == device
             and (offsets is None or offsets.dim() == 1 and groups <= MAX_GROUPS and offsets.get_device() == device
                  and (offsets.dtype == torch.int32 or offsets.dtype == torch.int64) and offsets.is_contiguous())):
         _check_product(A, B, offsets, out, out_dtype)
-    T, N = shape[0], rows // groups
+    N = rows // groups
     fill = out is None
     if fill:
-        out = torch.empty((T, N), dtype=dtype, device=data.device)
+        out = torch.empty(T, N, dtype=dtype, device=B.device)
     if T == 0:
         return out
     if packed:
-        x, ldx, kind, a, sa = 0, 0, -1, A.data.data_ptr(), A.scales.data_ptr()
+        x, ldx, a, sa = 0, 0, A._data_ptr, A._scales_ptr
     else:
         # A in four bits, for the length of the call
         A, ldx = _row_stride(A)
         size = T * ((K + 31) // 32 * 16)
-        work = torch.empty(size + T * ((K + 127) // 128 * 4), dtype=torch.uint8, device=data.device)
-        x, kind, a = A.data_ptr(), TYPES[A.dtype], work.data_ptr()
+        work = torch.empty(size + T * ((K + 127) // 128 * 4), dtype=torch.uint8, device=out.device)
+        x, a = A.data_ptr(), work.data_ptr()
         sa = a + size
-    _lib.call_on(device, "pcl_mx4_rows", x, ldx, kind, a, sa, data.data_ptr(), B.scales.data_ptr(),
-                 None if offsets is None else offsets.data_ptr(), offsets is not None and offsets.dtype == torch.int64, out.data_ptr(),
-                 out.stride(0), TYPES[dtype], T, groups, N, K, fill)
+    _lib.call_on(device, "pcl_mx4_rows", x, ldx, kind, a, sa, B._data_ptr, B._scales_ptr, None if offsets is None else offsets.data_ptr(),
+                 offsets is not None and offsets.dtype == torch.int64, out.data_ptr(), out.stride(0), TYPES[dtype], T, groups, N, K, fill)
     return out
 
 
