@@ -36,11 +36,23 @@ __device__ __forceinline__ uint32_t pack8(const float* v) {
   return d;
 }
 
-// value of a four-bit code: codes 0 and 1 are 0 and 1/2, above them (2 + mantissa) / 2 * 2^(exponent - 1)
-__device__ __forceinline__ float code_value(uint32_t c) {
-  const uint32_t m = c & 7u;
-  const float v = m < 2u ? 0.5f * (float)m : __uint_as_float((m << 22) + (126u << 23));
-  return (c & 8u) ? -v : v;
+// the values of eight codes, v[0] of the lowest: the conversion to fp16 is exact
+__device__ __forceinline__ void unpack8(uint32_t codes, float* v) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(codes));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(h + i));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
 }
 
 struct QuantArgs {
@@ -53,61 +65,73 @@ struct QuantArgs {
   int vec;             // rows of x can be read 16 bytes at a time
 };
 
-// A thread takes eight neighbouring values of a row; four lanes make a block of 32, sixteen a word of scales.  A block of
-// the grid takes 128 columns of QROWS rows and stores its words of scales side by side.
-constexpr int QROWS = 32, QTHREADS = 256;
+// A thread takes eight neighbouring values of a row, four lanes make a block of 32 and sixteen a word of scales: a warp reads 256 values (512 bytes of 16-bit
+// ones) and stores 128 bytes.  It goes over ITERS times as many of one row, all of its loads before the first use; the block's eight rows
+// make whole sectors of scales.  Bound by memory: 32768 x 8192 of bf16 takes 123 us (5.6 TB/s), back to bf16 106 us (6.5 TB/s); 32 rows x 128
+// columns to a block, whose rows are 256 bytes here and 64 there, took 161 and 184 us.  The registers are bounded so that six blocks share an SM: with
+// five of them quantisation takes 164 us, with seven, whose loads no longer fit, 224.
+constexpr int QROWS = 8, QTHREADS = 32 * QROWS;
 
-template <class T>
-__global__ void __launch_bounds__(QTHREADS) quantize_kernel(QuantArgs a) {
-  __shared__ uint32_t words[QROWS];
-  const int word = blockIdx.x % a.words;
-  const long long r0 = (long long)(blockIdx.x / a.words) * QROWS;
-  const int part = threadIdx.x & 15;
-  const int c0 = word * 128 + part * 8;
-  const int row_bytes4 = (a.K + 31) / 32 * 4;          // 4-byte words of a row of data
+template <int ITERS, class T>
+__global__ void __launch_bounds__(QTHREADS, 6) quantize_kernel(QuantArgs a) {
+  constexpr int QCOLS = 256 * ITERS, QWORDS = QCOLS / 128;
+  // a product that is queued behind this may set itself up meanwhile; it waits before it reads what is written here
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ uint32_t words[QWORDS][QROWS];
+  const int across = (a.words + QWORDS - 1) / QWORDS;
+  const int part = (int)(blockIdx.x % across);
+  const long long r0 = (long long)(blockIdx.x / across) * QROWS, r = r0 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int row_words = (a.K + 31) / 32 * 4;           // 4-byte words of a row of data
+  const T* src = static_cast<const T*>(a.x) + r * a.ldx;
+  constexpr int PER = sizeof(T) / 2;                   // 16-byte loads of eight values
+  uint4 raw[ITERS][PER];
+  if (r < a.rows) {
 #pragma unroll
-  for (int i = 0; i < QROWS * 16 / QTHREADS; ++i) {
-    const int lr = i * (QTHREADS / 16) + (threadIdx.x >> 4);
-    const long long r = r0 + lr;
-    float v[8];
+    for (int i = 0; i < ITERS; ++i) {
+      const int c = part * QCOLS + i * 256 + lane * 8;
+      if (a.vec && c + 8 <= a.K) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    if (r < a.rows && c0 < a.K) {
-      const T* src = static_cast<const T*>(a.x) + r * a.ldx + c0;
-      if (a.vec && c0 + 8 <= a.K) {
-        uint4 raw[sizeof(T) / 2];
-#pragma unroll
-        for (int q = 0; q < (int)(sizeof(T) / 2); ++q) raw[q] = reinterpret_cast<const uint4*>(src)[q];
-        const T* p = reinterpret_cast<const T*>(raw);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_f32(p[j]);
+        for (int q = 0; q < PER; ++q) raw[i][q] = __ldcs(reinterpret_cast<const uint4*>(src + c) + q);
       } else {
+        T v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c0 + j < a.K) v[j] = to_f32(src[j]);
+        for (int j = 0; j < 8; ++j) v[j] = c + j < a.K ? src[c + j] : to_out<T>(0.f);
+        memcpy(raw[i], v, sizeof(v));
       }
     }
-    // the largest magnitude of the block, by its bits: NaN and infinity come out on top
-    uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const bool bad = most >= 0x7f800000u;
-    // floor(log2(most)) - 2, at least -127 (all that is below 2^-125 takes the smallest scale)
-    const int code = bad ? 255 : max((int)(most >> 23) - 2, 0);
-    const float inv = __uint_as_float((uint32_t)(254 - min(code, 253)) << 23);
+    for (int i = 0; i < ITERS; ++i) {
+      const int c = part * QCOLS + i * 256 + lane * 8;
+      T t[8];
+      memcpy(t, raw[i], sizeof(t));
+      float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = bad ? 0.f : mul_keep(v[j], inv);
-    if (r < a.rows && c0 < row_bytes4 * 8) a.data[r * row_bytes4 + (c0 >> 3)] = pack8(v);
-    uint32_t w = (c0 < row_bytes4 * 8) ? (uint32_t)code << (8 * (part >> 2)) : 0u;
-    w |= __shfl_xor_sync(0xffffffffu, w, 4);
-    w |= __shfl_xor_sync(0xffffffffu, w, 8);
-    if (part == 0) words[lr] = w;
+      for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
+      // the largest magnitude of the block, by its bits: NaN and infinity come out on top
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const bool bad = most >= 0x7f800000u;
+      // floor(log2(most)) - 2, at least -127 (all that is below 2^-125 takes the smallest scale)
+      const int code = bad ? 255 : max((int)(most >> 23) - 2, 0);
+      const float inv = __uint_as_float((uint32_t)(254 - min(code, 253)) << 23);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = mul_keep(v[j], inv);   // no matter which in a block that is not a number
+      const bool in = c < row_words * 8;
+      if (in) a.data[r * row_words + (c >> 3)] = pack8(v);
+      uint32_t w = in ? (uint32_t)code << (8 * ((lane & 15) >> 2)) : 0u;
+      w |= __shfl_xor_sync(0xffffffffu, w, 4);
+      w |= __shfl_xor_sync(0xffffffffu, w, 8);
+      if ((lane & 15) == 0) words[i * 2 + (lane >> 4)][threadIdx.x >> 5] = w;
+    }
   }
   __syncthreads();
-  if (threadIdx.x < QROWS && r0 + threadIdx.x < a.rows)
-    a.scales[(long long)word * a.rows + r0 + threadIdx.x] = words[threadIdx.x];
+  const int word = part * QWORDS + (int)threadIdx.x / QROWS, row = threadIdx.x % QROWS;
+  if (threadIdx.x < QWORDS * QROWS && word < a.words && r0 + row < a.rows)
+    a.scales[(long long)word * a.rows + r0 + row] = words[threadIdx.x / QROWS][row];
 }
 
 struct DequantArgs {
@@ -118,29 +142,45 @@ struct DequantArgs {
   int K, words, vec;
 };
 
-template <class T>
+template <int ITERS, class T>
 __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
-  const int word = blockIdx.x % a.words;
-  const long long r0 = (long long)(blockIdx.x / a.words) * QROWS;
-  const int part = threadIdx.x & 15;
-  const int c0 = word * 128 + part * 8;
-  const int row_bytes4 = (a.K + 31) / 32 * 4;
+  constexpr int QCOLS = 256 * ITERS, QWORDS = QCOLS / 128;
+  const int across = (a.words + QWORDS - 1) / QWORDS;
+  const int part = (int)(blockIdx.x % across);
+  const long long r = (long long)(blockIdx.x / across) * QROWS + (threadIdx.x >> 5);
+  if (r >= a.rows) return;
+  const int lane = threadIdx.x & 31;
+  const int row_words = (a.K + 31) / 32 * 4;
+  uint32_t codes[ITERS], scale[ITERS];
 #pragma unroll
-  for (int i = 0; i < QROWS * 16 / QTHREADS; ++i) {
-    const long long r = r0 + i * (QTHREADS / 16) + (threadIdx.x >> 4);
-    if (r >= a.rows || c0 >= a.K) continue;
-    const uint32_t codes = a.data[r * row_bytes4 + (c0 >> 3)];
-    const float s = scale_value((a.scales[(long long)word * a.rows + r] >> (8 * (part >> 2))) & 255u);
-    T* dst = static_cast<T*>(a.out) + r * a.ldo + c0;
-    __align__(16) T v[8];
+  for (int i = 0; i < ITERS; ++i) {
+    const int c = part * QCOLS + i * 256 + lane * 8;
+    codes[i] = scale[i] = 0;
+    if (c < a.K) {
+      codes[i] = __ldcs(a.data + r * row_words + (c >> 3));
+      scale[i] = a.scales[(long long)(c >> 7) * a.rows + r];
+    }
+  }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_out<T>(mul_keep(code_value((codes >> (4 * j)) & 15u), s));
-    if (a.vec && c0 + 8 <= a.K) {
+  for (int i = 0; i < ITERS; ++i) {
+    const int c = part * QCOLS + i * 256 + lane * 8;
+    if (c >= a.K) continue;
+    const float s = scale_value((scale[i] >> (8 * ((lane & 15) >> 2))) & 255u);
+    float f[8];
+    unpack8(codes[i], f);
+    T v[8];
 #pragma unroll
-      for (int q = 0; q < (int)(sizeof(T) / 2); ++q) reinterpret_cast<uint4*>(dst)[q] = reinterpret_cast<uint4*>(v)[q];
+    for (int j = 0; j < 8; ++j) v[j] = to_out<T>(mul_keep(f[j], s));
+    T* dst = static_cast<T*>(a.out) + r * a.ldo + c;
+    if (a.vec && c + 8 <= a.K) {
+      uint4 raw[sizeof(T) / 2];
+      memcpy(raw, v, sizeof(v));
+#pragma unroll
+      for (int q = 0; q < (int)(sizeof(T) / 2); ++q) __stcs(reinterpret_cast<uint4*>(dst) + q, raw[q]);
     } else {
+#pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c0 + j < a.K) dst[j] = v[j];
+        if (c + j < a.K) dst[j] = v[j];
     }
   }
 }
@@ -194,6 +234,7 @@ struct Args {
   Offsets off;
   int N, steps, words, blocks, fill;
   bool boxed;   // results leave through mapOut
+  bool behind;  // launched while the quantisation of A still runs
 };
 
 struct Shared {
@@ -304,6 +345,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   };
 
   if (warp == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the quantisation of A, where it is queued right before
     int stage = 0;
     uint32_t phase = 0;
     for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
@@ -379,6 +421,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     }
   } else if (warp >= SCALE_WARP) {
     const int part = warp - SCALE_WARP;      // 0: P, 1 and 2: Q
+    if (part > 0) asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long rows = part == 0 ? (long long)a.off.groups * a.N : a.off.rows;
     const uint8_t* src = reinterpret_cast<const uint8_t*>(part == 0 ? a.sp : a.sq);
     // Of 128 rows a lane copies 8 q + lane mod 8 + 32 (lane / 8), q = 0 .. 3: together the lanes read whole sectors and write
@@ -476,18 +519,25 @@ int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, co
   const long long mb = (a.N + LANES - 1) / LANES;
   const long long chunks = most_chunks(a.off.rows, a.off.groups, COLS);
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = parts;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  int attrs = 0;
+  if (SPLIT) {
+    attr[attrs].id = cudaLaunchAttributeClusterDimension;
+    attr[attrs].val.clusterDim.x = parts;
+    attr[attrs].val.clusterDim.y = 1;
+    attr[attrs++].val.clusterDim.z = 1;
+  }
+  if (a.behind) {
+    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[attrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
   // a cluster that shares a tile has no other
   cfg.gridDim = dim3(SPLIT ? (unsigned)(chunks * mb) * parts : (unsigned)min((long long)sms, chunks * mb));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = SPLIT ? 1 : 0;
+  cfg.numAttrs = attrs;
   e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, o, a);
   return e != cudaSuccess ? (int)e : pcl_last_error();
 }
@@ -500,9 +550,24 @@ int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CU
   return launch<COLS, SPLIT, __half>(p, q, qs, o, a, parts, stream);
 }
 
-bool blocks_of(long long rows, int words, long long* n) {
-  *n = (rows + QROWS - 1) / QROWS * words;
+// Blocks of the grid, and with how many passes a warp: four where that leaves every SM four blocks, else one
+bool blocks_of(long long rows, int words, long long* n, bool* long_rows) {
+  const long long down = (rows + QROWS - 1) / QROWS;
+  *long_rows = down * ((words + 7) / 8) >= 4 * 148;
+  *n = down * (*long_rows ? (words + 7) / 8 : (words + 1) / 2);
   return *n < (1ll << 31);
+}
+
+template <class T>
+void launch_quantize(unsigned n, bool long_rows, const QuantArgs& a, cudaStream_t stream) {
+  if (long_rows) quantize_kernel<4, T><<<n, QTHREADS, 0, stream>>>(a);
+  else quantize_kernel<1, T><<<n, QTHREADS, 0, stream>>>(a);
+}
+
+template <class T>
+void launch_dequantize(unsigned n, bool long_rows, const DequantArgs& a, cudaStream_t stream) {
+  if (long_rows) dequantize_kernel<4, T><<<n, QTHREADS, 0, stream>>>(a);
+  else dequantize_kernel<1, T><<<n, QTHREADS, 0, stream>>>(a);
 }
 
 }  // namespace
@@ -512,11 +577,12 @@ static int quantize(const void* x, long long ldx, int in_type, void* data, void*
   const int size = in_type == TYPE_F32 ? 4 : 2;
   a.vec = ((uintptr_t)x & 15) == 0 && (ldx * size & 15) == 0;
   long long n;
-  if (rows < 0 || K < 1 || in_type < 0 || in_type > 2 || !blocks_of(rows, a.words, &n)) return (int)cudaErrorInvalidValue;
+  bool long_rows;
+  if (rows < 0 || K < 1 || in_type < 0 || in_type > 2 || !blocks_of(rows, a.words, &n, &long_rows)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
-  if (in_type == TYPE_F32) quantize_kernel<float><<<(unsigned)n, QTHREADS, 0, stream>>>(a);
-  else if (in_type == TYPE_BF16) quantize_kernel<__nv_bfloat16><<<(unsigned)n, QTHREADS, 0, stream>>>(a);
-  else quantize_kernel<__half><<<(unsigned)n, QTHREADS, 0, stream>>>(a);
+  if (in_type == TYPE_F32) launch_quantize<float>((unsigned)n, long_rows, a, stream);
+  else if (in_type == TYPE_BF16) launch_quantize<__nv_bfloat16>((unsigned)n, long_rows, a, stream);
+  else launch_quantize<__half>((unsigned)n, long_rows, a, stream);
   return pcl_last_error();
 }
 
@@ -532,11 +598,12 @@ PCL_API int pcl_mx4_dequantize(const void* data, const void* scales, void* out, 
   const int size = out_type == TYPE_F32 ? 4 : 2;
   a.vec = ((uintptr_t)out & 15) == 0 && (ldo * size & 15) == 0;
   long long n;
-  if (rows < 0 || K < 1 || out_type < 0 || out_type > 2 || !blocks_of(rows, a.words, &n)) return (int)cudaErrorInvalidValue;
+  bool long_rows;
+  if (rows < 0 || K < 1 || out_type < 0 || out_type > 2 || !blocks_of(rows, a.words, &n, &long_rows)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
-  if (out_type == TYPE_F32) dequantize_kernel<float><<<(unsigned)n, QTHREADS, 0, stream>>>(a);
-  else if (out_type == TYPE_BF16) dequantize_kernel<__nv_bfloat16><<<(unsigned)n, QTHREADS, 0, stream>>>(a);
-  else dequantize_kernel<__half><<<(unsigned)n, QTHREADS, 0, stream>>>(a);
+  if (out_type == TYPE_F32) launch_dequantize<float>((unsigned)n, long_rows, a, stream);
+  else if (out_type == TYPE_BF16) launch_dequantize<__nv_bfloat16>((unsigned)n, long_rows, a, stream);
+  else launch_dequantize<__half>((unsigned)n, long_rows, a, stream);
   return pcl_last_error();
 }
 
@@ -565,7 +632,7 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
   if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, SMALL_BOX);
   if (rc) return rc;
   Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
-         N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false};
+         N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false, x_type >= 0};
   a.boxed = make_out_map(&o, p, out_type, out, N, rows, 1, ldo, ldo);
   if (!few) return launch_as<MANY_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
   const long long tiles = most_chunks(rows, groups, FEW_COLS) * ((N + LANES - 1) / LANES);
