@@ -75,6 +75,9 @@ SHAPES = [
     ([16, 31, 33, 1], 3, 72, 200), ([64] * 4, 0, 64, 64), ([128, 256], 0, 256, 128), ([127, 129, 255, 257], 1, 257, 129),
     ([300, 0, 0, 1, 511], 17, 520, 264), ([1000], 0, 1001, 777), ([5] * 100, 0, 100, 100), ([0] * 63 + [70], 0, 136, 328),
     ([2, 260, 3], 0, 128, 1032), ([1500, 40], 0, 384, 512), ([600, 17], 0, 900, 2050),
+    # a cluster for a tile; tiles of 256 rows for one CTA, and for a pair; with ends of every kind
+    ([1], 0, 300, 1000), ([3, 0, 1], 2, 256, 520), ([33, 64], 0, 130, 4100), ([700, 0, 1300, 33, 256], 5, 2000, 1900),
+    ([700, 0, 1300, 33, 256], 5, 4008, 3800), ([257, 15, 1000, 0, 500, 470, 60], 0, 3777, 4001),
 ]
 
 

@@ -137,7 +137,9 @@ def _grid(rows, k, seed):
 
 
 PRODUCTS = [(1, 1, 1), (1, 8, 32), (1, 128, 64), (1, 4096, 512), (2, 130, 33), (7, 1000, 100), (8, 256, 256), (17, 129, 257), (64, 64, 1024),
-            (100, 200, 300), (129, 127, 511), (256, 384, 768), (300, 1001, 1000), (513, 260, 2050), (1000, 640, 96)]
+            (100, 200, 300), (129, 127, 511), (256, 384, 768), (300, 1001, 1000), (513, 260, 2050), (1000, 640, 96),
+            # a cluster for a tile; tiles of as many rows as an accumulator holds
+            (1, 300, 2100), (64, 129, 4000), (33, 1000, 2048), (3000, 2500, 520), (2113, 4000, 300), (1700, 3333, 2049)]
 
 
 @pytest.mark.parametrize("M,N,K", PRODUCTS)
@@ -187,7 +189,8 @@ def test_far_scales():
 
 GROUPS = [([1], 0, 1, 1), ([0, 1, 0], 0, 33, 40), ([0, 0], 5, 40, 32), ([7, 0, 9], 0, 130, 65), ([16, 31, 33, 1], 3, 72, 200),
           ([127, 129, 255, 257], 1, 257, 130), ([300, 0, 0, 1, 511], 17, 520, 264), ([5] * 100, 0, 100, 100), ([0] * 63 + [70], 0, 136, 328),
-          ([2, 260, 3], 0, 128, 1056), ([1500, 40], 0, 384, 512)]
+          ([2, 260, 3], 0, 128, 1056), ([1500, 40], 0, 384, 512),
+          ([3, 0, 1], 2, 256, 2100), ([33, 64], 0, 130, 4096), ([700, 0, 1300, 33, 208], 5, 2500, 288), ([257, 15, 1000, 0, 500, 470, 60], 0, 3333, 520)]
 
 
 @pytest.mark.parametrize("counts,spare,N,K", GROUPS)
