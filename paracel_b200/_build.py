@@ -1,13 +1,15 @@
 """In-tree build of the native parts of paracel_b200.
 
-Two artefacts are produced under ``paracel_b200/_lib``:
+Three artefacts are produced under ``paracel_b200/_lib``:
 
 * ``libpcl_kernels.so`` -- every ``csrc/cuda/*.cu`` compiled by nvcc for
   sm_100a only (``-gencode arch=compute_100a,code=sm_100a``) and linked into
   one shared object with a plain C ABI (loaded through ctypes);
 * ``_pcl_core*.so`` -- the host runtime (KV store, parameter-server daemon,
   wire protocol client, msgpack codec, hash ring, partitioner, parsers,
-  ball tree, default handlers) as a pybind11 module.
+  ball tree, default handlers) as a pybind11 module;
+* ``_pcl_calls*.so`` -- the plain calls of the smallest products over torch's C++ interface
+  (``csrc/calls``), which launch the kernels of the first.
 
 The reference builds its native parts with CMake (CMakeLists.txt:1-75,
 src/CMakeLists.txt:1-16); this file plays that role.  nvcc cross-compiles, so
@@ -135,10 +137,36 @@ def build_core(force=False, verbose=False) -> Path:
     return out
 
 
+def calls_path() -> Path:
+    return LIB / ("_pcl_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_calls(force=False, verbose=False) -> Path:
+    import torch
+
+    LIB.mkdir(exist_ok=True)
+    src = CSRC / "calls" / "calls.cpp"
+    out = calls_path()
+    st = _stamp([src], " ".join(CXX_FLAGS) + torch.__version__)
+    stamp_file = LIB / "calls.stamp"
+    if not force and out.exists() and stamp_file.exists() and stamp_file.read_text() == st:
+        return out
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    _run(["g++", *CXX_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", root / "include",
+          "-isystem", root / "include" / "torch" / "csrc" / "api" / "include", "-isystem", cuda / "include",
+          "-isystem", sysconfig.get_paths()["include"], "-shared", "-o", out, src, "-L", root / "lib",
+          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"], verbose)
+    stamp_file.write_text(st)
+    return out
+
+
 def build_all(force=False, verbose=False):
-    k = build_kernels(force=force, verbose=verbose)
-    c = build_core(force=force, verbose=verbose)
-    return k, c
+    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        calls = ex.submit(build_calls, force=force, verbose=verbose)
+        k = build_kernels(force=force, verbose=verbose)
+        c = build_core(force=force, verbose=verbose)
+        return k, c, calls.result()
 
 
 if __name__ == "__main__":

@@ -1,0 +1,243 @@
+// Python module `_pcl_calls`: the plain calls of the products by group and of the four-bit matrices without Python's part of their cost.
+//
+// A call of these takes the device a few microseconds at the smallest sizes, and looking at the tensors, two torch.empty and a foreign call
+// through ctypes took the host more than the launches themselves.  Every function here looks at its arguments, and where they are
+// as they mostly are (one device, the current one; aligned rows; a new result) makes the result and launches; for anything else, an error
+// among it, it returns None, and the caller goes the long way.  The launchers are the extern "C" ones of libpcl_kernels.so, bound
+// by address.
+#include <Python.h>
+
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+namespace {
+
+using Rows = int (*)(int, int, int, const void*, long long, const void*, long long, long long, const void*, int, void*, long long,
+                     long long, int, int, int, int, cudaStream_t);
+using Tn = int (*)(int, int, const void*, long long, const void*, long long, const void*, int, void*, long long, int, int, int,
+                   cudaStream_t);
+using Quantize = int (*)(const void*, long long, int, void*, void*, long long, int, cudaStream_t);
+using Dequantize = int (*)(const void*, const void*, void*, long long, int, long long, int, cudaStream_t);
+using Mx4Rows = int (*)(const void*, long long, int, void*, void*, const void*, const void*, const void*, int, void*, long long, int, long long,
+                        int, int, int, int, cudaStream_t);
+using ErrorString = const char* (*)(int);
+
+Rows rows_fn;
+Tn tn_fn;
+Quantize quantize_fn;
+Dequantize dequantize_fn;
+Mx4Rows mx4_rows_fn;
+ErrorString error_fn;
+
+constexpr int64_t MAX_GROUPS = 1024, MAX_ROWS = (1ll << 31) - 512, MAX_SIZE = 1ll << 30;
+
+// number of a type as the launchers have it, -1 for others
+int type_of(at::ScalarType t) {
+  return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1;
+}
+
+bool is_tensor(PyObject* o) { return THPVariable_Check(o); }
+const at::Tensor& tensor(PyObject* o) { return THPVariable_Unpack(o); }
+
+// out_dtype or, for None, `own`; false for what is neither
+bool type_arg(PyObject* o, at::ScalarType own, at::ScalarType* t) {
+  *t = own;
+  if (o == Py_None) return true;
+  if (!THPDtype_Check(o)) return false;
+  *t = reinterpret_cast<THPDtype*>(o)->scalar_type;
+  return true;
+}
+
+// on the current device
+bool here(const at::Tensor& t, int device) { return t.is_cuda() && t.get_device() == device; }
+
+bool plain_offsets(const at::Tensor& o, int device) {
+  return o.dim() == 1 && (o.scalar_type() == at::kInt || o.scalar_type() == at::kLong) && o.size(0) >= 2 &&
+         o.size(0) <= MAX_GROUPS + 1 && o.is_contiguous() && here(o, device);
+}
+
+bool aligned(const at::Tensor& t) {   // 16-bit rows at multiples of 16 bytes
+  const int64_t d = t.dim();
+  if ((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) || t.stride(d - 1) != 1) return false;
+  for (int64_t i = 0; i + 1 < d; ++i)
+    if (t.stride(i) <= 0 || (t.stride(i) & 7)) return false;
+  return true;
+}
+
+bool size_ok(int64_t v) { return v > 0 && v < MAX_SIZE; }
+
+template <class F>
+PyObject* launched(const char* name, F&& launch, const at::Tensor& result) {
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = launch();
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return PyErr_Format(PyExc_RuntimeError, "%s failed: CUDA error %d (%s)", name, rc, error_fn(rc));
+  return THPVariable_Wrap(result);
+}
+
+// bind(rows, tn, quantize, dequantize, mx4_rows, error_string): addresses
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) return PyErr_Format(PyExc_TypeError, "six addresses are wanted");
+  void* p[6];
+  for (int i = 0; i < 6; ++i) {
+    p[i] = PyLong_AsVoidPtr(a[i]);
+    if (p[i] == nullptr) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "address %d is null", i);
+  }
+  rows_fn = reinterpret_cast<Rows>(p[0]);
+  tn_fn = reinterpret_cast<Tn>(p[1]);
+  quantize_fn = reinterpret_cast<Quantize>(p[2]);
+  dequantize_fn = reinterpret_cast<Dequantize>(p[3]);
+  mx4_rows_fn = reinterpret_cast<Mx4Rows>(p[4]);
+  error_fn = reinterpret_cast<ErrorString>(p[5]);
+  Py_RETURN_NONE;
+}
+
+// grouped_rows(mode, X, W, offsets, out_dtype)
+PyObject* grouped_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || rows_fn == nullptr || !is_tensor(a[1]) || !is_tensor(a[2]) || !is_tensor(a[3])) Py_RETURN_NONE;
+  const long mode = PyLong_AsLong(a[0]);
+  const at::Tensor &X = tensor(a[1]), &W = tensor(a[2]), &offsets = tensor(a[3]);
+  if ((mode != 0 && mode != 1) || X.dim() != 2 || W.dim() != 3 || !X.is_cuda()) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::ScalarType type = X.scalar_type();
+  const int in = type_of(type);
+  at::ScalarType out_type;
+  const int64_t T = X.size(0), E = W.size(0), N = W.size(1), K = W.size(2);
+  if (in < 1 || W.scalar_type() != type || !type_arg(a[4], type, &out_type) || (out_type != type && out_type != at::kFloat) || T < 1 ||
+      T >= MAX_ROWS || !size_ok(N) || !size_ok(K) || X.size(1) != (mode == 0 ? K : N) || !plain_offsets(offsets, device) ||
+      offsets.size(0) != E + 1 || !here(X, device) || !here(W, device) || !aligned(X) || !aligned(W))
+    Py_RETURN_NONE;
+  const int64_t cols = mode == 0 ? N : K;
+  const at::Tensor out = at::empty({T, cols}, X.options().dtype(out_type));
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  return launched("pcl_grouped_rows", [&] {
+    return rows_fn((int)mode, in, type_of(out_type), X.data_ptr(), X.stride(0), W.data_ptr(), W.stride(0), W.stride(1), offsets.data_ptr(),
+                   offsets.scalar_type() == at::kLong, out.data_ptr(), cols, T, (int)E, (int)N, (int)K, 1, stream);
+  }, out);
+  END_HANDLE_TH_ERRORS
+}
+
+// grouped_tn(dY, X, offsets, out_dtype)
+PyObject* grouped_tn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || tn_fn == nullptr || !is_tensor(a[0]) || !is_tensor(a[1]) || !is_tensor(a[2])) Py_RETURN_NONE;
+  const at::Tensor &Y = tensor(a[0]), &X = tensor(a[1]), &offsets = tensor(a[2]);
+  if (X.dim() != 2 || Y.dim() != 2 || !X.is_cuda()) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::ScalarType type = X.scalar_type();
+  const int in = type_of(type);
+  at::ScalarType out_type;
+  const int64_t T = X.size(0), K = X.size(1), N = Y.size(1);
+  if (in < 1 || Y.scalar_type() != type || !type_arg(a[3], type, &out_type) || (out_type != type && out_type != at::kFloat) || T < 1 ||
+      T >= MAX_ROWS || Y.size(0) != T || !size_ok(N) || !size_ok(K) || !plain_offsets(offsets, device) || !here(X, device) || !here(Y, device) ||
+      !aligned(X) || !aligned(Y))
+    Py_RETURN_NONE;
+  const int64_t E = offsets.size(0) - 1;
+  const at::Tensor out = at::empty({E, N, K}, X.options().dtype(out_type));
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  return launched("pcl_grouped_tn", [&] {
+    return tn_fn(in, type_of(out_type), Y.data_ptr(), Y.stride(0), X.data_ptr(), X.stride(0), offsets.data_ptr(),
+                 offsets.scalar_type() == at::kLong, out.data_ptr(), T, (int)E, (int)N, (int)K, stream);
+  }, out);
+  END_HANDLE_TH_ERRORS
+}
+
+// rows of a matrix that is quantised: contiguous values, any distance
+bool plain_rows(const at::Tensor& x) { return x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1); }
+
+int64_t data_bytes(int64_t rows, int64_t cols) { return rows * ((cols + 31) / 32 * 16); }
+int64_t scale_bytes(int64_t rows, int64_t cols) { return rows * ((cols + 127) / 128 * 4); }
+
+// quantize(X) -> (bytes of data and scales, device, rows, cols, address of data, of scales)
+PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 1 || quantize_fn == nullptr || !is_tensor(a[0])) Py_RETURN_NONE;
+  const at::Tensor& X = tensor(a[0]);
+  if (!X.is_cuda() || type_of(X.scalar_type()) < 0 || !(plain_rows(X) || (X.dim() == 3 && X.is_contiguous()))) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const int64_t d = X.dim(), K = X.size(d - 1);
+  if (!size_ok(K) || !here(X, device)) Py_RETURN_NONE;
+  const int64_t rows = d == 2 ? X.size(0) : X.size(0) * X.size(1);
+  if (rows < 1 || rows >= MAX_ROWS) Py_RETURN_NONE;
+  const at::Tensor buf = at::empty({data_bytes(rows, K) + scale_bytes(rows, K)}, X.options().dtype(at::kByte));
+  uint8_t* data = static_cast<uint8_t*>(buf.data_ptr());
+  uint8_t* scales = data + data_bytes(rows, K);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  PyObject* t = launched("pcl_mx4_quantize", [&] {
+    return quantize_fn(X.data_ptr(), X.stride(d - 2), type_of(X.scalar_type()), data, scales, rows, (int)K, stream);
+  }, buf);
+  if (t == nullptr) return nullptr;
+  return Py_BuildValue("(NiLLKK)", t, device, (long long)rows, (long long)K, (unsigned long long)(uintptr_t)data,
+                       (unsigned long long)(uintptr_t)scales);
+  END_HANDLE_TH_ERRORS
+}
+
+// dequantize(a tensor on the matrix's device, address of data, of scales, rows, cols, dtype)
+PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  at::ScalarType type;
+  if (n != 6 || dequantize_fn == nullptr || !is_tensor(a[0]) || a[5] == Py_None || !type_arg(a[5], at::kFloat, &type)) Py_RETURN_NONE;
+  const at::Tensor& base = tensor(a[0]);
+  if (!base.is_cuda() || type_of(type) < 0) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const long long rows = PyLong_AsLongLong(a[3]), cols = PyLong_AsLongLong(a[4]);
+  void *data = PyLong_AsVoidPtr(a[1]), *scales = PyLong_AsVoidPtr(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  if (rows < 1 || !size_ok(cols) || !here(base, device)) Py_RETURN_NONE;
+  const at::Tensor out = at::empty({rows, cols}, base.options().dtype(type));
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  return launched("pcl_mx4_dequantize", [&] { return dequantize_fn(data, scales, out.data_ptr(), cols, type_of(type), rows, (int)cols, stream); }, out);
+  END_HANDLE_TH_ERRORS
+}
+
+// mx4_rows(A, address of B's data, of its scales, B's rows, cols, device, offsets or None, out_dtype): A is quantised in the call
+PyObject* mx4_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || mx4_rows_fn == nullptr || !is_tensor(a[0]) || !(a[6] == Py_None || is_tensor(a[6]))) Py_RETURN_NONE;
+  const at::Tensor& A = tensor(a[0]);
+  at::ScalarType out_type;
+  if (!A.is_cuda() || !plain_rows(A) || type_of(A.scalar_type()) < 0 || !type_arg(a[7], A.scalar_type(), &out_type) || type_of(out_type) < 0)
+    Py_RETURN_NONE;
+  void *data = PyLong_AsVoidPtr(a[1]), *scales = PyLong_AsVoidPtr(a[2]);
+  const long long rows = PyLong_AsLongLong(a[3]), K = PyLong_AsLongLong(a[4]), b_device = PyLong_AsLongLong(a[5]);
+  if (PyErr_Occurred()) return nullptr;
+  const int device = c10::cuda::current_device();
+  const int64_t T = A.size(0);
+  if (A.size(1) != K || !here(A, device) || b_device != device || T < 1 || T >= MAX_ROWS) Py_RETURN_NONE;
+  int64_t groups = 1;
+  const void* offsets = nullptr;
+  bool wide = false;
+  if (a[6] != Py_None) {
+    const at::Tensor& o = tensor(a[6]);
+    if (!plain_offsets(o, device)) Py_RETURN_NONE;
+    groups = o.size(0) - 1;
+    offsets = o.data_ptr();
+    wide = o.scalar_type() == at::kLong;
+  }
+  if (rows < 1 || rows % groups) Py_RETURN_NONE;
+  const int64_t N = rows / groups;
+  const at::Tensor out = at::empty({T, N}, A.options().dtype(out_type));
+  const at::Tensor work = at::empty({data_bytes(T, K) + scale_bytes(T, K)}, A.options().dtype(at::kByte));
+  uint8_t* qa = static_cast<uint8_t*>(work.data_ptr());
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  return launched("pcl_mx4_rows", [&] {
+    return mx4_rows_fn(A.data_ptr(), A.stride(0), type_of(A.scalar_type()), qa, qa + data_bytes(T, K), data, scales, offsets, wide,
+                       out.data_ptr(), N, type_of(out_type), T, (int)groups, (int)N, (int)K, 1, stream);
+  }, out);
+  END_HANDLE_TH_ERRORS
+}
+
+#define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {FAST(bind), FAST(grouped_rows), FAST(grouped_tn), FAST(quantize), FAST(dequantize), FAST(mx4_rows),
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pcl_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__pcl_calls(void) { return PyModule_Create(&module); }

@@ -144,8 +144,14 @@ _LAUNCHES = 0
 
 
 def launches() -> int:
-    """Number of kernel-launching calls made through :func:`call` so far."""
+    """Number of kernel-launching calls made through :func:`call` (or counted by :func:`count_launch`) so far."""
     return _LAUNCHES
+
+
+def count_launch() -> None:
+    """One kernel-launching call that did not go through :func:`call`."""
+    global _LAUNCHES
+    _LAUNCHES += 1
 
 
 def call(name: str, *args) -> None:

@@ -18,6 +18,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
+from ._calls import calls
 from .grouped import MAX_GROUPS, MAX_ROWS, TYPES, check_devices, check_offsets, check_out, read_status, result_type
 
 BLOCK = 32
@@ -45,14 +46,11 @@ class Mx4Matrix:
         self.rows, self.cols, self._data_ptr, self._scales_ptr = ds[0], cols, data_ptr, scales_ptr
 
     @classmethod
-    def _empty(cls, rows: int, cols: int, device: torch.device) -> "Mx4Matrix":
-        """One whose values are not set: both parts in one allocation (two and their checks take 3 us more)."""
+    def _of(cls, buf: torch.Tensor, device: int, rows: int, cols: int, data_ptr: int, scales_ptr: int) -> "Mx4Matrix":
+        """One whose parts lie in ``buf``, the scales behind the data, and are looked at as tensors only when asked for."""
         q = cls.__new__(cls)
-        size = rows * ((cols + 31) // 32 * 16)           # a multiple of 16
-        buf = torch.empty(size + (cols + 127) // 128 * rows * 4, dtype=torch.uint8, device=device)
-        q._data, q._scales, q._buf, q._device, q.rows, q.cols = None, None, buf, buf.get_device(), rows, cols
-        q._data_ptr = buf.data_ptr()
-        q._scales_ptr = q._data_ptr + size
+        q._data, q._scales, q._buf, q._device, q.rows, q.cols = None, None, buf, device, rows, cols
+        q._data_ptr, q._scales_ptr = data_ptr, scales_ptr
         return q
 
     @property
@@ -103,6 +101,11 @@ def check_status(device=None) -> None:
 def mx4_quantize(X: torch.Tensor) -> Mx4Matrix:
     """``X [rows, K]`` (float32, bfloat16, float16) in four bits; ``X [E, N, K]``, the matrices of E groups, becomes one
     of ``E N`` rows."""
+    if X.is_cuda:
+        parts = calls().quantize(X)
+        if parts is not None:
+            _lib.count_launch()
+            return Mx4Matrix._of(*parts)
     shape, kind, device = X.shape, TYPES.get(X.dtype), X.get_device()
     if kind is None:
         raise ValueError(f"X must be float32, bfloat16 or float16, got {X.dtype}")
@@ -119,7 +122,9 @@ def mx4_quantize(X: torch.Tensor) -> Mx4Matrix:
     rows = X.shape[0]
     if rows >= MAX_ROWS:
         raise ValueError(f"at most 2^31 - 513 rows, got {rows}")
-    q = Mx4Matrix._empty(rows, K, X.device)
+    size = rows * ((K + 31) // 32 * 16)                  # a multiple of 16
+    buf = torch.empty(size + (K + 127) // 128 * rows * 4, dtype=torch.uint8, device=X.device)
+    q = Mx4Matrix._of(buf, device, rows, K, buf.data_ptr(), buf.data_ptr() + size)
     if rows:
         _lib.call_on(device, "pcl_mx4_quantize", X.data_ptr(), ldx, kind, q._data_ptr, q._scales_ptr, rows, K)
     return q
@@ -139,6 +144,11 @@ def mx4_dequantize(q: Mx4Matrix, dtype: torch.dtype = torch.float32, out: Option
     either); float16 rounds."""
     if dtype not in TYPES:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+    if out is None and q._device >= 0:
+        out = calls().dequantize(q._data if q._buf is None else q._buf, q._data_ptr, q._scales_ptr, q.rows, q.cols, dtype)
+        if out is not None:
+            _lib.count_launch()
+            return out
     if out is not None or q._device < 0:
         check_out(out, (q.rows, q.cols), dtype)
         check_devices(q=q, out=out)
@@ -175,6 +185,11 @@ def _product(A, B: Mx4Matrix, offsets, out, out_dtype):
     if not isinstance(B, Mx4Matrix):
         _check_product(A, B, offsets, out, out_dtype)
     K, rows, device = B.cols, B.rows, B._device
+    if out is None and not packed and A.is_cuda:
+        out = calls().mx4_rows(A, B._data_ptr, B._scales_ptr, rows, K, device, offsets, out_dtype)
+        if out is not None:
+            _lib.count_launch()
+            return out
     if packed:
         T, cols, kind, place, own = A.rows, A.cols, -1, A._device, torch.float32
     else:
