@@ -396,30 +396,41 @@ int launch_as(int in_type, int out_type, const CUtensorMap& p, const CUtensorMap
   return in_type == TYPE_BF16 ? launch<MODE, CG, COLS, SPLIT, __nv_bfloat16>(p, q, qs, o, a, parts, stream) : launch<MODE, CG, COLS, SPLIT, __half>(p, q, qs, o, a, parts, stream);
 }
 
-// Whether pairs of CTAs take the tiles.  A pair loads a third fewer bytes for its 256 x 256 tile than two CTAs for theirs, but there are half as
-// many tiles: below two for every SM single CTAs spread better.
-bool use_pairs(long long chunks, int mdim) { return chunks * ((mdim + LANES - 1) / LANES) >= 2 * 148; }
+// The shapes of a call's tiles: tiles of at most 64, 128 or 256 rows of Q, whichever takes the shortest time; and of 256 by pairs of CTAs, which load a third
+// fewer bytes for a tile of 256 x 256 than two CTAs for theirs, where there are two tiles for every SM without (fewer spread better).  Measured, us:
+// 1537 rows of 11 groups, nt, 1001 x 776: 15.1 with 64, 13.3 with 128, 16.6 with 256; 16 rows of 32 groups, nt, 1536 x 1024: 9.2 with 64, 10.3 with 256.
+enum Shape { FEW, SOME, MANY, PAIR };
+constexpr int FEW_COLS = 64, SOME_COLS = 128;
+constexpr int SHAPE_COLS[] = {FEW_COLS, SOME_COLS, MAX_COLS, MAX_COLS / 2 /* of each CTA */};
 
-// The forms of nt and nn.  FEW: groups of few rows stream their matrices once, and what counts is how many bytes are on their way: a stage
-// without room for 256 rows of Q is 24 KB instead of 48, and there are eight instead of four.
-enum RowsForm { FEW, SINGLE, PAIR };
-constexpr int FEW_COLS = 64;
+// tn takes the last two only: with few rows to a group its tiles have few stages, and 64 columns instead of 256 in each took 11.1 instead of 9.2 us for 1000
+// rows of 24 groups, 520 x 264.
+bool pairs_pay(long long chunks, int mdim) { return chunks * ((mdim + LANES - 1) / LANES) >= 2 * 148; }
 
-RowsForm rows_form(long long rows, int groups, int mdim) {
-  const long long chunks = rows / MAX_COLS + min((long long)groups, rows) / 2;
-  if (rows <= FEW_COLS || rows / groups <= FEW_COLS / 4 || chunks * ((mdim + LANES - 1) / LANES) < 148) return FEW;
-  return use_pairs(chunks, mdim) ? PAIR : SINGLE;
+Shape shape_of(long long rows, int groups, int mdim, int steps) {
+  Shape best = FEW;
+  long long least = -1, chunks = 0;
+  for (const Shape f : {FEW, SOME, MANY}) {
+    chunks = likely_chunks(rows, groups, SHAPE_COLS[f]);
+    const long long c = tiles_cost(chunks, SHAPE_COLS[f], mdim, steps, 148);
+    if (least < 0 || c < least) { least = c; best = f; }
+  }
+  return best == MANY && pairs_pay(chunks, mdim) ? PAIR : best;
 }
 
 template <int MODE>
-int launch_form(RowsForm form, int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o,
-                const Args& a, cudaStream_t stream) {
-  if (form == SINGLE) return launch_as<MODE, 1, MAX_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
-  if (form == PAIR) return launch_as<MODE, 2, MAX_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
-  const long long tiles = most_chunks(a.off.rows, a.off.groups, FEW_COLS) * ((a.mdim + LANES - 1) / LANES);
-  const int parts = parts_of(tiles, (a.red + BR - 1) / BR, 148);
-  return parts > 1 ? launch_as<MODE, 1, FEW_COLS, true>(in_type, out_type, p, q, qs, o, a, parts, stream)
-                   : launch_as<MODE, 1, FEW_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
+int launch_shape(Shape shape, int in_type, int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o,
+                 const Args& a, cudaStream_t stream) {
+  if (shape == MANY) return launch_as<MODE, 1, MAX_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
+  if (shape == PAIR) return launch_as<MODE, 2, MAX_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
+  if constexpr (MODE != TN) {
+    if (shape == SOME) return launch_as<MODE, 1, SOME_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
+    const long long tiles = most_chunks(a.off.rows, a.off.groups, FEW_COLS) * ((a.mdim + LANES - 1) / LANES);
+    const int parts = parts_of(tiles, (a.red + BR - 1) / BR, 148);
+    return parts > 1 ? launch_as<MODE, 1, FEW_COLS, true>(in_type, out_type, p, q, qs, o, a, parts, stream)
+                     : launch_as<MODE, 1, FEW_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
+  }
+  return (int)cudaErrorInvalidValue;
 }
 
 bool sizes_ok(int in_type, long long rows, int groups, int N, int K) {
@@ -440,16 +451,16 @@ PCL_API int pcl_grouped_rows(int mode, int in_type, int out_type, const void* X,
   if (rows == 0) return 0;
   const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int red = mode == 0 ? K : N;
-  const RowsForm form = rows_form(rows, groups, mode == 0 ? N : K);
+  const Shape shape = shape_of(rows, groups, mode == 0 ? N : K, (red + BR - 1) / BR);
   CUtensorMap p, q, qs, o;
   int rc = make_map_3d(&p, t, W, K, N, groups, ws_n * 2, ws_e * 2, 64, mode == 0 ? LANES : BR);
-  if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, form == FEW ? FEW_COLS : form == PAIR ? MAX_COLS / 2 : MAX_COLS);
+  if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SHAPE_COLS[shape]);
   if (rc == 0) rc = make_map_3d(&qs, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SMALL_BOX);
   if (rc) return rc;
   Args a{out, ldo, Offsets{offsets, off64, groups, (int)rows}, mode == 0 ? N : K, 0, red, in_type == TYPE_BF16 ? 1u : 0u, fill, false};
   a.boxed = make_out_map(&o, p, out_type, out, a.mdim, rows, 1, ldo, ldo);
-  if (mode == 0) return launch_form<NT>(form, in_type, out_type, p, q, qs, o, a, stream);
-  return launch_form<NN>(form, in_type, out_type, p, q, qs, o, a, stream);
+  if (mode == 0) return launch_shape<NT>(shape, in_type, out_type, p, q, qs, o, a, stream);
+  return launch_shape<NN>(shape, in_type, out_type, p, q, qs, o, a, stream);
 }
 
 // out [groups, N, K] (contiguous): every matrix is written, zeros where a group has no row
@@ -464,8 +475,8 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
   if (rc) return rc;
   Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0, false};
   a.boxed = make_out_map(&o, p, out_type, out, K, N, groups, K, (long long)N * K);
-  return use_pairs((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K) ? launch_as<TN, 2, MAX_COLS, false>(in_type, out_type, p, q, q, o, a, 1, stream)
-                                                                            : launch_as<TN, 1, MAX_COLS, false>(in_type, out_type, p, q, q, o, a, 1, stream);
+  const bool pair = pairs_pay((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K);
+  return launch_shape<TN>(pair ? PAIR : MANY, in_type, out_type, p, q, q, o, a, stream);
 }
 
 // Copies the status block of the grouped products to `host` and clears it (waits for the stream).

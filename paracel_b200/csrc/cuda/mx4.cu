@@ -213,7 +213,7 @@ constexpr int SCALE_WARP = 2 + EPI_WARPS;
 constexpr int THREADS = 32 * (SCALE_WARP + 3);
 constexpr int SMALL_BOX = 32;
 
-// COLS: columns of an accumulator, the most rows of A in a tile.  64 of them leave room for seven stages of 27 KB, 208 for four of 45.
+// COLS: columns of an accumulator, the most rows of A in a tile.  64 of them leave room for seven stages of 27 KB, 128 for five of 35, 208 for four of 45.
 // SPLIT: a cluster shares a tile's reduction (COLS 64 only)
 template <int COLS, bool SPLIT>
 struct Form {
@@ -224,7 +224,7 @@ struct Form {
   static_assert(2 * COLS + STAGES * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
   static_assert(COLS % 16 == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
 };
-constexpr int FEW_COLS = 64, MANY_COLS = 208;
+constexpr int FEW_COLS = 64, SOME_COLS = 128, MANY_COLS = 208;
 
 struct Args {
   const uint32_t* sp;   // words of B's scales [words, groups * N]
@@ -622,19 +622,24 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
     if (rc) return rc;
   }
   const long long row_bytes = (K + 31) / 32 * 16;
-  // groups of few rows stream their matrices, and what counts is how many bytes are on their way
-  const bool few = rows <= FEW_COLS || rows / groups <= FEW_COLS / 4 ||
-                   (rows / MANY_COLS + min((long long)groups, rows) / 2) * ((N + LANES - 1) / LANES) < 148;
+  // tiles of the number of rows that takes the shortest time
+  int cols = 0;
+  long long least = 0;
+  for (const int c : {FEW_COLS, SOME_COLS, MANY_COLS}) {
+    const long long t = tiles_cost(likely_chunks(rows, groups, c), c, N, (int)((row_bytes + 127) / 128), 148);
+    if (cols == 0 || t < least) { cols = c; least = t; }
+  }
   CUtensorMap p, q, qs, o;
   const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int rc = make_map_3d(&p, t, B, row_bytes, N, groups, row_bytes, row_bytes * N, 128, LANES);
-  if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, few ? FEW_COLS : MANY_COLS);
+  if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, cols);
   if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, SMALL_BOX);
   if (rc) return rc;
   Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
          N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false, x_type >= 0};
   a.boxed = make_out_map(&o, p, out_type, out, N, rows, 1, ldo, ldo);
-  if (!few) return launch_as<MANY_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
+  if (cols == SOME_COLS) return launch_as<SOME_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
+  if (cols == MANY_COLS) return launch_as<MANY_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
   const long long tiles = most_chunks(rows, groups, FEW_COLS) * ((N + LANES - 1) / LANES);
   const int parts = parts_of(tiles, a.steps, 148);
   return parts > 1 ? launch_as<FEW_COLS, true>(out_type, p, q, qs, o, a, parts, stream) : launch_as<FEW_COLS, false>(out_type, p, q, qs, o, a, 1, stream);

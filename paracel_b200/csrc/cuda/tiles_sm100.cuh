@@ -373,6 +373,20 @@ static inline long long most_chunks(long long rows, int groups, int cols) {
   return (rows - taken) / cols + taken;
 }
 
+// How long a call of single CTAs takes with `chunks` chunks of at most `cols` rows of Q, in units of about 2.5 cycles.  A CTA takes in 52 bytes a cycle
+// whatever it computes, so a stage costs its 128 + cols lines of 128 bytes; storing a tile takes 21 cycles a column, beside the
+// next tile's stages.
+static inline long long tiles_cost(long long chunks, int cols, int mdim, int steps, int sms) {
+  const long long tiles = chunks * ((mdim + 127) / 128), store = 9ll * cols, main = (long long)steps * (128 + cols);
+  return (tiles + sms - 1) / sms * (main > store ? main : store) + store;
+}
+
+// Chunks that `rows` rows of `groups` groups may be expected to make: half a chunk more for each group, one at least
+static inline long long likely_chunks(long long rows, int groups, int cols) {
+  const long long taken = rows < groups ? rows : groups, all = (rows + cols - 1) / cols;
+  return taken <= 1 ? all : (taken > all + taken / 2 ? taken : all + taken / 2);
+}
+
 // Parts that a tile's reduction of `steps` stages is cut into where `tiles` of them leave more than half the SMs idle: as many as fill these, at most
 // eight (the largest portable cluster), and two stages at least for each.  1: not cut.
 static inline int parts_of(long long tiles, int steps, int sms) {
