@@ -282,7 +282,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const int last = (stage + steps + STAGES - 1) % STAGES;
       stage = (stage + steps) % STAGES;
       if (len % BR == 0) continue;
-      if (!mbar_wait(s.tail + last, (phases >> last) & 1u, abort_flag)) {
+      if (!wait_full(s.tail + last, (phases >> last) & 1u, abort_flag, tile_ns(steps))) {
         if (lane == 0) report(&g_status, 0, 45, last, 0);
         abort_all<CG>(abort_flag, me ^ 1u);
         ok = false;
@@ -315,7 +315,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
           for (int j = half; j < w.n; j += 2) dst[(long long)j * a.ldo + lane] = to_out<TO>(0.f);
         continue;
       }
-      if (!mbar_wait(s.tfull + acc, acc_phase >> acc & 1u, abort_flag)) {
+      if (!wait_full(s.tfull + acc, acc_phase >> acc & 1u, abort_flag, tile_ns((w.r1 - w.r0) / BR))) {
         if (lane == 0) report(&g_status, 0, 44, acc, 0);
         abort_all<CG>(abort_flag, me ^ 1u);
         ok = false;
@@ -405,14 +405,14 @@ constexpr int SHAPE_COLS[] = {FEW_COLS, SOME_COLS, MAX_COLS, MAX_COLS / 2 /* of 
 
 // tn takes the last two only: with few rows to a group its tiles have few stages, and 64 columns instead of 256 in each took 11.1 instead of 9.2 us for 1000
 // rows of 24 groups, 520 x 264.
-bool pairs_pay(long long chunks, int mdim) { return chunks * ((mdim + LANES - 1) / LANES) >= 2 * 148; }
+bool pairs_pay(long long chunks, int mdim) { return chunks * ((mdim + LANES - 1) / LANES) >= 2 * SMS; }
 
 Shape shape_of(long long rows, int groups, int mdim, int steps) {
   Shape best = FEW;
   long long least = -1, chunks = 0;
   for (const Shape f : {FEW, SOME, MANY}) {
     chunks = likely_chunks(rows, groups, SHAPE_COLS[f]);
-    const long long c = tiles_cost(chunks, SHAPE_COLS[f], mdim, steps, 148);
+    const long long c = tiles_cost(chunks, SHAPE_COLS[f], mdim, steps);
     if (least < 0 || c < least) { least = c; best = f; }
   }
   return best == MANY && pairs_pay(chunks, mdim) ? PAIR : best;
@@ -426,7 +426,7 @@ int launch_shape(Shape shape, int in_type, int out_type, const CUtensorMap& p, c
   if constexpr (MODE != TN) {
     if (shape == SOME) return launch_as<MODE, 1, SOME_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
     const long long tiles = most_chunks(a.off.rows, a.off.groups, FEW_COLS) * ((a.mdim + LANES - 1) / LANES);
-    const int parts = parts_of(tiles, (a.red + BR - 1) / BR, 148);
+    const int parts = parts_of(tiles, (a.red + BR - 1) / BR);
     return parts > 1 ? launch_as<MODE, 1, FEW_COLS, true>(in_type, out_type, p, q, qs, o, a, parts, stream)
                      : launch_as<MODE, 1, FEW_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
   }

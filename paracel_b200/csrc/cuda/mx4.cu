@@ -466,7 +466,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     uint32_t acc_phase = 0;                   // bit i: accumulator i
     for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
-      if (!mbar_wait(s.tfull + acc, acc_phase >> acc & 1u, abort_flag)) { gave_up(44, acc, 0); break; }
+      if (!wait_full(s.tfull + acc, acc_phase >> acc & 1u, abort_flag, tile_ns(w.k1 - w.k0))) { gave_up(44, acc, 0); break; }
       acc_phase ^= 1u << acc;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int m = w.m0 + sub * 32;
@@ -553,7 +553,7 @@ int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CU
 // Blocks of the grid, and with how many passes a warp: four where that leaves every SM four blocks, else one
 bool blocks_of(long long rows, int words, long long* n, bool* long_rows) {
   const long long down = (rows + QROWS - 1) / QROWS;
-  *long_rows = down * ((words + 7) / 8) >= 4 * 148;
+  *long_rows = down * ((words + 7) / 8) >= 4 * SMS;
   *n = down * (*long_rows ? (words + 7) / 8 : (words + 1) / 2);
   return *n < (1ll << 31);
 }
@@ -626,7 +626,7 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
   int cols = 0;
   long long least = 0;
   for (const int c : {FEW_COLS, SOME_COLS, MANY_COLS}) {
-    const long long t = tiles_cost(likely_chunks(rows, groups, c), c, N, (int)((row_bytes + 127) / 128), 148);
+    const long long t = tiles_cost(likely_chunks(rows, groups, c), c, N, (int)((row_bytes + 127) / 128));
     if (cols == 0 || t < least) { cols = c; least = t; }
   }
   CUtensorMap p, q, qs, o;
@@ -641,7 +641,7 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
   if (cols == SOME_COLS) return launch_as<SOME_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
   if (cols == MANY_COLS) return launch_as<MANY_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
   const long long tiles = most_chunks(rows, groups, FEW_COLS) * ((N + LANES - 1) / LANES);
-  const int parts = parts_of(tiles, a.steps, 148);
+  const int parts = parts_of(tiles, a.steps);
   return parts > 1 ? launch_as<FEW_COLS, true>(out_type, p, q, qs, o, a, parts, stream) : launch_as<FEW_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
 }
 

@@ -14,6 +14,7 @@ namespace pcl_tiles {
 using namespace pcl_sm100;
 
 constexpr int MAX_COLS = 256;   // columns of an accumulator
+constexpr int SMS = 148;        // that the rules for a call's shape count on
 
 // The rows of a group are cut into chunks of at most MAX_COLS, as equal as multiples of `step` allow.
 struct Table {
@@ -94,8 +95,8 @@ __device__ __forceinline__ bool has_passed(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
-// as mbar_wait, for a barrier that the other CTA of a pair arrives on
-__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+// as mbar_wait, for a barrier that the other CTA of a pair arrives on; the limit grows by `more_ns`
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned long long more_ns = 0) {
   const uint32_t addr = smem_u32(bar);
   unsigned long long t0 = 0;
   for (unsigned it = 0;; ++it) {
@@ -112,10 +113,12 @@ __device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, volati
       if (*abort_flag) return false;
       const unsigned long long now = pcl_globaltimer();
       if (t0 == 0) t0 = now;
-      else if (now - t0 > WAIT_NS) return false;
+      else if (now - t0 > WAIT_NS + more_ns) return false;
     }
   }
 }
+// What a tile of `steps` stages may take beyond the usual limit (a stage takes a fraction of a microsecond; a reduction over 2^31 rows has 2^25)
+__device__ __forceinline__ unsigned long long tile_ns(int steps) { return 2000ull * (unsigned)steps; }
 
 // arrive on a barrier given by its cluster address, after this CTA's writes to its shared memory
 __device__ __forceinline__ void arrive_cluster(uint32_t cluster_addr) {
@@ -376,9 +379,9 @@ static inline long long most_chunks(long long rows, int groups, int cols) {
 // How long a call of single CTAs takes with `chunks` chunks of at most `cols` rows of Q, in units of about 2.5 cycles.  A CTA takes in 52 bytes a cycle
 // whatever it computes, so a stage costs its 128 + cols lines of 128 bytes; storing a tile takes 21 cycles a column, beside the
 // next tile's stages.
-static inline long long tiles_cost(long long chunks, int cols, int mdim, int steps, int sms) {
+static inline long long tiles_cost(long long chunks, int cols, int mdim, int steps) {
   const long long tiles = chunks * ((mdim + 127) / 128), store = 9ll * cols, main = (long long)steps * (128 + cols);
-  return (tiles + sms - 1) / sms * (main > store ? main : store) + store;
+  return (tiles + SMS - 1) / SMS * (main > store ? main : store) + store;
 }
 
 // Chunks that `rows` rows of `groups` groups may be expected to make: half a chunk more for each group, one at least
@@ -389,9 +392,9 @@ static inline long long likely_chunks(long long rows, int groups, int cols) {
 
 // Parts that a tile's reduction of `steps` stages is cut into where `tiles` of them leave more than half the SMs idle: as many as fill these, at most
 // eight (the largest portable cluster), and two stages at least for each.  1: not cut.
-static inline int parts_of(long long tiles, int steps, int sms) {
+static inline int parts_of(long long tiles, int steps) {
   int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= sms && steps >= max(8, parts * 4)) parts *= 2;
+  while (parts < 8 && tiles * parts * 2 <= SMS && steps >= max(8, parts * 4)) parts *= 2;
   return parts;
 }
 
