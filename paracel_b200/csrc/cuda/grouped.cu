@@ -146,6 +146,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   if (warp == 2 && lane == 0) {
     for (const CUtensorMap* m : {&mapP, &mapQ, &mapQ_small, &mapOut}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
+  let_next_begin();
+  after_previous();
   load_bounds(a.off, s.table.bounds, &g_status);
   __syncthreads();
   if (warp == 0) s.table.build(a.off.groups, COLS, &g_status);
@@ -371,20 +373,10 @@ int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, co
   const long long mb = (a.mdim + Form<CG, COLS, SPLIT>::M - 1) / Form<CG, COLS, SPLIT>::M;
   const long long chunks = MODE == TN ? (long long)a.off.groups * ((a.jdim + COLS - 1) / COLS)
                                       : most_chunks(a.off.rows, a.off.groups, COLS);
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = SPLIT ? parts : CG;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
   // a cluster that shares a tile has no other
-  cfg.gridDim = dim3(SPLIT ? (unsigned)(chunks * mb) * parts : (unsigned)min((long long)(sms / CG), chunks * mb) * CG);
-  cfg.blockDim = dim3(threads_of(MODE));
-  cfg.dynamicSmemBytes = SMEM_BYTES;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = CG > 1 || SPLIT ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, o, a);
+  const unsigned grid = SPLIT ? (unsigned)(chunks * mb) * parts : (unsigned)min((long long)(sms / CG), chunks * mb) * CG;
+  const Launch l(grid, threads_of(MODE), SMEM_BYTES, SPLIT ? parts : CG, stream);
+  e = cudaLaunchKernelEx(&l.cfg, kernel, p, q, qs, o, a);
   return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 

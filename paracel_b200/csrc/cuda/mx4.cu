@@ -10,6 +10,7 @@
 namespace {
 
 using namespace pcl_group;
+using namespace pcl_tiles;
 
 // the file is compiled with subnormals flushed to zero: a plain product would lose blocks whose scale is below 2^-126
 __device__ __forceinline__ float mul_keep(float a, float b) {
@@ -75,8 +76,9 @@ constexpr int QROWS = 8, QTHREADS = 32 * QROWS;
 template <int ITERS, class T>
 __global__ void __launch_bounds__(QTHREADS, 6) quantize_kernel(QuantArgs a) {
   constexpr int QCOLS = 256 * ITERS, QWORDS = QCOLS / 128;
-  // a product that is queued behind this may set itself up meanwhile; it waits before it reads what is written here
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // Behind the wait: the product that follows reads its other operand without one of its own, and that may come from the kernel before this
+  after_previous();
+  let_next_begin();
   __shared__ uint32_t words[QWORDS][QROWS];
   const int across = (a.words + QWORDS - 1) / QWORDS;
   const int part = (int)(blockIdx.x % across);
@@ -199,8 +201,6 @@ __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
 // four stages fill the 512.  (224 columns and scales for two stages: a stage's copy then waits for the products of the stage before the last,
 // and 1000 cycles go by per stage, 270 us for 8192^3.)
 // Roles in a CTA: warp 0 loads operands, warp 1 issues products, warps 2-9 store, warps 10-12 fetch scales.
-using namespace pcl_tiles;
-
 constexpr int LANES = 128;
 constexpr int BR = 256;                        // values of a row in a stage: 128 bytes
 constexpr int P_BYTES = LANES * 128;
@@ -234,7 +234,7 @@ struct Args {
   Offsets off;
   int N, steps, words, blocks, fill;
   bool boxed;   // results leave through mapOut
-  bool behind;  // launched while the quantisation of A still runs
+  bool behind;  // the kernel before is the quantisation of A, and wrote nothing else that is read here
 };
 
 struct Shared {
@@ -326,6 +326,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   if (warp == 2 && lane == 0) {
     for (const CUtensorMap* m : {&mapP, &mapQ, &mapQ_small, &mapOut}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
+  let_next_begin();
+  if (!a.behind) after_previous();
   load_bounds(a.off, s.table.bounds, &g_status);
   __syncthreads();
   if (warp == 0) s.table.build(a.off.groups, COLS, &g_status);
@@ -345,7 +347,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   };
 
   if (warp == 0) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // the quantisation of A, where it is queued right before
+    after_previous();   // A may still be being quantised
     int stage = 0;
     uint32_t phase = 0;
     for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
@@ -421,7 +423,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     }
   } else if (warp >= SCALE_WARP) {
     const int part = warp - SCALE_WARP;      // 0: P, 1 and 2: Q
-    if (part > 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (part > 0) after_previous();
     const long long rows = part == 0 ? (long long)a.off.groups * a.N : a.off.rows;
     const uint8_t* src = reinterpret_cast<const uint8_t*>(part == 0 ? a.sp : a.sq);
     // Of 128 rows a lane copies 8 q + lane mod 8 + 32 (lane / 8), q = 0 .. 3: together the lanes read whole sectors and write
@@ -518,27 +520,10 @@ int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, co
   if (e != cudaSuccess) return (int)e;
   const long long mb = (a.N + LANES - 1) / LANES;
   const long long chunks = most_chunks(a.off.rows, a.off.groups, COLS);
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  int attrs = 0;
-  if (SPLIT) {
-    attr[attrs].id = cudaLaunchAttributeClusterDimension;
-    attr[attrs].val.clusterDim.x = parts;
-    attr[attrs].val.clusterDim.y = 1;
-    attr[attrs++].val.clusterDim.z = 1;
-  }
-  if (a.behind) {
-    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[attrs++].val.programmaticStreamSerializationAllowed = 1;
-  }
   // a cluster that shares a tile has no other
-  cfg.gridDim = dim3(SPLIT ? (unsigned)(chunks * mb) * parts : (unsigned)min((long long)sms, chunks * mb));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = attrs;
-  e = cudaLaunchKernelEx(&cfg, kernel, p, q, qs, o, a);
+  const unsigned grid = SPLIT ? (unsigned)(chunks * mb) * parts : (unsigned)min((long long)sms, chunks * mb);
+  const Launch l(grid, THREADS, smem, parts, stream);
+  e = cudaLaunchKernelEx(&l.cfg, kernel, p, q, qs, o, a);
   return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 
@@ -559,9 +544,9 @@ bool blocks_of(long long rows, int words, long long* n, bool* long_rows) {
 }
 
 template <class T>
-void launch_quantize(unsigned n, bool long_rows, const QuantArgs& a, cudaStream_t stream) {
-  if (long_rows) quantize_kernel<4, T><<<n, QTHREADS, 0, stream>>>(a);
-  else quantize_kernel<1, T><<<n, QTHREADS, 0, stream>>>(a);
+int launch_quantize(unsigned n, bool long_rows, const QuantArgs& a, cudaStream_t stream) {
+  const Launch l(n, QTHREADS, 0, 1, stream);
+  return (int)cudaLaunchKernelEx(&l.cfg, long_rows ? quantize_kernel<4, T> : quantize_kernel<1, T>, a);
 }
 
 template <class T>
@@ -580,10 +565,10 @@ static int quantize(const void* x, long long ldx, int in_type, void* data, void*
   bool long_rows;
   if (rows < 0 || K < 1 || in_type < 0 || in_type > 2 || !blocks_of(rows, a.words, &n, &long_rows)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
-  if (in_type == TYPE_F32) launch_quantize<float>((unsigned)n, long_rows, a, stream);
-  else if (in_type == TYPE_BF16) launch_quantize<__nv_bfloat16>((unsigned)n, long_rows, a, stream);
-  else launch_quantize<__half>((unsigned)n, long_rows, a, stream);
-  return pcl_last_error();
+  const int rc = in_type == TYPE_F32    ? launch_quantize<float>((unsigned)n, long_rows, a, stream)
+                 : in_type == TYPE_BF16 ? launch_quantize<__nv_bfloat16>((unsigned)n, long_rows, a, stream)
+                                        : launch_quantize<__half>((unsigned)n, long_rows, a, stream);
+  return rc ? rc : pcl_last_error();
 }
 
 // x [rows, K] of in_type (0 fp32, 1 bf16, 2 fp16), rows ldx values apart

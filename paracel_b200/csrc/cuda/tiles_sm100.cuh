@@ -206,6 +206,12 @@ struct Counter {
   }
 };
 
+// The kernels here are launched while the one before them in the stream may still run, so that their blocks find their place and set up barriers and tensor
+// memory meanwhile (2 to 3 us of a call that takes 5 to 10); `after_previous` comes before the first access to global memory.  They let the next one
+// begin the same way from their own start: it waits for their end.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <bool CLUSTER>
 __device__ __forceinline__ void sync_cluster_or_block() {
   __syncthreads();
@@ -397,6 +403,30 @@ static inline int parts_of(long long tiles, int steps) {
   while (parts < 8 && tiles * parts * 2 <= SMS && steps >= max(8, parts * 4)) parts *= 2;
   return parts;
 }
+
+// A launch in clusters of `cluster` CTAs, behind the previous kernel of the stream as `let_next_begin` says
+struct Launch {
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = {};
+
+  Launch(unsigned grid, int threads, size_t smem, int cluster, cudaStream_t stream) {
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster > 1) {
+      attr[1].id = cudaLaunchAttributeClusterDimension;
+      attr[1].val.clusterDim.x = (unsigned)cluster;
+      attr[1].val.clusterDim.y = 1;
+      attr[1].val.clusterDim.z = 1;
+      cfg.numAttrs = 2;
+    }
+  }
+};
 
 // map of `depth` matrices [rows x inner]; strides in bytes; box: box_in values x box_rows rows of one matrix.  `inner` and box_in count elements of `type`.
 static inline int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, long long inner, long long rows, long long depth,
