@@ -331,6 +331,53 @@ def test_calls_on_two_streams_at_once():
         assert torch.equal(y.double(), ref) and torch.equal(d.double(), rd)
 
 
+def test_a_chain_of_calls_waits_for_what_it_reads():
+    """Every call reads what the one right before it wrote, operands and bounds among it, and takes over memory that others just gave back: kernels
+    that begin before their predecessor has ended must not be seen to."""
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt, grouped_tn
+    T, E, N, K = 96, 4, 136, 72
+    X0, _, W0 = _whole(T, E, N, K, BF, seed=3)
+    bounds = [_offsets(c) for c in ([24, 24, 24, 24], [0, 90, 1, 5], [96, 0, 0, 0], [3, 3, 3, 80])]
+
+    def chain(wait):
+        off, X, W, seen = torch.empty_like(bounds[0]), X0.clone(), W0.clone(), []
+        for i in range(60):
+            off.copy_(bounds[i % 4])
+            y = grouped_nt(X, W, off)
+            wait()
+            y.clamp_(-8, 8)
+            z = grouped_nn(y, W, off)
+            wait()
+            X = z.clamp_(-4, 4)
+            d = grouped_tn(y, X, off)
+            wait()
+            W = d.clamp_(-4, 4)
+            a = grouped_nt(X, W, off)
+            b = grouped_nt(X, W, off, out=torch.empty_like(a))
+            wait()
+            W = grouped_tn(a, X, off).clamp_(-4, 4)
+            seen += [a.clone(), b, W]
+        return seen
+
+    apart = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(lambda: None), apart))
+    check_status()
+
+
+def test_a_reduction_over_a_million_rows():
+    from paracel_b200.ops.grouped import check_status, grouped_tn
+    T, N, K = 1_000_003, 40, 72
+    g = torch.Generator(device="cuda").manual_seed(6)
+    X = torch.randint(-1, 2, (T, K), device="cuda", generator=g, dtype=torch.int8)
+    dY = torch.randint(-1, 2, (T, N), device="cuda", generator=g, dtype=torch.int8)
+    off = torch.tensor([0, T - 3, T], device="cuda")
+    d = grouped_tn(dY.to(FP), X.to(FP), off, out_dtype=torch.float32)
+    check_status()
+    assert torch.equal(d[0].double(), dY[:-3].double().T @ X[:-3].double())
+    assert torch.equal(d[1].double(), dY[-3:].double().T @ X[-3:].double())
+
+
 def test_the_same_call_gives_the_same_bits():
     from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
     X, dY, W = _make(2000, 5, 264, 1032, BF)

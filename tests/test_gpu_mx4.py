@@ -290,6 +290,35 @@ def test_captured_calls_follow_their_inputs_and_streams_do_not_mix():
     check_status()
 
 
+def test_a_chain_of_calls_waits_for_what_it_reads():
+    """Both operands, and the bounds, are written by the kernel right before the one that reads them, in memory that others just gave back."""
+    from paracel_b200.ops.mx4 import check_status, mx4_dequantize, mx4_gemm_nt, mx4_grouped_nt, mx4_quantize
+    T, E, N = 70, 3, 160
+    X0, W0 = _grid(T, N, 1), _grid(E * N, N, 2)
+    bounds = [torch.tensor(b, device="cuda") for b in ([0, 20, 40, 70], [0, 0, 70, 70], [0, 1, 2, 70])]
+
+    def chain(wait):
+        X, W, off, seen = X0.clone(), W0.clone(), torch.empty_like(bounds[0]), []
+        for i in range(40):
+            q = mx4_quantize(W)
+            wait()
+            off.copy_(bounds[i % 3])
+            y = mx4_grouped_nt(X, q, off)
+            wait()
+            X = y.clamp_(-8, 8)
+            z = mx4_gemm_nt(mx4_quantize(X), q)
+            wait()
+            X = mx4_gemm_nt(z[:, :N].contiguous(), mx4_quantize(W[:N])).clamp_(-8, 8)
+            W = torch.roll(mx4_dequantize(q), i, 0)
+            seen += [y, z, X.clone()]
+        return seen
+
+    apart = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(lambda: None), apart))
+    check_status()
+
+
 def test_experts_trained_in_16_bits_answer_from_four():
     """The set as it is used: rows sorted by expert, a step of training, the weights quantised, and served; each stage against the formulas."""
     from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
