@@ -42,10 +42,12 @@ struct Form {
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
   static constexpr int STAGES = (OPERAND_BYTES - (SPLIT ? INBOX_BYTES : 0)) / STAGE_BYTES;
   static constexpr int M = LANES * CG;   // m of a tile
+  // Rows of Q that a load brings: all that fit, or a quarter of them, up to three times.  A load takes the warp that issues it 135 cycles, and the products of a
+  // stage 512 at most: four or five loads to a stage were what bound a call.
+  static constexpr int BOX = COLS / CG, SMALL_BOX = BOX / 4;
   static_assert(STAGES <= MAX_STAGES, "barriers");
   static_assert(COLS % (16 * CG) == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
 };
-constexpr int SMALL_BOX = 32;                  // rows of Q that are loaded at a time where a chunk is not full
 
 struct Args {
   void* out;
@@ -57,6 +59,7 @@ struct Args {
   uint32_t type;       // operands: 0 fp16, 1 bf16
   int fill;            // nt, nn: rows of no group become zero
   bool boxed;          // results leave through mapOut
+  bool wide;           // tn: the maps have columns in blocks of 64 as their third dimension, so that one load brings all blocks of an operand
 };
 
 struct Shared {
@@ -84,7 +87,8 @@ struct Walk {
     jparts = jsize = 0;
     if (MODE == TN) {
       jparts = (a.jdim + COLS - 1) / COLS;
-      jsize = ((a.jdim + jparts - 1) / jparts + 16 * CG - 1) / (16 * CG) * (16 * CG);
+      const int step = (a.wide ? 64 : 16) * CG;
+      jsize = ((a.jdim + jparts - 1) / jparts + step - 1) / step * step;
       chunks = a.off.groups * jparts;
     } else {
       chunks = t.chunks[a.off.groups];
@@ -169,9 +173,9 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const int steps = (w.r1 - w.r0 + BR - 1) / BR;
       const int mine = w.ncol / CG;
       const int j = w.j0 + (int)me * mine;
-      const bool whole = MODE != TN && mine == COLS / CG;
-      const int boxes = MODE == TN ? (mine + 63) / 64 : whole ? 1 : (mine + SMALL_BOX - 1) / SMALL_BOX;
-      const uint32_t q_bytes = MODE == TN ? boxes * 8192u : whole ? (uint32_t)Q_BYTES : boxes * (uint32_t)(SMALL_BOX * BR * 2);
+      const bool whole = MODE == TN ? a.wide : mine > 3 * F::SMALL_BOX;
+      const int boxes = whole ? 1 : MODE == TN ? (mine + 63) / 64 : (mine + F::SMALL_BOX - 1) / F::SMALL_BOX;
+      const uint32_t q_bytes = whole ? (uint32_t)Q_BYTES : MODE == TN ? boxes * 8192u : boxes * (uint32_t)(F::SMALL_BOX * BR * 2);
       for (int kb = 0; kb < steps; ++kb) {
         if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) {
           if (lane == 0) report(&g_status, 0, 41, kb, stage);
@@ -198,6 +202,14 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
           const int m = w.m0 + (int)me * LANES;
           if (MODE == NT) {
             tma_load_3d<CG>(sp, &mapP, bar, r, m, w.e);
+          } else if (MODE == TN && a.wide) {
+            if (tail) {
+              tma_load_3d<1>(sp, &mapP, bar, 0, r, m / 64);
+              tma_load_3d<1>(sq, &mapQ, bar, 0, r, j / 64);
+            } else {
+              tma_load_3d<CG>(sp, &mapP, bar, 0, r, m / 64);
+              tma_load_3d<CG>(sq, &mapQ, bar, 0, r, j / 64);
+            }
           } else {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -206,7 +218,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
             }
           }
           if (MODE == TN) {
-            for (int b = 0; b < boxes; ++b) {
+            for (int b = 0; b < (a.wide ? 0 : boxes); ++b) {
               if (tail) tma_load_3d<1>(sq + b * 8192, &mapQ, bar, j + 64 * b, r, 0);
               else tma_load_3d<CG>(sq + b * 8192, &mapQ, bar, j + 64 * b, r, 0);
             }
@@ -214,7 +226,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
             tma_load_3d<CG>(sq, &mapQ, bar, r, j, 0);
           } else {
             for (int b = 0; b < boxes; ++b)
-              tma_load_3d<CG>(sq + b * SMALL_BOX * BR * 2, &mapQ_small, bar, r, j + b * SMALL_BOX, 0);
+              tma_load_3d<CG>(sq + b * F::SMALL_BOX * BR * 2, &mapQ_small, bar, r, j + b * F::SMALL_BOX, 0);
           }
         }
         __syncwarp();
@@ -447,9 +459,9 @@ PCL_API int pcl_grouped_rows(int mode, int in_type, int out_type, const void* X,
   CUtensorMap p, q, qs, o;
   int rc = make_map_3d(&p, t, W, K, N, groups, ws_n * 2, ws_e * 2, 64, mode == 0 ? LANES : BR);
   if (rc == 0) rc = make_map_3d(&q, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SHAPE_COLS[shape]);
-  if (rc == 0) rc = make_map_3d(&qs, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SMALL_BOX);
+  if (rc == 0) rc = make_map_3d(&qs, t, X, red, rows, 1, ldx * 2, ldx * 2, BR, SHAPE_COLS[shape] / 4);
   if (rc) return rc;
-  Args a{out, ldo, Offsets{offsets, off64, groups, (int)rows}, mode == 0 ? N : K, 0, red, in_type == TYPE_BF16 ? 1u : 0u, fill, false};
+  Args a{out, ldo, Offsets{offsets, off64, groups, (int)rows}, mode == 0 ? N : K, 0, red, in_type == TYPE_BF16 ? 1u : 0u, fill, false, false};
   a.boxed = make_out_map(&o, p, out_type, out, a.mdim, rows, 1, ldo, ldo);
   if (mode == 0) return launch_shape<NT>(shape, in_type, out_type, p, q, qs, o, a, stream);
   return launch_shape<NN>(shape, in_type, out_type, p, q, qs, o, a, stream);
@@ -461,13 +473,21 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
                            cudaStream_t stream) {
   if (!sizes_ok(in_type, rows, groups, N, K) || rows == 0) return (int)cudaErrorInvalidValue;
   const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap p, q, o;
-  int rc = make_map_3d(&p, t, X, K, rows, 1, ldx * 2, ldx * 2, 64, BR);
-  if (rc == 0) rc = make_map_3d(&q, t, Y, N, rows, 1, ldy * 2, ldy * 2, 64, BR);
-  if (rc) return rc;
-  Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0, false};
-  a.boxed = make_out_map(&o, p, out_type, out, K, N, groups, K, (long long)N * K);
   const bool pair = pairs_pay((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K);
+  // (a block that is not full would reach into the next row, and behind the last one)
+  const bool wide = N % 64 == 0 && K % 64 == 0;
+  CUtensorMap p, q, o;
+  int rc = 0;
+  if (wide) {
+    rc = make_map_3d(&p, t, X, 64, rows, K / 64, ldx * 2, 128, 64, BR, CU_TENSOR_MAP_SWIZZLE_128B, LANES / 64);
+    if (rc == 0) rc = make_map_3d(&q, t, Y, 64, rows, N / 64, ldy * 2, 128, 64, BR, CU_TENSOR_MAP_SWIZZLE_128B, MAX_COLS / (pair ? 2 : 1) / 64);
+  } else {
+    rc = make_map_3d(&p, t, X, K, rows, 1, ldx * 2, ldx * 2, 64, BR);
+    if (rc == 0) rc = make_map_3d(&q, t, Y, N, rows, 1, ldy * 2, ldy * 2, 64, BR);
+  }
+  if (rc) return rc;
+  Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0, false, wide};
+  a.boxed = make_out_map(&o, p, out_type, out, K, N, groups, K, (long long)N * K);
   return launch_shape<TN>(pair ? PAIR : MANY, in_type, out_type, p, q, q, o, a, stream);
 }
 

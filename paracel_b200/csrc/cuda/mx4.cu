@@ -211,13 +211,16 @@ constexpr int MAX_STAGES = 7;
 constexpr int EPI_WARPS = 8;
 constexpr int SCALE_WARP = 2 + EPI_WARPS;
 constexpr int THREADS = 32 * (SCALE_WARP + 3);
-constexpr int SMALL_BOX = 32;
+
+// Rows of A that a load brings where a tile has not all that fit: up to three times a quarter of them, in whole groups of eight
+constexpr int small_box(int cols) { return (cols / 4 + 7) / 8 * 8; }
 
 // COLS: columns of an accumulator, the most rows of A in a tile.  64 of them leave room for seven stages of 27 KB, 128 for five of 35, 208 for four of 45.
 // SPLIT: a cluster shares a tile's reduction (COLS 64 only)
 template <int COLS, bool SPLIT>
 struct Form {
   static constexpr int STAGE_BYTES = P_BYTES + COLS * 128;
+  static constexpr int SMALL_BOX = small_box(COLS);
   static constexpr int STAGES = (192 * 1024 - (SPLIT ? INBOX_BYTES : 0)) / (STAGE_BYTES + SCALE_BYTES);
   static constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (SPLIT ? INBOX_BYTES : 0);   // and Shared
   static_assert(STAGES <= MAX_STAGES, "barriers");
@@ -352,7 +355,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     uint32_t phase = 0;
     for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
-      const bool whole = w.ncol == COLS;
+      constexpr int SMALL_BOX = Form<COLS, SPLIT>::SMALL_BOX;
+      const bool whole = w.ncol > 3 * SMALL_BOX;
       const int boxes = whole ? 1 : (w.ncol + SMALL_BOX - 1) / SMALL_BOX;
       const uint32_t bytes = P_BYTES + (whole ? COLS * 128 : boxes * SMALL_BOX * 128);
       for (int kb = w.k0; kb < w.k1; ++kb) {
@@ -618,7 +622,7 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
   const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int rc = make_map_3d(&p, t, B, row_bytes, N, groups, row_bytes, row_bytes * N, 128, LANES);
   if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, cols);
-  if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, SMALL_BOX);
+  if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, small_box(cols));
   if (rc) return rc;
   Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
          N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false, x_type >= 0};

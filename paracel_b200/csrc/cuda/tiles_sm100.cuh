@@ -428,15 +428,15 @@ struct Launch {
   }
 };
 
-// map of `depth` matrices [rows x inner]; strides in bytes; box: box_in values x box_rows rows of one matrix.  `inner` and box_in count elements of `type`.
+// map of `depth` matrices [rows x inner]; strides in bytes; box: box_in values x box_rows rows x box_mats matrices.  `inner` and box_in count elements of `type`.
 static inline int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, long long inner, long long rows, long long depth,
                               long long row_bytes, long long mat_bytes, int box_in, int box_rows,
-                              CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+                              CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B, int box_mats = 1) {
   encode_fn_t enc = get_encode2();
   if (enc == nullptr) return (int)cudaErrorNotSupported;
   cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)depth};
   cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)mat_bytes};
-  cuuint32_t box[3] = {(cuuint32_t)box_in, (cuuint32_t)box_rows, 1};
+  cuuint32_t box[3] = {(cuuint32_t)box_in, (cuuint32_t)box_rows, (cuuint32_t)box_mats};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(map, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
