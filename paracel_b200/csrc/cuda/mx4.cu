@@ -64,76 +64,121 @@ struct QuantArgs {
   long long rows;
   int K, words;        // words: ceil(K / 128)
   int vec;             // rows of x can be read 16 bytes at a time
+  int shift;           // log2 of the words side by side in a CTA
 };
 
-// A thread takes eight neighbouring values of a row, four lanes make a block of 32 and sixteen a word of scales: a warp reads 256 values (512 bytes of 16-bit
-// ones) and stores 128 bytes.  It goes over ITERS times as many of one row, all of its loads before the first use; the block's eight rows
-// make whole sectors of scales.  Bound by memory: 32768 x 8192 of bf16 takes 123 us (5.6 TB/s), back to bf16 106 us (6.5 TB/s); 32 rows x 128
-// columns to a block, whose rows are 256 bytes here and 64 there, took 161 and 184 us.  The registers are bounded so that six blocks share an SM: with
-// five of them quantisation takes 164 us, with seven, whose loads no longer fit, 224.
-constexpr int QROWS = 8, QTHREADS = 32 * QROWS;
+// A thread takes eight neighbouring values of a row, four lanes make a block of 32 and sixteen a word of scales, 128 values.  A CTA has 16 ITERS words, of which
+// 2^shift lie side by side in a row: 1024 columns of eight rows where rows are that long, and 64 rows of 128 columns.  All loads of a thread come before
+// the first use, and the words of neighbouring rows are stored together.  Bound by memory: 32768 x 8192 of bf16 takes 120 us (5.7 TB/s) and of fp32 178 us
+// (6.8 TB/s), back to bf16 110 us (6.2 TB/s); 1000000 x 128 of fp32 89 us (6.5 TB/s; 418 where a CTA's rows have 1024 columns whatever the matrix has).  The registers are
+// bounded so that six blocks share an SM: with five of them quantisation of bf16 takes 164 us, with seven, whose loads no longer fit, 224.
+constexpr int QTHREADS = 256;
 
-template <int ITERS, class T>
-__global__ void __launch_bounds__(QTHREADS, 6) quantize_kernel(QuantArgs a) {
-  constexpr int QCOLS = 256 * ITERS, QWORDS = QCOLS / 128;
+template <int ITERS>
+struct Units {
+  static constexpr int COUNT = 16 * ITERS, LOG = ITERS == 4 ? 6 : 4;
+  long long r0;
+  int word0, shift;
+
+  __device__ Units(int words, int shift_) : shift(shift_) {
+    const int across = (words + (1 << shift) - 1) >> shift;
+    word0 = (int)(blockIdx.x % across) << shift;
+    r0 = (long long)(blockIdx.x / across) << (LOG - shift);
+  }
+  // of this thread: its word, the same in every pass, its row in the first, and the rows from one pass to the next
+  __device__ int word() const { return word0 + ((threadIdx.x >> 4) & ((1 << shift) - 1)); }
+  __device__ long long row() const { return r0 + (threadIdx.x >> (4 + shift)); }
+  __device__ int step() const { return 16 >> shift; }
+};
+
+// The largest magnitude of eight values, as the bits of an fp32 value: compared by their bits NaN and infinity come out on top.  16-bit values are
+// compared in pairs, before they are widened.
+template <class T>
+__device__ __forceinline__ uint32_t top_bits(const uint4* raw);
+template <>
+__device__ __forceinline__ uint32_t top_bits<float>(const uint4* raw) {
+  constexpr uint32_t M = 0x7fffffffu;
+  const uint32_t a = max(max(raw[0].x & M, raw[0].y & M), max(raw[0].z & M, raw[0].w & M));
+  const uint32_t b = max(max(raw[1].x & M, raw[1].y & M), max(raw[1].z & M, raw[1].w & M));
+  return max(a, b);
+}
+__device__ __forceinline__ uint32_t top_16(const uint4& r) {
+  constexpr uint32_t M = 0x7fff7fffu;
+  const uint32_t m = __vmaxu2(__vmaxu2(r.x & M, r.y & M), __vmaxu2(r.z & M, r.w & M));
+  return max(m & 0xffffu, m >> 16);
+}
+template <>
+__device__ __forceinline__ uint32_t top_bits<__nv_bfloat16>(const uint4* raw) { return top_16(raw[0]) << 16; }
+template <>
+__device__ __forceinline__ uint32_t top_bits<__half>(const uint4* raw) {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top_16(raw[0]))));
+}
+
+// VEC: rows start at multiples of 16 bytes and have a multiple of eight values.  ALONG: a CTA has eight words of a row (shift 3) and a thread goes along one
+// row instead of down one column (bf16 32768 x 8192: 120 instead of 134 us).
+template <int ITERS, bool VEC, bool ALONG, class T>
+__global__ void __launch_bounds__(QTHREADS, !VEC ? 1 : sizeof(T) == 4 ? 4 : 6) quantize_kernel(QuantArgs a) {
   // Behind the wait: the product that follows reads its other operand without one of its own, and that may come from the kernel before this
   after_previous();
   let_next_begin();
-  __shared__ uint32_t words[QWORDS][QROWS];
-  const int across = (a.words + QWORDS - 1) / QWORDS;
-  const int part = (int)(blockIdx.x % across);
-  const long long r0 = (long long)(blockIdx.x / across) * QROWS, r = r0 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  using U = Units<ITERS>;
+  __shared__ uint32_t words[U::COUNT];
+  const U u(a.words, a.shift);
   const int row_words = (a.K + 31) / 32 * 4;           // 4-byte words of a row of data
-  const T* src = static_cast<const T*>(a.x) + r * a.ldx;
+  const int part = threadIdx.x & 15, step = ALONG ? 0 : u.step();
+  const int c = (ALONG ? u.word0 + (int)(threadIdx.x >> 4 & 1) : u.word()) * 128 + part * 8;
+  const long long r = ALONG ? u.r0 + (threadIdx.x >> 5) : u.row();
+  const int left = ALONG ? (r < a.rows ? 1 : 0) : (int)min(a.rows - r, (long long)U::COUNT);
+  auto valid = [&](int i) { return i * step < left && (ALONG ? c + i * 256 < a.K : !VEC || c < a.K); };
+  const T* src = static_cast<const T*>(a.x) + r * a.ldx + c;
+  const long long src_step = ALONG ? 256 : (long long)step * a.ldx;
   constexpr int PER = sizeof(T) / 2;                   // 16-byte loads of eight values
   uint4 raw[ITERS][PER];
-  if (r < a.rows) {
+  if (VEC || (a.vec && c + 8 <= a.K)) {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i)
+#pragma unroll
+      for (int q = 0; q < PER; ++q)
+        raw[i][q] = valid(i) ? __ldcs(reinterpret_cast<const uint4*>(src + i * src_step) + q) : make_uint4(0, 0, 0, 0);
+  } else {
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) {
-      const int c = part * QCOLS + i * 256 + lane * 8;
-      if (a.vec && c + 8 <= a.K) {
+      T v[8];
 #pragma unroll
-        for (int q = 0; q < PER; ++q) raw[i][q] = __ldcs(reinterpret_cast<const uint4*>(src + c) + q);
-      } else {
-        T v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < a.K ? src[c + j] : to_out<T>(0.f);
-        memcpy(raw[i], v, sizeof(v));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < ITERS; ++i) {
-      const int c = part * QCOLS + i * 256 + lane * 8;
-      T t[8];
-      memcpy(t, raw[i], sizeof(t));
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
-      // the largest magnitude of the block, by its bits: NaN and infinity come out on top
-      uint32_t most = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const bool bad = most >= 0x7f800000u;
-      // floor(log2(most)) - 2, at least -127 (all that is below 2^-125 takes the smallest scale)
-      const int code = bad ? 255 : max((int)(most >> 23) - 2, 0);
-      const float inv = __uint_as_float((uint32_t)(254 - min(code, 253)) << 23);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = mul_keep(v[j], inv);   // no matter which in a block that is not a number
-      const bool in = c < row_words * 8;
-      if (in) a.data[r * row_words + (c >> 3)] = pack8(v);
-      uint32_t w = in ? (uint32_t)code << (8 * ((lane & 15) >> 2)) : 0u;
-      w |= __shfl_xor_sync(0xffffffffu, w, 4);
-      w |= __shfl_xor_sync(0xffffffffu, w, 8);
-      if ((lane & 15) == 0) words[i * 2 + (lane >> 4)][threadIdx.x >> 5] = w;
+      for (int j = 0; j < 8; ++j) v[j] = i * step < left && c + j < a.K ? src[i * src_step + j] : to_out<T>(0.f);
+      memcpy(raw[i], v, sizeof(v));
     }
   }
+  uint32_t* dst = a.data + r * row_words + (c >> 3);
+  const long long dst_step = ALONG ? 32 : (long long)step * row_words;
+  const int slot = ((c / 128 - u.word0) << (U::LOG - u.shift)) + (int)(r - u.r0), slot_step = ALONG ? 16 : step;
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) {
+    T t[8];
+    memcpy(t, raw[i], sizeof(t));
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
+    uint32_t most = top_bits<T>(raw[i]);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const bool bad = most >= 0x7f800000u;
+    // floor(log2(most)) - 2, at least -127 (all that is below 2^-125 takes the smallest scale)
+    const int code = bad ? 255 : max((int)(most >> 23) - 2, 0);
+    const float inv = __uint_as_float((uint32_t)(254 - min(code, 253)) << 23);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = mul_keep(v[j], inv);   // no matter which in a block that is not a number
+    const bool in = c + (ALONG ? i * 256 : 0) < row_words * 8;
+    if (in && i * step < left) dst[i * dst_step] = pack8(v);
+    uint32_t w = in ? (uint32_t)code << (8 * (part >> 2)) : 0u;
+    w |= __shfl_xor_sync(0xffffffffu, w, 4);
+    w |= __shfl_xor_sync(0xffffffffu, w, 8);
+    if (part == 0) words[slot + i * slot_step] = w;
+  }
   __syncthreads();
-  const int word = part * QWORDS + (int)threadIdx.x / QROWS, row = threadIdx.x % QROWS;
-  if (threadIdx.x < QWORDS * QROWS && word < a.words && r0 + row < a.rows)
-    a.scales[(long long)word * a.rows + r0 + row] = words[threadIdx.x / QROWS][row];
+  const int rows = U::COUNT >> u.shift, word = u.word0 + (int)threadIdx.x / rows;
+  const long long row = u.r0 + (threadIdx.x & (rows - 1));
+  if (threadIdx.x < U::COUNT && word < a.words && row < a.rows) a.scales[(long long)word * a.rows + row] = words[threadIdx.x];
 }
 
 struct DequantArgs {
@@ -141,49 +186,59 @@ struct DequantArgs {
   const uint32_t* scales;
   void* out;
   long long ldo, rows;
-  int K, words, vec;
+  int K, words, vec, shift;
 };
 
 template <int ITERS, class T>
 __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
-  constexpr int QCOLS = 256 * ITERS, QWORDS = QCOLS / 128;
-  const int across = (a.words + QWORDS - 1) / QWORDS;
-  const int part = (int)(blockIdx.x % across);
-  const long long r = (long long)(blockIdx.x / across) * QROWS + (threadIdx.x >> 5);
-  if (r >= a.rows) return;
-  const int lane = threadIdx.x & 31;
+  const Units<ITERS> u(a.words, a.shift);
   const int row_words = (a.K + 31) / 32 * 4;
+  const int part = threadIdx.x & 15, c = u.word() * 128 + part * 8, step = u.step();
+  const long long r = u.row();
+  if (c >= a.K) return;
+  const int left = (int)min(a.rows - r, (long long)(16 * ITERS));
+  const uint32_t* src = a.data + r * row_words + (c >> 3);
+  const uint32_t* scales = a.scales + (long long)u.word() * a.rows + r;
   uint32_t codes[ITERS], scale[ITERS];
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
-    const int c = part * QCOLS + i * 256 + lane * 8;
-    codes[i] = scale[i] = 0;
-    if (c < a.K) {
-      codes[i] = __ldcs(a.data + r * row_words + (c >> 3));
-      scale[i] = a.scales[(long long)(c >> 7) * a.rows + r];
-    }
+    codes[i] = i * step < left ? __ldcs(src + (long long)(i * step) * row_words) : 0u;
+    scale[i] = i * step < left ? scales[i * step] : 0u;
   }
+  T* dst = static_cast<T*>(a.out) + r * a.ldo + c;
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
-    const int c = part * QCOLS + i * 256 + lane * 8;
-    if (c >= a.K) continue;
-    const float s = scale_value((scale[i] >> (8 * ((lane & 15) >> 2))) & 255u);
+    if (i * step >= left) break;
+    const float s = scale_value((scale[i] >> (8 * (part >> 2))) & 255u);
     float f[8];
     unpack8(codes[i], f);
     T v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = to_out<T>(mul_keep(f[j], s));
-    T* dst = static_cast<T*>(a.out) + r * a.ldo + c;
-    if (a.vec && c + 8 <= a.K) {
-      uint4 raw[sizeof(T) / 2];
-      memcpy(raw, v, sizeof(v));
-#pragma unroll
-      for (int q = 0; q < (int)(sizeof(T) / 2); ++q) __stcs(reinterpret_cast<uint4*>(dst) + q, raw[q]);
+    if (sizeof(T) == 2 && a.vec && c + 8 <= a.K) {
+      uint4 raw;
+      memcpy(&raw, v, 16);
+      __stcs(reinterpret_cast<uint4*>(dst), raw);
+    } else if (sizeof(T) == 4 && a.vec && (c & ~15) + 16 <= a.K) {
+      // two lanes have 64 bytes: they change halves, so that each of their two stores is a whole sector (195 instead of 261 us for 32768 x 8192)
+      const bool odd = part & 1;
+      uint4 lo, hi, other;
+      memcpy(&lo, v, 16);
+      memcpy(&hi, reinterpret_cast<const char*>(v) + 16, 16);
+      const uint4 give = odd ? lo : hi;
+      const unsigned pair = 3u << (threadIdx.x & 30);
+      other.x = __shfl_xor_sync(pair, give.x, 1);
+      other.y = __shfl_xor_sync(pair, give.y, 1);
+      other.z = __shfl_xor_sync(pair, give.z, 1);
+      other.w = __shfl_xor_sync(pair, give.w, 1);
+      __stcs(reinterpret_cast<uint4*>(dst - (odd ? 4 : 0)), odd ? other : lo);
+      __stcs(reinterpret_cast<uint4*>(dst + (odd ? 4 : 8)), odd ? hi : other);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (c + j < a.K) dst[j] = v[j];
     }
+    dst += (long long)step * a.ldo;
   }
 }
 
@@ -201,6 +256,11 @@ __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
 // four stages fill the 512.  (224 columns and scales for two stages: a stage's copy then waits for the products of the stage before the last,
 // and 1000 cycles go by per stage, 270 us for 8192^3.)
 // Roles in a CTA: warp 0 loads operands, warp 1 issues products, warps 2-9 store, warps 10-12 fetch scales.
+//
+// Measured: 8192^3 in 261 us = 4.2 PFLOP/s (nominal peak 9), 32 groups of together 16384 rows x 4096 x 2048 in 100 us, with A from bf16 290 and 117; one row
+// against 8192 x 4096 10.2 us.  Bound by the tensor pipe: a stage takes 600 cycles of it, 416 for the products of 208 columns and 30 for each of the six
+// copies of scales; by the bytes that an SM takes in (45 KB a stage) where a reduction is short; by latency, about 4 us, for the smallest.  Pairs of
+// CTAs, which load less, took 283 us: the leader has to be told of the other's scales.
 constexpr int LANES = 128;
 constexpr int BR = 256;                        // values of a row in a stage: 128 bytes
 constexpr int P_BYTES = LANES * 128;
@@ -539,39 +599,47 @@ int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CU
   return launch<COLS, SPLIT, __half>(p, q, qs, o, a, parts, stream);
 }
 
-// Blocks of the grid, and with how many passes a warp: four where that leaves every SM four blocks, else one
-bool blocks_of(long long rows, int words, long long* n, bool* long_rows) {
-  const long long down = (rows + QROWS - 1) / QROWS;
-  *long_rows = down * ((words + 7) / 8) >= 4 * SMS;
-  *n = down * (*long_rows ? (words + 7) / 8 : (words + 1) / 2);
+// CTAs of the grid, how long their rows are, and whether they go over four words a thread: where that leaves every SM four of them
+bool blocks_of(long long rows, int words, long long* n, int* shift, bool* four) {
+  for (const int iters : {4, 1}) {
+    *shift = 0;
+    while ((1 << *shift) < words && *shift < (iters == 4 ? 3 : 1)) ++*shift;
+    const int down = 16 * iters >> *shift;
+    *n = (rows + down - 1) / down * ((words + (1 << *shift) - 1) >> *shift);
+    *four = iters == 4;
+    if (*n >= 4 * SMS) break;
+  }
   return *n < (1ll << 31);
 }
 
 template <class T>
-int launch_quantize(unsigned n, bool long_rows, const QuantArgs& a, cudaStream_t stream) {
+int launch_quantize(unsigned n, bool four, const QuantArgs& a, cudaStream_t stream) {
   const Launch l(n, QTHREADS, 0, 1, stream);
-  return (int)cudaLaunchKernelEx(&l.cfg, long_rows ? quantize_kernel<4, T> : quantize_kernel<1, T>, a);
+  const bool vec = a.vec && a.K % 8 == 0;
+  auto kernel = vec ? (four ? (a.shift == 3 ? quantize_kernel<4, true, true, T> : quantize_kernel<4, true, false, T>) : quantize_kernel<1, true, false, T>)
+                    : (four ? quantize_kernel<4, false, false, T> : quantize_kernel<1, false, false, T>);
+  return (int)cudaLaunchKernelEx(&l.cfg, kernel, a);
 }
 
 template <class T>
-void launch_dequantize(unsigned n, bool long_rows, const DequantArgs& a, cudaStream_t stream) {
-  if (long_rows) dequantize_kernel<4, T><<<n, QTHREADS, 0, stream>>>(a);
+void launch_dequantize(unsigned n, bool four, const DequantArgs& a, cudaStream_t stream) {
+  if (four) dequantize_kernel<4, T><<<n, QTHREADS, 0, stream>>>(a);
   else dequantize_kernel<1, T><<<n, QTHREADS, 0, stream>>>(a);
 }
 
 }  // namespace
 
 static int quantize(const void* x, long long ldx, int in_type, void* data, void* scales, long long rows, int K, cudaStream_t stream) {
-  QuantArgs a{x, ldx, static_cast<uint32_t*>(data), static_cast<uint32_t*>(scales), rows, K, (K + 127) / 128, 0};
+  QuantArgs a{x, ldx, static_cast<uint32_t*>(data), static_cast<uint32_t*>(scales), rows, K, (K + 127) / 128, 0, 0};
   const int size = in_type == TYPE_F32 ? 4 : 2;
   a.vec = ((uintptr_t)x & 15) == 0 && (ldx * size & 15) == 0;
   long long n;
-  bool long_rows;
-  if (rows < 0 || K < 1 || in_type < 0 || in_type > 2 || !blocks_of(rows, a.words, &n, &long_rows)) return (int)cudaErrorInvalidValue;
+  bool four;
+  if (rows < 0 || K < 1 || in_type < 0 || in_type > 2 || !blocks_of(rows, a.words, &n, &a.shift, &four)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
-  const int rc = in_type == TYPE_F32    ? launch_quantize<float>((unsigned)n, long_rows, a, stream)
-                 : in_type == TYPE_BF16 ? launch_quantize<__nv_bfloat16>((unsigned)n, long_rows, a, stream)
-                                        : launch_quantize<__half>((unsigned)n, long_rows, a, stream);
+  const int rc = in_type == TYPE_F32    ? launch_quantize<float>((unsigned)n, four, a, stream)
+                 : in_type == TYPE_BF16 ? launch_quantize<__nv_bfloat16>((unsigned)n, four, a, stream)
+                                        : launch_quantize<__half>((unsigned)n, four, a, stream);
   return rc ? rc : pcl_last_error();
 }
 
@@ -583,16 +651,16 @@ PCL_API int pcl_mx4_quantize(const void* x, long long ldx, int in_type, void* da
 
 PCL_API int pcl_mx4_dequantize(const void* data, const void* scales, void* out, long long ldo, int out_type, long long rows,
                                int K, cudaStream_t stream) {
-  DequantArgs a{static_cast<const uint32_t*>(data), static_cast<const uint32_t*>(scales), out, ldo, rows, K, (K + 127) / 128, 0};
+  DequantArgs a{static_cast<const uint32_t*>(data), static_cast<const uint32_t*>(scales), out, ldo, rows, K, (K + 127) / 128, 0, 0};
   const int size = out_type == TYPE_F32 ? 4 : 2;
   a.vec = ((uintptr_t)out & 15) == 0 && (ldo * size & 15) == 0;
   long long n;
-  bool long_rows;
-  if (rows < 0 || K < 1 || out_type < 0 || out_type > 2 || !blocks_of(rows, a.words, &n, &long_rows)) return (int)cudaErrorInvalidValue;
+  bool four;
+  if (rows < 0 || K < 1 || out_type < 0 || out_type > 2 || !blocks_of(rows, a.words, &n, &a.shift, &four)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
-  if (out_type == TYPE_F32) launch_dequantize<float>((unsigned)n, long_rows, a, stream);
-  else if (out_type == TYPE_BF16) launch_dequantize<__nv_bfloat16>((unsigned)n, long_rows, a, stream);
-  else launch_dequantize<__half>((unsigned)n, long_rows, a, stream);
+  if (out_type == TYPE_F32) launch_dequantize<float>((unsigned)n, four, a, stream);
+  else if (out_type == TYPE_BF16) launch_dequantize<__nv_bfloat16>((unsigned)n, four, a, stream);
+  else launch_dequantize<__half>((unsigned)n, four, a, stream);
   return pcl_last_error();
 }
 
