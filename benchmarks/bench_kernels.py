@@ -1,10 +1,10 @@
 #!/usr/bin/env python
 """Micro-benchmarks of the single-GPU algorithm kernels against stock PyTorch ops doing the same
 job: batched ALS solve, k-means accumulate, Gram matrix, device ball-tree search, dense LR gradient,
-the CSR products of the SVD, blockwise similarity with top-k.  CUDA events, 3 warm-ups, L2 flushed
+the CSR products of the SVD, blockwise similarity with top-k, products by group, four-bit products.  CUDA events, 3 warm-ups, L2 flushed
 between timed launches, one JSON line per kernel.
 
-    python benchmarks/bench_kernels.py [--kernel als|kmeans|gram|balltree|dense_grad|spmm|sim_topk|all]
+    python benchmarks/bench_kernels.py [--kernel als|kmeans|gram|balltree|dense_grad|spmm|sim_topk|grouped|mx4|all]
 """
 import argparse
 import json
@@ -210,14 +210,43 @@ def bench_sim_topk(flush):
             "speedup": ms_ref / ms}
 
 
+def bench_grouped(flush):
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt, grouped_tn
+    g = torch.Generator(device="cuda").manual_seed(1)
+    E, T, N, K = 16, 16384, 2048, 1024
+    X, dY = (torch.randn(T, c, device="cuda", generator=g).bfloat16() for c in (K, N))
+    W = torch.randn(E, N, K, device="cuda", generator=g).bfloat16()
+    off = (torch.arange(E + 1, device="cuda") * (T // E)).int()
+    ms = {f.__name__: timeit(lambda f=f, a=a: f(*a, off), flush)
+          for f, a in ((grouped_nt, (X, W)), (grouped_nn, (dY, W)), (grouped_tn, (dY, X)))}
+    check_status()
+    bmm = timeit(lambda: torch.bmm(X.view(E, -1, K), W.transpose(1, 2)), flush)
+    return {"kernel": "grouped", "groups": E, "rows": T, "N": N, "K": K, "ms": ms, "tflops": {k: 2 * T * N * K / v / 1e9 for k, v in ms.items()},
+            "torch_bmm_equal_groups_ms": bmm}
+
+
+def bench_mx4(flush):
+    from paracel_b200.ops.mx4 import check_status, mx4_dequantize, mx4_gemm_nt, mx4_quantize
+    g = torch.Generator(device="cuda").manual_seed(1)
+    M = N = K = 8192
+    A, B = (torch.randn(r, K, device="cuda", generator=g).bfloat16() for r in (M, N))
+    qa, qb = mx4_quantize(A), mx4_quantize(B)
+    ms = {"quantize": timeit(lambda: mx4_quantize(A), flush), "dequantize": timeit(lambda: mx4_dequantize(qa, A.dtype), flush),
+          "product": timeit(lambda: mx4_gemm_nt(qa, qb, out_dtype=A.dtype), flush), "from_bf16": timeit(lambda: mx4_gemm_nt(A, qb), flush)}
+    check_status()
+    return {"kernel": "mx4", "M": M, "N": N, "K": K, "ms": ms, "product_tflops": 2 * M * N * K / ms["product"] / 1e9,
+            "torch_matmul_bf16_ms": timeit(lambda: A @ B.T, flush)}
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--kernel", default="all", choices=["all", "als", "kmeans", "gram", "balltree", "dense_grad", "spmm",
-                                                         "sim_topk"])
+                                                         "sim_topk", "grouped", "mx4"])
     args = ap.parse_args()
     flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
     table = {"als": bench_als, "kmeans": bench_kmeans, "gram": bench_gram, "balltree": bench_balltree,
-             "dense_grad": bench_dense_grad, "spmm": bench_spmm, "sim_topk": bench_sim_topk}
+             "dense_grad": bench_dense_grad, "spmm": bench_spmm, "sim_topk": bench_sim_topk,
+             "grouped": bench_grouped, "mx4": bench_mx4}
     for name, fn in table.items():
         if args.kernel in ("all", name):
             print(json.dumps(fn(flush)))

@@ -123,7 +123,9 @@ struct Walk {
         w.r1 = min(a.red, (rank + 1) * steps / parts * BR);
       }
     }
-    w.ncol = (w.n + 16 * CG - 1) / (16 * CG) * (16 * CG);
+    // (with the wide maps either CTA of a pair begins with a block of 64)
+    const int unit = (MODE == TN && a.wide ? 64 : 16) * CG;
+    w.ncol = (w.n + unit - 1) / unit * unit;
     return w;
   }
 };

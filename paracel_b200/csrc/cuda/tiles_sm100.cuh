@@ -285,7 +285,7 @@ __device__ __forceinline__ void store_singly(uint32_t taddr, int n, TO* dst, lon
 // A warp's part of an accumulator goes to out: column j of [0, n) and the warp's 32 lanes to dst[j * ldo + lane], lanes < `lanes` only.  Columns 32 at a time,
 // first + 0, 64, 128 ..  16-bit results turn around in shared memory (stmatrix) and leave as boxes of 32 rows
 // x 64 bytes, where `boxed` says that the map can take them; what is left of a chunk, and 32-bit results, are stored lane by lane, a row's 32 neighbours at a
-// time.  Stored so throughout, 16-bit results took two thirds as long again as the products of 2048 four-bit values that they came from.
+// time (stored so throughout, nt of 16 groups of 1024 rows, 2048 x 1024 took 81 instead of 68 us).
 template <class TO>
 __device__ __forceinline__ void store_columns(uint32_t taddr, int first, int n, TO* dst, long long ldo, int lanes, bool boxed, uint8_t* piece,
                                               const CUtensorMap* map, int x, int y, int z) {

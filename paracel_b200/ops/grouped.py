@@ -197,7 +197,7 @@ def grouped_nt(X: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, out: Opt
 
     ``X [T, K]`` and ``W [E, N, K]`` may be strided; where their rows do not start at multiples of 16 bytes (an odd K) they are copied
     first.  Rows that no group has, before ``offsets[0]`` or from ``offsets[E]`` on, are zero in a new result, and are
-    left as they were in ``out``."""
+    left as they were in ``out``, which must not overlap an operand."""
     return _rows(0, X, W, offsets, out, out_dtype)
 
 

@@ -85,8 +85,12 @@ class Mx4Matrix:
     def device(self) -> torch.device:
         return (self._data if self._buf is None else self._buf).device
 
+    def __reduce__(self):
+        # copies and pickles are made of the two tensors: addresses are not theirs
+        return Mx4Matrix, (self.data, self.scales, self.cols)
+
     def nbytes(self) -> int:
-        return self.data.numel() + self.scales.numel()
+        return self.rows * ((self.cols + 31) // 32 * 16 + (self.cols + 127) // 128 * 4)
 
     def __repr__(self):
         return f"Mx4Matrix({self.rows} x {self.cols}, {self.device})"
@@ -226,7 +230,7 @@ def _product(A, B: Mx4Matrix, offsets, out, out_dtype):
 def mx4_gemm_nt(A: Union[torch.Tensor, Mx4Matrix], B: Mx4Matrix, out: Optional[torch.Tensor] = None,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``A @ B.T`` for ``A [M, K]`` and ``B [N, K]`` in four bits; an ``A`` in float32, bfloat16 or float16 is quantised here.
-    Sums are held in float32.  The result has ``out``'s type, ``out_dtype``, ``A``'s own, or float32 if A is in four bits."""
+    Sums are held in float32 (their error grows as ``ops.grouped`` says).  ``out`` must not overlap an operand.  The result has ``out``'s type, ``out_dtype``, ``A``'s own, or float32 if A is in four bits."""
     return _product(A, B, None, out, out_dtype)
 
 

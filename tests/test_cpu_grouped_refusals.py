@@ -129,3 +129,14 @@ def test_rows_at_multiples_of_16_bytes():
         assert y is not odd and torch.equal(y, odd) and y.stride(0) % 8 == 0 and y.data_ptr() % 16 == 0
     one = torch.zeros(1, 9, dtype=H)
     assert aligned(one) is one and stride_of(one, 0, 16) == 16
+
+
+def test_copies_of_a_four_bit_matrix_have_memory_of_their_own():
+    import copy
+    import pickle
+    q = _packed(4, 33)
+    q.data.fill_(7)
+    for other in (copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert torch.equal(other.data, q.data) and torch.equal(other.scales, q.scales) and other.cols == 33
+        assert other._data_ptr == other.data.data_ptr() != q._data_ptr and other._scales_ptr == other.scales.data_ptr()
+    assert copy.copy(q).data.data_ptr() == q._data_ptr and q.nbytes() == q.data.numel() + q.scales.numel()

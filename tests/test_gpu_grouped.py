@@ -78,6 +78,8 @@ SHAPES = [
     # a cluster for a tile; tiles of 256 rows for one CTA, and for a pair; with ends of every kind
     ([1], 0, 300, 1000), ([3, 0, 1], 2, 256, 520), ([33, 64], 0, 130, 4100), ([700, 0, 1300, 33, 256], 5, 2000, 1900),
     ([700, 0, 1300, 33, 256], 5, 4008, 3800), ([257, 15, 1000, 0, 500, 470, 60], 0, 3777, 4001),
+    # tn by pairs with columns in whole blocks of 64, an odd number of them
+    ([30, 0, 65, 64, 1] * 20, 0, 320, 256), ([200, 7] * 40, 3, 64, 640), ([63, 65, 128, 0] * 16, 0, 448, 320),
 ]
 
 
