@@ -24,6 +24,7 @@ using Quantize = int (*)(const void*, long long, int, void*, void*, long long, i
 using Dequantize = int (*)(const void*, const void*, void*, long long, int, long long, int, cudaStream_t);
 using Mx4Rows = int (*)(const void*, long long, int, void*, void*, const void*, const void*, const void*, int, void*, long long, int, long long,
                         int, int, int, int, cudaStream_t);
+using Mx4Room = long long (*)(int, long long, int, int, int);
 using ErrorString = const char* (*)(int);
 
 Rows rows_fn;
@@ -31,6 +32,7 @@ Tn tn_fn;
 Quantize quantize_fn;
 Dequantize dequantize_fn;
 Mx4Rows mx4_rows_fn;
+Mx4Room mx4_room_fn;
 ErrorString error_fn;
 
 constexpr int64_t MAX_GROUPS = 1024, MAX_ROWS = (1ll << 31) - 512, MAX_SIZE = 1ll << 30;
@@ -80,11 +82,11 @@ PyObject* launched(const char* name, F&& launch, const at::Tensor& result) {
   return THPVariable_Wrap(result);
 }
 
-// bind(rows, tn, quantize, dequantize, mx4_rows, error_string): addresses
+// bind(rows, tn, quantize, dequantize, mx4_rows, mx4_room, error_string): addresses
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 6) return PyErr_Format(PyExc_TypeError, "six addresses are wanted");
-  void* p[6];
-  for (int i = 0; i < 6; ++i) {
+  if (n != 7) return PyErr_Format(PyExc_TypeError, "seven addresses are wanted");
+  void* p[7];
+  for (int i = 0; i < 7; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (p[i] == nullptr) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "address %d is null", i);
   }
@@ -93,7 +95,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   quantize_fn = reinterpret_cast<Quantize>(p[2]);
   dequantize_fn = reinterpret_cast<Dequantize>(p[3]);
   mx4_rows_fn = reinterpret_cast<Mx4Rows>(p[4]);
-  error_fn = reinterpret_cast<ErrorString>(p[5]);
+  mx4_room_fn = reinterpret_cast<Mx4Room>(p[5]);
+  error_fn = reinterpret_cast<ErrorString>(p[6]);
   Py_RETURN_NONE;
 }
 
@@ -223,11 +226,13 @@ PyObject* mx4_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (rows < 1 || rows % groups) Py_RETURN_NONE;
   const int64_t N = rows / groups;
   const at::Tensor out = at::empty({T, N}, A.options().dtype(out_type));
-  const at::Tensor work = at::empty({data_bytes(T, K) + scale_bytes(T, K)}, A.options().dtype(at::kByte));
-  uint8_t* qa = static_cast<uint8_t*>(work.data_ptr());
+  at::Tensor work;
+  const int64_t room = mx4_room_fn(type_of(A.scalar_type()), T, (int)groups, (int)N, (int)K);
+  if (room > 0) work = at::empty({room}, A.options().dtype(at::kByte));
+  uint8_t* qa = room > 0 ? static_cast<uint8_t*>(work.data_ptr()) : nullptr;
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
   return launched("pcl_mx4_rows", [&] {
-    return mx4_rows_fn(A.data_ptr(), A.stride(0), type_of(A.scalar_type()), qa, qa + data_bytes(T, K), data, scales, offsets, wide,
+    return mx4_rows_fn(A.data_ptr(), A.stride(0), type_of(A.scalar_type()), qa, qa ? qa + data_bytes(T, K) : nullptr, data, scales, offsets, wide,
                        out.data_ptr(), N, type_of(out_type), T, (int)groups, (int)N, (int)K, 1, stream);
   }, out);
   END_HANDLE_TH_ERRORS

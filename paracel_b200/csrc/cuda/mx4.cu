@@ -114,6 +114,23 @@ __device__ __forceinline__ uint32_t top_bits<__half>(const uint4* raw) {
   return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top_16(raw[0]))));
 }
 
+// Eight values of a block that starts at a multiple of four lanes, `most` the bits of the largest magnitude of these: their codes, and in `word` the word of scales
+// of the sixteen lanes around.  `in`: the row has this block.
+__device__ __forceinline__ uint32_t encode8(float (&v)[8], uint32_t most, bool in, int part, uint32_t& word) {
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+  const bool bad = most >= 0x7f800000u;
+  // floor(log2(most)) - 2, at least -127 (all that is below 2^-125 takes the smallest scale)
+  const int code = bad ? 255 : max((int)(most >> 23) - 2, 0);
+  const float inv = __uint_as_float((uint32_t)(254 - min(code, 253)) << 23);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = mul_keep(v[j], inv);   // no matter which in a block that is not a number
+  word = in ? (uint32_t)code << (8 * (part >> 2)) : 0u;
+  word |= __shfl_xor_sync(0xffffffffu, word, 4);
+  word |= __shfl_xor_sync(0xffffffffu, word, 8);
+  return pack8(v);
+}
+
 // VEC: rows start at multiples of 16 bytes and have a multiple of eight values.  ALONG: a CTA has eight words of a row (shift 3) and a thread goes along one
 // row instead of down one column (bf16 32768 x 8192: 120 instead of 134 us).
 template <int ITERS, bool VEC, bool ALONG, class T>
@@ -159,20 +176,10 @@ __global__ void __launch_bounds__(QTHREADS, !VEC ? 1 : sizeof(T) == 4 ? 4 : 6) q
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
-    uint32_t most = top_bits<T>(raw[i]);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const bool bad = most >= 0x7f800000u;
-    // floor(log2(most)) - 2, at least -127 (all that is below 2^-125 takes the smallest scale)
-    const int code = bad ? 255 : max((int)(most >> 23) - 2, 0);
-    const float inv = __uint_as_float((uint32_t)(254 - min(code, 253)) << 23);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = mul_keep(v[j], inv);   // no matter which in a block that is not a number
     const bool in = c + (ALONG ? i * 256 : 0) < row_words * 8;
-    if (in && i * step < left) dst[i * dst_step] = pack8(v);
-    uint32_t w = in ? (uint32_t)code << (8 * (part >> 2)) : 0u;
-    w |= __shfl_xor_sync(0xffffffffu, w, 4);
-    w |= __shfl_xor_sync(0xffffffffu, w, 8);
+    uint32_t w;
+    const uint32_t codes = encode8(v, top_bits<T>(raw[i]), in, part, w);
+    if (in && i * step < left) dst[i * dst_step] = codes;
     if (part == 0) words[slot + i * slot_step] = w;
   }
   __syncthreads();
@@ -264,7 +271,6 @@ __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
 constexpr int LANES = 128;
 constexpr int BR = 256;                        // values of a row in a stage: 128 bytes
 constexpr int P_BYTES = LANES * 128;
-constexpr int SCALE_BYTES = 3 * 1024;          // P, Q rows 0-127, Q rows 128-255: two blocks of 512 bytes each
 constexpr int SCALE_COLS = 24;
 constexpr int TMEM_COLS = 512;
 constexpr int MAX_STAGES = 7;
@@ -277,17 +283,22 @@ constexpr int small_box(int cols) { return (cols / 4 + 7) / 8 * 8; }
 
 // COLS: columns of an accumulator, the most rows of A in a tile.  64 of them leave room for seven stages of 27 KB, 128 for five of 35, 208 for four of 45.
 // SPLIT: a cluster shares a tile's reduction (COLS 64 only)
-template <int COLS, bool SPLIT>
+// FUSED: A comes as bf16, fp16 or fp32, and a CTA quantises the rows of its one tile into shared memory, where they stay; stages hold P alone (COLS 64 only)
+template <int COLS, bool SPLIT, bool FUSED>
 struct Form {
-  static constexpr int STAGE_BYTES = P_BYTES + COLS * 128;
+  static constexpr int STAGE_BYTES = P_BYTES + (FUSED ? 0 : COLS * 128);
+  static constexpr int SCALE_BYTES = (FUSED ? 1 : 3) * 1024;   // P, Q rows 0-127, Q rows 128-255: two blocks of 512 bytes each
   static constexpr int SMALL_BOX = small_box(COLS);
-  static constexpr int STAGES = (192 * 1024 - (SPLIT ? INBOX_BYTES : 0)) / (STAGE_BYTES + SCALE_BYTES);
+  static constexpr int STAGES = FUSED ? 6 : (192 * 1024 - (SPLIT ? INBOX_BYTES : 0)) / (STAGE_BYTES + SCALE_BYTES);
   static constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (SPLIT ? INBOX_BYTES : 0);   // and Shared
   static_assert(STAGES <= MAX_STAGES, "barriers");
   static_assert(2 * COLS + STAGES * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
   static_assert(COLS % 16 == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
 };
 constexpr int FEW_COLS = 64, SOME_COLS = 128, MANY_COLS = 208;
+constexpr int FUSED_MOST = 56 * 1024;          // bytes of a tile's quantised rows that leave room for the rest
+// Bytes of `rows` quantised rows over `steps` stages: 128 of values each, and a block of scales for either half
+constexpr int fused_bytes(int rows, int steps) { return steps * (rows * 128 + 1024); }
 
 struct Args {
   const uint32_t* sp;   // words of B's scales [words, groups * N]
@@ -298,10 +309,15 @@ struct Args {
   int N, steps, words, blocks, fill;
   bool boxed;   // results leave through mapOut
   bool behind;  // the kernel before is the quantisation of A, and wrote nothing else that is read here
+  // FUSED
+  const void* x;
+  long long ldx;
+  int x_type, K, room, cap;   // room: bytes of shared memory for `cap` quantised rows
+  bool x_vec;                 // rows of x can be read 16 bytes at a time
 };
 
 struct Shared {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2];
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2], quantized;
   uint32_t tmem;
   int abort_flag;
   Table table;
@@ -363,14 +379,93 @@ struct Walk {
   }
 };
 
-template <int COLS, bool SPLIT, class TO>
+// Eight values of a row, from column c on, zeros behind column K; and the bits of their largest magnitude
+__device__ __forceinline__ void load8(const Args& a, long long r, int c, float (&v)[8]) {
+  const int size = a.x_type == TYPE_F32 ? 4 : 2;
+  const char* p = static_cast<const char*>(a.x) + (r * a.ldx + c) * size;
+  if (a.x_vec && c + 8 <= a.K) {
+    uint4 raw[2];
+    raw[0] = *reinterpret_cast<const uint4*>(p);
+    if (size == 4) {
+      raw[1] = *(reinterpret_cast<const uint4*>(p) + 1);
+      memcpy(v, raw, 32);
+    } else {
+      const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (a.x_type == TYPE_BF16) {
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(w + i));
+          v[2 * i] = f.x;
+          v[2 * i + 1] = f.y;
+        }
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    v[j] = 0.f;
+    if (c + j < a.K) {
+      if (size == 4) v[j] = reinterpret_cast<const float*>(p)[j];
+      else if (a.x_type == TYPE_BF16) v[j] = to_f32(reinterpret_cast<const __nv_bfloat16*>(p)[j]);
+      else v[j] = to_f32(reinterpret_cast<const __half*>(p)[j]);
+    }
+  }
+}
+
+// FUSED: the rows of the tile into `room`, by warp `w` of QUANT_WARPS: for every stage `cap` rows of 128 bytes, swizzled as an operand, behind them for every stage two
+// blocks of scales.  Sixteen lanes take a word of scales, 128 values; two words of each lane are on their way together.
+constexpr int QUANT_WARPS = EPI_WARPS + 2;
+__device__ __forceinline__ void quantize_tile(const Args& a, const Tile& t, uint8_t* room, int w) {
+  const int lane = threadIdx.x & 31, part = lane & 15;
+  const int across = 2 * (t.k1 - t.k0), units = t.n * across, row_values = a.blocks * 32;
+  uint8_t* scales = room + (t.k1 - t.k0) * a.cap * 128;
+  constexpr int AHEAD = 2;
+  for (int u0 = w * 2 + (lane >> 4); u0 - (lane >> 4) < units; u0 += 2 * QUANT_WARPS * AHEAD) {
+    float v[AHEAD][8];
+    int row[AHEAD], word[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int u = u0 + i * 2 * QUANT_WARPS;
+      row[i] = u / across;
+      word[i] = u - row[i] * across;
+      if (u < units) {
+        load8(a, (long long)t.j0 + row[i], (t.k0 * 2 + word[i]) * 128 + part * 8, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[i][j]) & 0x7fffffffu);
+      const bool in = (t.k0 * 2 + word[i]) * 128 + part * 8 < row_values;
+      uint32_t scale;
+      const uint32_t codes = encode8(v[i], most, in, part, scale);
+      if (u0 + i * 2 * QUANT_WARPS < units) {
+        const int r = row[i], step = word[i] >> 1, half = word[i] & 1, chunk = half * 4 + (part >> 2);
+        *reinterpret_cast<uint32_t*>(room + (step * a.cap + r) * 128 + ((chunk ^ (r & 7)) << 4) + (part & 3) * 4) = in ? codes : 0u;
+        if (part == 0) *reinterpret_cast<uint32_t*>(scales + step * 1024 + half * 512 + (r & 31) * 16 + (r >> 5) * 4) = scale;
+      }
+    }
+  }
+}
+
+template <int COLS, bool SPLIT, bool FUSED, class TO>
 __global__ void __launch_bounds__(THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                const __grid_constant__ CUtensorMap mapQ_small, const __grid_constant__ CUtensorMap mapOut, Args a) {
-  constexpr int STAGES = Form<COLS, SPLIT>::STAGES, STAGE_BYTES = Form<COLS, SPLIT>::STAGE_BYTES;
+  using F = Form<COLS, SPLIT, FUSED>;
+  constexpr int STAGES = F::STAGES, STAGE_BYTES = F::STAGE_BYTES, SCALE_BYTES = F::SCALE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t* scales = stages + STAGES * STAGE_BYTES;
+  uint8_t* room = stages + STAGES * STAGE_BYTES;                              // FUSED
+  uint8_t* scales = room + (FUSED ? a.room : 0);
   uint8_t* pieces = scales + STAGES * SCALE_BYTES;
   float* inbox = reinterpret_cast<float*>(pieces + EPI_WARPS * PIECE_BYTES);   // SPLIT
   Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES + (SPLIT ? INBOX_BYTES : 0));
@@ -379,11 +474,11 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
 
   if (warp == 0) {
     if (lane < STAGES) {
-      mbar_init(s.full + lane, 1 + 3 * 32);   // the loads, and every lane that copies scales
+      mbar_init(s.full + lane, 1 + (FUSED ? 1 : 3) * 32);   // the loads, and every lane that copies scales
       mbar_init(s.empty + lane, 1);
     }
     if (lane < 2) { mbar_init(s.tfull + lane, 1); mbar_init(s.tempty + lane, EPI_WARPS); }
-    if (lane == 0) s.abort_flag = 0;
+    if (lane == 0) { mbar_init(&s.quantized, QUANT_WARPS); s.abort_flag = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2 && lane == 0) {
@@ -408,6 +503,12 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     *abort_flag = 1;
     ok = false;
   };
+  if (FUSED && warp >= 2 && warp != SCALE_WARP && walk.has(walk.start(group, groups))) {
+    quantize_tile(a, walk.at(walk.start(group, groups)), room, warp < SCALE_WARP ? warp - 2 : warp - 3);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&s.quantized)) : "memory");
+  }
 
   if (warp == 0) {
     after_previous();   // A may still be being quantised
@@ -415,10 +516,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     uint32_t phase = 0;
     for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
       const Tile w = walk.at(i);
-      constexpr int SMALL_BOX = Form<COLS, SPLIT>::SMALL_BOX;
+      constexpr int SMALL_BOX = F::SMALL_BOX;
       const bool whole = w.ncol > 3 * SMALL_BOX;
       const int boxes = whole ? 1 : (w.ncol + SMALL_BOX - 1) / SMALL_BOX;
-      const uint32_t bytes = P_BYTES + (whole ? COLS * 128 : boxes * SMALL_BOX * 128);
+      const uint32_t bytes = P_BYTES + (FUSED ? 0 : whole ? COLS * 128 : boxes * SMALL_BOX * 128);
       for (int kb = w.k0; kb < w.k1; ++kb) {
         if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) { gave_up(41, kb, stage); break; }
         if (elect()) {
@@ -426,7 +527,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
           const uint32_t bar = smem_u32(s.full + stage);
           mbar_expect_tx(s.full + stage, bytes);
           tma_load_3d<1>(sp, &mapP, bar, kb * 128, w.m0, w.e);
-          if (whole) {
+          if (FUSED) {
+          } else if (whole) {
             tma_load_3d<1>(sq, &mapQ, bar, kb * 128, w.j0, 0);
           } else {
             for (int b = 0; b < boxes; ++b)
@@ -454,6 +556,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
       const uint32_t d = tmem + (uint32_t)(acc * COLS);
       const bool wide = w.ncol > 128;
+      if (FUSED && !mbar_wait(&s.quantized, 0, abort_flag)) { gave_up(49, 0, 0); break; }   // a CTA has one tile
       for (int kb = w.k0; kb < w.k1; ++kb) {
         if (!ready && !mbar_wait(s.full + stage, phase, abort_flag)) { gave_up(43, kb, stage); break; }
         const int next = stage + 1 == STAGES ? 0 : stage + 1;
@@ -467,14 +570,15 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
             copy_scales(sf + v * 4, ds + v * 32);
-            copy_scales(sf + 8 + v * 8, ds + 64 + v * 32);
+            copy_scales(sf + 8 + v * 8, FUSED ? desc_scales(smem_u32(room)) + (uint32_t)((w.k1 - w.k0) * a.cap * 128 + (kb - w.k0) * 1024) / 16 + v * 32 : ds + 64 + v * 32);
             if (wide) copy_scales(sf + 12 + v * 8, ds + 128 + v * 32);
           }
           const uint64_t dp = dp0 + (uint32_t)(stage * STAGE_BYTES) / 16;
+          const uint64_t dq = FUSED ? desc_k_major(smem_u32(room)) + (uint32_t)((kb - w.k0) * a.cap * 128) / 16 : dp + P_BYTES / 16;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t id = (uint32_t)(k & 1) * 2;   // codes 0, 1 or 2, 3 of a word
-            umma_mxf4(d, dp + 2 * k, dp + P_BYTES / 16 + 2 * k, idesc | (id << 4) | (id << 29), sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8,
+            umma_mxf4(d, dp + 2 * k, dq + 2 * k, idesc | (id << 4) | (id << 29), sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8,
                           (kb > w.k0 || k > 0) ? 1u : 0u);
           }
           commit<1>(smem_u32(s.empty + stage));
@@ -485,7 +589,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       }
       acc ^= 1;
     }
-  } else if (warp >= SCALE_WARP) {
+  } else if (warp >= SCALE_WARP && (!FUSED || warp == SCALE_WARP)) {
     const int part = warp - SCALE_WARP;      // 0: P, 1 and 2: Q
     if (part > 0) after_previous();
     const long long rows = part == 0 ? (long long)a.off.groups * a.N : a.off.rows;
@@ -524,7 +628,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else {
+  } else if (warp < SCALE_WARP) {
     const int sub = warp & 3;                 // the quarter of the tensor memory's lanes that this warp can read
     const int half = (warp - 2) >> 2;         // two warps share a quarter: 32 columns in turn
     TO* out = static_cast<TO*>(a.out);
@@ -573,10 +677,12 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   }
 }
 
-template <int COLS, bool SPLIT, class TO>
+template <int COLS, bool SPLIT, bool FUSED, class TO>
 int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, int parts, cudaStream_t stream) {
-  auto kernel = product_kernel<COLS, SPLIT, TO>;
-  constexpr int smem = Form<COLS, SPLIT>::SMEM_BYTES + (int)sizeof(Shared);
+  auto kernel = product_kernel<COLS, SPLIT, FUSED, TO>;
+  constexpr int fixed = Form<COLS, SPLIT, FUSED>::SMEM_BYTES + (int)sizeof(Shared);
+  static_assert(fixed + (FUSED ? FUSED_MOST : 0) <= 227 * 1024, "shared memory of an SM");
+  const int smem = fixed + (FUSED ? a.room : 0);
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -591,12 +697,12 @@ int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, co
   return e != cudaSuccess ? (int)e : pcl_last_error();
 }
 
-template <int COLS, bool SPLIT>
+template <int COLS, bool SPLIT, bool FUSED>
 int launch_as(int out_type, const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, int parts,
               cudaStream_t stream) {
-  if (out_type == TYPE_F32) return launch<COLS, SPLIT, float>(p, q, qs, o, a, parts, stream);
-  if (out_type == TYPE_BF16) return launch<COLS, SPLIT, __nv_bfloat16>(p, q, qs, o, a, parts, stream);
-  return launch<COLS, SPLIT, __half>(p, q, qs, o, a, parts, stream);
+  if (out_type == TYPE_F32) return launch<COLS, SPLIT, FUSED, float>(p, q, qs, o, a, parts, stream);
+  if (out_type == TYPE_BF16) return launch<COLS, SPLIT, FUSED, __nv_bfloat16>(p, q, qs, o, a, parts, stream);
+  return launch<COLS, SPLIT, FUSED, __half>(p, q, qs, o, a, parts, stream);
 }
 
 // CTAs of the grid, how long their rows are, and whether they go over four words a thread: where that leaves every SM four of them
@@ -664,6 +770,38 @@ PCL_API int pcl_mx4_dequantize(const void* data, const void* scales, void* out, 
   return pcl_last_error();
 }
 
+struct Plan {
+  int cols, parts, cap, room;
+  bool fused;
+};
+
+// Tiles of the number of rows that takes the shortest time; and whether A, of x_type, is quantised by the product's own CTAs: where each has one tile at most, and the words
+// of its rows go through its warps in one pass (QUANT_WARPS * 4 of them).  One row against 8192 x 4096 takes 9.3 us so, 10.2 with a kernel for the quantisation,
+// most of it the second launch; 64 rows of 8 words a CTA 20 us, and 8.
+static Plan plan_of(int x_type, long long rows, int groups, int N, int K) {
+  Plan plan{0, 1, 0, 0, false};
+  const int steps = (K + 255) / 256;
+  long long least = 0;
+  for (const int c : {FEW_COLS, SOME_COLS, MANY_COLS}) {
+    const long long t = tiles_cost(likely_chunks(rows, groups, c), c, N, steps);
+    if (plan.cols == 0 || t < least) { plan.cols = c; least = t; }
+  }
+  if (plan.cols != FEW_COLS) return plan;
+  const long long tiles = most_chunks(rows, groups, FEW_COLS) * ((N + LANES - 1) / LANES);
+  plan.parts = parts_of(tiles, steps);
+  const int own = (steps + plan.parts - 1) / plan.parts;
+  plan.cap = (int)(rows < FEW_COLS ? (rows + 15) / 16 * 16 : FEW_COLS);
+  plan.fused = x_type >= 0 && tiles * plan.parts <= SMS && 2 * own * min(rows, (long long)FEW_COLS) <= 4 * QUANT_WARPS && fused_bytes(plan.cap, own) <= FUSED_MOST;
+  plan.room = plan.fused ? fused_bytes(plan.cap, own) : 0;
+  return plan;
+}
+
+// Bytes that A and its scales have to have room for in a call with an x of x_type
+PCL_API long long pcl_mx4_room(int x_type, long long rows, int groups, int N, int K) {
+  if (rows < 1 || groups < 1 || N < 1 || K < 1 || plan_of(x_type, rows, groups, N, K).fused) return 0;
+  return rows * ((K + 31) / 32 * 16ll + (K + 127) / 128 * 4ll);
+}
+
 // A [rows, K], B [groups * N, K], both in four bits -> out [rows, N] of out_type; offsets null: one group of all rows.  x_type 0, 1, 2: A and
 // sa are room for x [rows, K] (fp32, bf16, fp16, rows ldx values apart), which is quantised into them first; -1: they are the operand.
 PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void* sa, const void* B, const void* sb, const void* offsets,
@@ -674,32 +812,29 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
     return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   if (out_type < 0 || out_type > 2) return (int)cudaErrorInvalidValue;
-  if (x_type >= 0) {
+  const long long row_bytes = (K + 31) / 32 * 16;
+  const Plan plan = plan_of(x_type, rows, groups, N, K);
+  const int cols = plan.cols;
+  if (x_type >= 0 && !plan.fused) {
     const int rc = quantize(x, ldx, x_type, A, sa, rows, K, stream);
     if (rc) return rc;
-  }
-  const long long row_bytes = (K + 31) / 32 * 16;
-  // tiles of the number of rows that takes the shortest time
-  int cols = 0;
-  long long least = 0;
-  for (const int c : {FEW_COLS, SOME_COLS, MANY_COLS}) {
-    const long long t = tiles_cost(likely_chunks(rows, groups, c), c, N, (int)((row_bytes + 127) / 128));
-    if (cols == 0 || t < least) { cols = c; least = t; }
   }
   CUtensorMap p, q, qs, o;
   const CUtensorMapDataType t = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int rc = make_map_3d(&p, t, B, row_bytes, N, groups, row_bytes, row_bytes * N, 128, LANES);
-  if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, cols);
-  if (rc == 0) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, small_box(cols));
+  if (plan.fused) q = qs = p;   // not used
+  else if (rc == 0) rc = make_map_3d(&q, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, cols);
+  if (rc == 0 && !plan.fused) rc = make_map_3d(&qs, t, A, row_bytes, rows, 1, row_bytes, row_bytes, 128, small_box(cols));
   if (rc) return rc;
   Args a{static_cast<const uint32_t*>(sb), static_cast<const uint32_t*>(sa), out, ldo, Offsets{offsets, off64, groups, (int)rows},
-         N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false, x_type >= 0};
+         N, (int)((row_bytes + 127) / 128), (K + 127) / 128, (K + 31) / 32, fill, false, x_type >= 0 && !plan.fused,
+         x, ldx, x_type, K, plan.room, plan.cap, ((uintptr_t)x & 15) == 0 && (ldx * (x_type == TYPE_F32 ? 4 : 2) & 15) == 0};
   a.boxed = make_out_map(&o, p, out_type, out, N, rows, 1, ldo, ldo);
-  if (cols == SOME_COLS) return launch_as<SOME_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
-  if (cols == MANY_COLS) return launch_as<MANY_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
-  const long long tiles = most_chunks(rows, groups, FEW_COLS) * ((N + LANES - 1) / LANES);
-  const int parts = parts_of(tiles, a.steps);
-  return parts > 1 ? launch_as<FEW_COLS, true>(out_type, p, q, qs, o, a, parts, stream) : launch_as<FEW_COLS, false>(out_type, p, q, qs, o, a, 1, stream);
+  if (cols == SOME_COLS) return launch_as<SOME_COLS, false, false>(out_type, p, q, qs, o, a, 1, stream);
+  if (cols == MANY_COLS) return launch_as<MANY_COLS, false, false>(out_type, p, q, qs, o, a, 1, stream);
+  if (plan.fused)
+    return plan.parts > 1 ? launch_as<FEW_COLS, true, true>(out_type, p, q, qs, o, a, plan.parts, stream) : launch_as<FEW_COLS, false, true>(out_type, p, q, qs, o, a, 1, stream);
+  return plan.parts > 1 ? launch_as<FEW_COLS, true, false>(out_type, p, q, qs, o, a, plan.parts, stream) : launch_as<FEW_COLS, false, false>(out_type, p, q, qs, o, a, 1, stream);
 }
 
 // Copies the status block of these products to `host` and clears it (waits for the stream).

@@ -82,6 +82,7 @@ SIGS = {
     "pcl_mx4_dequantize": "pppqiqip",
     "pcl_mx4_rows": "pqipppppipqiqiiiip",
     "pcl_mx4_status": "pp",
+    "pcl_mx4_room": "iqiii",
 }
 
 
@@ -103,7 +104,7 @@ def register(name: str, spec: str) -> None:
 def _bind(name, spec):
     fn = getattr(_LIB, name)
     fn.argtypes = [_T[c] for c in spec]
-    fn.restype = ctypes.c_int
+    fn.restype = ctypes.c_longlong if name == "pcl_mx4_room" else ctypes.c_int
     return fn
 
 

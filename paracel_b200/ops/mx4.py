@@ -219,7 +219,7 @@ def _product(A, B: Mx4Matrix, offsets, out, out_dtype):
         # A in four bits, for the length of the call
         A, ldx = _row_stride(A)
         size = T * ((K + 31) // 32 * 16)
-        work = torch.empty(size + T * ((K + 127) // 128 * 4), dtype=torch.uint8, device=out.device)
+        work = torch.empty(_lib.load().pcl_mx4_room(kind, T, groups, N, K), dtype=torch.uint8, device=out.device)
         x, a = A.data_ptr(), work.data_ptr()
         sa = a + size
     _lib.call_on(device, "pcl_mx4_rows", x, ldx, kind, a, sa, B._data_ptr, B._scales_ptr, None if offsets is None else offsets.data_ptr(),
