@@ -2,7 +2,7 @@
 //
 // A call of these takes the device a few microseconds at the smallest sizes, and looking at the tensors, two torch.empty and a foreign call
 // through ctypes took the host more than the launches themselves.  Every function here looks at its arguments, and where they are
-// as they mostly are (one device, the current one; aligned rows; a new result) makes the result and launches; for anything else, an error
+// as they mostly are (one device, the current one; contiguous columns; a new result) makes the result and launches; for anything else, an error
 // among it, it returns None, and the caller goes the long way.  The launchers are the extern "C" ones of libpcl_kernels.so, bound
 // by address.
 #include <Python.h>
@@ -20,6 +20,8 @@ using Rows = int (*)(int, int, int, const void*, long long, const void*, long lo
                      long long, int, int, int, int, cudaStream_t);
 using Tn = int (*)(int, int, const void*, long long, const void*, long long, const void*, int, void*, long long, int, int, int,
                    cudaStream_t);
+using PadFn = int (*)(const void*, long long, long long, long long, long long, int, void*, const void*, long long, long long, long long, long long, int,
+                      void*, cudaStream_t);
 using Quantize = int (*)(const void*, long long, int, void*, void*, long long, int, cudaStream_t);
 using Dequantize = int (*)(const void*, const void*, void*, long long, int, long long, int, cudaStream_t);
 using Mx4Rows = int (*)(const void*, long long, int, void*, void*, const void*, const void*, const void*, int, void*, long long, int, long long,
@@ -29,6 +31,7 @@ using ErrorString = const char* (*)(int);
 
 Rows rows_fn;
 Tn tn_fn;
+PadFn pad_fn;
 Quantize quantize_fn;
 Dequantize dequantize_fn;
 Mx4Rows mx4_rows_fn;
@@ -62,12 +65,49 @@ bool plain_offsets(const at::Tensor& o, int device) {
          o.size(0) <= MAX_GROUPS + 1 && o.is_contiguous() && here(o, device);
 }
 
-bool aligned(const at::Tensor& t) {   // 16-bit rows at multiples of 16 bytes
-  const int64_t d = t.dim();
-  if ((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) || t.stride(d - 1) != 1) return false;
-  for (int64_t i = 0; i + 1 < d; ++i)
-    if (t.stride(i) <= 0 || (t.stride(i) & 7)) return false;
-  return true;
+// A 16-bit operand [mats, rows, cols] with contiguous columns: as it lies where its rows start at multiples of 16 bytes, else with a copy to be made
+struct Operand {
+  const void* at;
+  int64_t mats, rows, cols, step_e, step;
+  bool plain, copy;
+
+  explicit Operand(const at::Tensor& t) : at(t.data_ptr()) {
+    const int64_t d = t.dim();
+    mats = d == 3 ? t.size(0) : 1;
+    rows = t.size(d - 2);
+    cols = t.size(d - 1);
+    step = rows > 1 ? t.stride(d - 2) : pitch();   // a dimension of one index may report any stride
+    step_e = mats > 1 ? t.stride(0) : rows * step;
+    plain = t.stride(d - 1) == 1 || cols == 1;
+    copy = (reinterpret_cast<uintptr_t>(at) & 15) || step <= 0 || (step & 7) || step_e <= 0 || (step_e & 7);
+  }
+  int64_t pitch() const { return (cols + 7) / 8 * 8; }
+  int64_t bytes() const { return copy ? mats * rows * pitch() * 2 : 0; }
+  Operand copied(void* to) const {
+    Operand o = *this;
+    if (copy) { o.at = to; o.step = pitch(); o.step_e = rows * o.step; }
+    return o;
+  }
+};
+
+// Buffer for the copies of what has to be copied
+at::Tensor room_for(const Operand& a, const Operand& b, const at::TensorOptions& options) {
+  return a.copy || b.copy ? at::empty({a.bytes() + b.bytes()}, options.dtype(at::kByte)) : at::Tensor();
+}
+
+// Copies it there, and points the operands to it
+int copy_operands(Operand& a, Operand& b, const at::Tensor& room, cudaStream_t stream) {
+  if (!a.copy && !b.copy) return 0;
+  char* to = static_cast<char*>(room.data_ptr());
+  const Operand na = a.copied(to), nb = b.copied(to + a.bytes());
+  const Operand& x = a.copy ? a : b;
+  void* dst = const_cast<void*>((a.copy ? na : nb).at);
+  const bool both = a.copy && b.copy;
+  const int rc = pad_fn(x.at, x.step_e, x.step, x.mats, x.rows, (int)x.cols, dst, both ? b.at : nullptr, b.step_e, b.step, b.mats, b.rows, (int)b.cols,
+                        both ? const_cast<void*>(nb.at) : nullptr, stream);
+  a = na;
+  b = nb;
+  return rc;
 }
 
 bool size_ok(int64_t v) { return v > 0 && v < MAX_SIZE; }
@@ -82,21 +122,23 @@ PyObject* launched(const char* name, F&& launch, const at::Tensor& result) {
   return THPVariable_Wrap(result);
 }
 
-// bind(rows, tn, quantize, dequantize, mx4_rows, mx4_room, error_string): addresses
+// bind(rows, tn, pad, quantize, dequantize, mx4_rows, mx4_room, error_string): addresses
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7) return PyErr_Format(PyExc_TypeError, "seven addresses are wanted");
-  void* p[7];
-  for (int i = 0; i < 7; ++i) {
+  constexpr int COUNT = 8;
+  if (n != COUNT) return PyErr_Format(PyExc_TypeError, "%d addresses are wanted", COUNT);
+  void* p[COUNT];
+  for (int i = 0; i < COUNT; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (p[i] == nullptr) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "address %d is null", i);
   }
   rows_fn = reinterpret_cast<Rows>(p[0]);
   tn_fn = reinterpret_cast<Tn>(p[1]);
-  quantize_fn = reinterpret_cast<Quantize>(p[2]);
-  dequantize_fn = reinterpret_cast<Dequantize>(p[3]);
-  mx4_rows_fn = reinterpret_cast<Mx4Rows>(p[4]);
-  mx4_room_fn = reinterpret_cast<Mx4Room>(p[5]);
-  error_fn = reinterpret_cast<ErrorString>(p[6]);
+  pad_fn = reinterpret_cast<PadFn>(p[2]);
+  quantize_fn = reinterpret_cast<Quantize>(p[3]);
+  dequantize_fn = reinterpret_cast<Dequantize>(p[4]);
+  mx4_rows_fn = reinterpret_cast<Mx4Rows>(p[5]);
+  mx4_room_fn = reinterpret_cast<Mx4Room>(p[6]);
+  error_fn = reinterpret_cast<ErrorString>(p[7]);
   Py_RETURN_NONE;
 }
 
@@ -114,14 +156,18 @@ PyObject* grouped_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t T = X.size(0), E = W.size(0), N = W.size(1), K = W.size(2);
   if (in < 1 || W.scalar_type() != type || !type_arg(a[4], type, &out_type) || (out_type != type && out_type != at::kFloat) || T < 1 ||
       T >= MAX_ROWS || !size_ok(N) || !size_ok(K) || X.size(1) != (mode == 0 ? K : N) || !plain_offsets(offsets, device) ||
-      offsets.size(0) != E + 1 || !here(X, device) || !here(W, device) || !aligned(X) || !aligned(W))
+      offsets.size(0) != E + 1 || !here(X, device) || !here(W, device))
     Py_RETURN_NONE;
+  Operand x(X), w(W);
+  if (!x.plain || !w.plain) Py_RETURN_NONE;
   const int64_t cols = mode == 0 ? N : K;
   const at::Tensor out = at::empty({T, cols}, X.options().dtype(out_type));
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  const at::Tensor room = room_for(x, w, X.options());
   return launched("pcl_grouped_rows", [&] {
-    return rows_fn((int)mode, in, type_of(out_type), X.data_ptr(), X.stride(0), W.data_ptr(), W.stride(0), W.stride(1), offsets.data_ptr(),
-                   offsets.scalar_type() == at::kLong, out.data_ptr(), cols, T, (int)E, (int)N, (int)K, 1, stream);
+    const int rc = copy_operands(x, w, room, stream);
+    return rc ? rc : rows_fn((int)mode, in, type_of(out_type), x.at, x.step, w.at, w.step_e, w.step, offsets.data_ptr(),
+                             offsets.scalar_type() == at::kLong, out.data_ptr(), cols, T, (int)E, (int)N, (int)K, 1, stream);
   }, out);
   END_HANDLE_TH_ERRORS
 }
@@ -138,15 +184,18 @@ PyObject* grouped_tn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::ScalarType out_type;
   const int64_t T = X.size(0), K = X.size(1), N = Y.size(1);
   if (in < 1 || Y.scalar_type() != type || !type_arg(a[3], type, &out_type) || (out_type != type && out_type != at::kFloat) || T < 1 ||
-      T >= MAX_ROWS || Y.size(0) != T || !size_ok(N) || !size_ok(K) || !plain_offsets(offsets, device) || !here(X, device) || !here(Y, device) ||
-      !aligned(X) || !aligned(Y))
+      T >= MAX_ROWS || Y.size(0) != T || !size_ok(N) || !size_ok(K) || !plain_offsets(offsets, device) || !here(X, device) || !here(Y, device))
     Py_RETURN_NONE;
+  Operand x(X), y(Y);
+  if (!x.plain || !y.plain) Py_RETURN_NONE;
   const int64_t E = offsets.size(0) - 1;
   const at::Tensor out = at::empty({E, N, K}, X.options().dtype(out_type));
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  const at::Tensor room = room_for(x, y, X.options());
   return launched("pcl_grouped_tn", [&] {
-    return tn_fn(in, type_of(out_type), Y.data_ptr(), Y.stride(0), X.data_ptr(), X.stride(0), offsets.data_ptr(),
-                 offsets.scalar_type() == at::kLong, out.data_ptr(), T, (int)E, (int)N, (int)K, stream);
+    const int rc = copy_operands(x, y, room, stream);
+    return rc ? rc : tn_fn(in, type_of(out_type), y.at, y.step, x.at, x.step, offsets.data_ptr(), offsets.scalar_type() == at::kLong, out.data_ptr(), T,
+                           (int)E, (int)N, (int)K, stream);
   }, out);
   END_HANDLE_TH_ERRORS
 }

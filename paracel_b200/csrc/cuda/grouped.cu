@@ -450,7 +450,95 @@ bool sizes_ok(int in_type, long long rows, int groups, int N, int K) {
          groups <= MAX_GROUPS && N >= 1 && N < (1 << 30) && K >= 1 && K < (1 << 30);
 }
 
+// ---- operands whose rows do not start at multiples of 16 bytes ----
+//
+// The tensor copies cannot read these, so a call copies them first, both of a product in one launch: rows of any distance to rows of whole 16 bytes, the last one
+// filled up with zeros.  A thread has a chunk of 16 bytes of up to PAD_CHUNKS places of a row, and reads it in the largest units that the rows' starts share
+// (WIDTH values: an odd number of columns leaves two bytes).  Bound by the launch for small operands, by memory for large ones.
+constexpr int PAD_THREADS = 256, PAD_CHUNKS = 4;
+
+struct Pad {
+  const uint16_t* src;
+  uint4* dst;
+  long long step_e, step, rows, per;   // `per` rows of a matrix
+  int cols, shift, col_blocks, width;  // 2^shift threads to a row
+  long long blocks;
+};
+
+template <class U>
+__device__ __forceinline__ uint4 load_chunk(const uint16_t* src) {
+  constexpr int N = 16 / sizeof(U);
+  U v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const U*>(src)[i];
+  uint4 r;
+  memcpy(&r, v, 16);
+  return r;
+}
+
+__global__ void __launch_bounds__(PAD_THREADS) pad_kernel(const __grid_constant__ Pad first, const __grid_constant__ Pad second) {
+  after_previous();
+  let_next_begin();
+  const bool other = blockIdx.x >= first.blocks;
+  const Pad& p = other ? second : first;
+  const unsigned b = blockIdx.x - (other ? (unsigned)first.blocks : 0u);
+  const unsigned row_block = b / (unsigned)p.col_blocks, col_block = b - row_block * p.col_blocks;
+  const long long r = (long long)row_block * (PAD_THREADS >> p.shift) + (threadIdx.x >> p.shift);
+  if (r >= p.rows) return;
+  const int chunks = (p.cols + 7) >> 3, lanes = 1 << p.shift;
+  const int c0 = (int)col_block * (lanes * PAD_CHUNKS) + ((int)threadIdx.x & (lanes - 1));
+  const long long e = p.per == p.rows ? 0 : r / p.per;
+  const uint16_t* src = p.src + e * p.step_e + (r - e * p.per) * p.step;
+  uint4 v[PAD_CHUNKS];
+#pragma unroll
+  for (int i = 0; i < PAD_CHUNKS; ++i) {
+    const int c = c0 + i * lanes;
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (c * 8ll + 8 <= p.cols) {
+      const uint16_t* at = src + c * 8ll;
+      v[i] = p.width == 4 ? load_chunk<uint2>(at) : p.width == 2 ? load_chunk<uint32_t>(at) : load_chunk<uint16_t>(at);
+    } else if (c < chunks) {
+      uint16_t t[8] = {};
+      const int left = p.cols - c * 8;
+#pragma unroll
+      for (int j = 0; j < 7; ++j)
+        if (j < left) t[j] = src[c * 8ll + j];
+      memcpy(&v[i], t, 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PAD_CHUNKS; ++i)
+    if (c0 + i * lanes < chunks) p.dst[r * chunks + c0 + i * lanes] = v[i];
+}
+
+// matrices [mats, rows, cols] of 16-bit values, the columns contiguous
+bool pad_of(Pad* p, const void* src, long long step_e, long long step, long long mats, long long rows, long long cols, void* dst) {
+  if (mats < 1 || rows < 1 || cols < 1 || cols >= (1 << 30) || ((uintptr_t)src & 1) || ((uintptr_t)dst & 15)) return false;
+  *p = Pad{static_cast<const uint16_t*>(src), static_cast<uint4*>(dst), step_e, step, mats * rows, rows, (int)cols, 0, 1, 1, 0};
+  if (step_e == rows * step) p->per = p->rows;
+  const unsigned long long bits = (uintptr_t)src / 2 | (unsigned long long)(p->per == p->rows ? 0 : step_e) | (unsigned long long)step;
+  p->width = bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+  const long long chunks = (cols + 7) / 8;
+  while (p->shift < 5 && (1ll << p->shift) < chunks) ++p->shift;
+  const long long place = (long long)PAD_CHUNKS << p->shift;
+  p->col_blocks = (int)((chunks + place - 1) / place);
+  const long long per_block = PAD_THREADS >> p->shift;
+  p->blocks = (p->rows + per_block - 1) / per_block * p->col_blocks;
+  return p->blocks < (1ll << 30);
+}
+
 }  // namespace
+
+// Copies of one or two operands [mats, rows, cols] of 16-bit values, matrices step_e and rows step values apart, the columns contiguous: dst has
+// mats * rows rows of ceil(cols / 8) * 8 values.  second may be null.
+PCL_API int pcl_grouped_pad(const void* first, long long step_e, long long step, long long mats, long long rows, int cols, void* dst, const void* second,
+                            long long step_e2, long long step2, long long mats2, long long rows2, int cols2, void* dst2, cudaStream_t stream) {
+  Pad a{}, b{};
+  if (!pad_of(&a, first, step_e, step, mats, rows, cols, dst)) return (int)cudaErrorInvalidValue;
+  if (second != nullptr && !pad_of(&b, second, step_e2, step2, mats2, rows2, cols2, dst2)) return (int)cudaErrorInvalidValue;
+  Launch l((unsigned)(a.blocks + b.blocks), PAD_THREADS, 0, 1, stream);
+  return (int)cudaLaunchKernelEx(&l.cfg, pad_kernel, a, b);
+}
 
 // mode 0: X [rows, K] -> out [rows, N]; mode 1: X [rows, N] -> out [rows, K].  W [groups, N, K] with strides (ws_e, ws_n, 1); rows of X and W
 // start at multiples of 16 bytes.  in_type 1 / 2 (bf16 / fp16), out_type the same or 0 (fp32).  fill: rows of no group

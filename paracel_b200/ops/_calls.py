@@ -10,7 +10,7 @@ import os
 from .. import _build
 from . import _lib
 
-_ENTRIES = ("pcl_grouped_rows", "pcl_grouped_tn", "pcl_mx4_quantize", "pcl_mx4_dequantize", "pcl_mx4_rows", "pcl_mx4_room",
+_ENTRIES = ("pcl_grouped_rows", "pcl_grouped_tn", "pcl_grouped_pad", "pcl_mx4_quantize", "pcl_mx4_dequantize", "pcl_mx4_rows", "pcl_mx4_room",
             "pcl_error_string")
 _mod = None
 

@@ -100,15 +100,20 @@ def check_out(out: Optional[torch.Tensor], shape, dtype) -> None:
 
 
 def aligned(x: torch.Tensor) -> torch.Tensor:
-    """``x`` if its last dimension is contiguous and every row starts at a multiple of 16 bytes, as the tensor copies need
-    it, else a copy that does."""
-    per = 16 // x.element_size()
-    if (x.shape[-1] == 1 or x.stride(-1) == 1) and x.data_ptr() % 16 == 0 and \
-            all(s % per == 0 and s > 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
+    """The 16-bit matrix or matrices ``x`` if the last dimension is contiguous and every row starts at a multiple of 16 bytes, as
+    the tensor copies need it, else a copy that does."""
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    if x.data_ptr() % 16 == 0 and all(s % 8 == 0 and s > 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
         return x
-    cols = x.shape[-1]
-    buf = torch.empty(*x.shape[:-1], (cols + per - 1) // per * per, dtype=x.dtype, device=x.device)[..., :cols]
-    return buf.copy_(x)
+    *mats, rows, cols = x.shape
+    pitch = (cols + 7) // 8 * 8
+    buf = torch.empty(*mats, rows, pitch, dtype=x.dtype, device=x.device)
+    step = stride_of(x, -2, pitch)
+    step_e = stride_of(x, 0, rows * step) if mats else rows * step
+    _lib.call_on(x.get_device(), "pcl_grouped_pad", x.data_ptr(), step_e, step, mats[0] if mats else 1, rows, cols, buf.data_ptr(),
+                 0, 0, 0, 0, 0, 0, 0)
+    return buf[..., :cols]
 
 
 def stride_of(x: torch.Tensor, dim: int, size: int) -> int:
@@ -195,7 +200,7 @@ def grouped_nt(X: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, out: Opt
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``Y [T, N]`` with ``Y[t] = W[e] x[t]`` for the rows of every group ``e``.
 
-    ``X [T, K]`` and ``W [E, N, K]`` may be strided; where their rows do not start at multiples of 16 bytes (an odd K) they are copied
+    ``X [T, K]`` and ``W [E, N, K]`` may be strided; where rows do not start at multiples of 16 bytes (an odd K) they are copied
     first.  Rows that no group has, before ``offsets[0]`` or from ``offsets[E]`` on, are zero in a new result, and are
     left as they were in ``out``, which must not overlap an operand."""
     return _rows(0, X, W, offsets, out, out_dtype)

@@ -412,3 +412,27 @@ def test_training_steps_of_a_grouped_layer():
         _near(dW, ref, mags, most)
         W -= 0.5 * dW
     check_status()
+
+
+@pytest.mark.parametrize("mats,rows,cols,step,extra,start", [
+    (1, 1, 1, 1, 0, 1), (1, 5, 7, 7, 0, 0), (1, 3, 8, 9, 0, 0), (2, 4, 9, 10, 3, 1), (3, 33, 20, 22, 0, 2), (1, 300, 33, 36, 0, 4), (2, 9, 1000, 1001, 1, 3),
+    (1, 3, 1031, 1032, 0, 5), (5, 1, 2050, 2051, 0, 0), (1, 2, 9001, 9001, 0, 7), (4, 17, 64, 0, 40, 1), (1, 70000, 3, 3, 0, 0), (1025, 2, 13, 13, 0, 3),
+])
+def test_operands_are_copied_to_whole_rows(mats, rows, cols, step, extra, start):
+    """Copies of the exact bits, of one operand and of two, zeros behind each row's end and nothing written outside."""
+    from paracel_b200.ops import _lib
+    step_e = rows * step + extra
+    need = start + (mats - 1) * step_e + (rows - 1) * step + cols
+    pitch = (cols + 7) // 8 * 8
+    flat = torch.randint(-32768, 32767, (need,), dtype=torch.int16, device="cuda")
+    src = flat.as_strided((mats, rows, cols), (step_e, step, 1), start)
+    other = torch.randint(-32768, 32767, (19, 5), dtype=torch.int16, device="cuda")
+    second = torch.full((19, 8), 77, dtype=torch.int16, device="cuda")
+    for both in (False, True):
+        room = torch.full((8 + mats * rows * pitch + 8,), 77, dtype=torch.int16, device="cuda")
+        dst = room[8:-8].view(mats, rows, pitch)
+        tail = (other.data_ptr(), 95, 5, 1, 19, 5, second.data_ptr()) if both else (0,) * 7
+        _lib.call_on(0, "pcl_grouped_pad", src.data_ptr(), step_e, step, mats, rows, cols, dst.data_ptr(), *tail)
+        assert torch.equal(dst[..., :cols], src) and not dst[..., cols:].any()
+        assert bool((room[:8] == 77).all()) and bool((room[-8:] == 77).all())
+        assert torch.equal(second[:, :5], other) == both and bool((second[:, 5:] == (0 if both else 77)).all())
