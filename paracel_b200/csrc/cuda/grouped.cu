@@ -41,12 +41,12 @@ constexpr int FIX_WARP = 2 + EPI_WARPS;
 constexpr int threads_of(int mode) { return 64 + 32 * EPI_WARPS + (mode == 2 ? 32 : 0); }
 // CG: CTAs that work on a tile, one or a pair on neighbouring SMs (tcgen05 cta_group::2); each of a pair holds its 128 m and half the j
 // COLS: columns of an accumulator, the most j of a tile
-// SPLIT: a cluster shares a tile's reduction (COLS 64 only)
+// SPLIT: a cluster shares a tile's reduction (single CTAs of 64 or 128 columns)
 template <int CG, int COLS, bool SPLIT>
 struct Form {
   static constexpr int Q_BYTES = COLS / CG * BR * 2;
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
-  static constexpr int STAGES = (OPERAND_BYTES - (SPLIT ? INBOX_BYTES : 0)) / STAGE_BYTES;
+  static constexpr int STAGES = (OPERAND_BYTES - (SPLIT ? inbox_bytes(COLS) : 0)) / STAGE_BYTES;
   static constexpr int M = LANES * CG;   // m of a tile
   // Rows of Q that a load brings: all that fit, or a quarter of them, up to three times.  A load takes the warp that issues it 135 cycles, and the products of a
   // stage 512 at most: four or five loads to a stage were what bound a call.
@@ -117,11 +117,12 @@ struct Walk {
       t.find(a.off.groups, i.c, 16 * CG, w.e, w.j0, w.n);
       w.r0 = 0;
       w.r1 = a.red;
-      if (SPLIT) {   // this CTA's stages
-        const int steps = (a.red + BR - 1) / BR, rank = (int)cluster_ctarank(), parts = (int)cluster_size();
-        w.r0 = rank * steps / parts * BR;
-        w.r1 = min(a.red, (rank + 1) * steps / parts * BR);
-      }
+    }
+    if (SPLIT) {   // this CTA's stages (none, where a group has fewer than the cluster has CTAs)
+      const long long steps = ((long long)w.r1 - w.r0 + BR - 1) / BR;
+      const int rank = (int)cluster_ctarank(), parts = (int)cluster_size(), first = w.r0;
+      w.r0 = first + (int)(rank * steps / parts) * BR;
+      w.r1 = (int)min((long long)w.r1, first + (rank + 1) * steps / parts * BR);
     }
     // (with the wide maps either CTA of a pair begins with a block of 64)
     const int unit = (MODE == TN && a.wide ? 64 : 16) * CG;
@@ -332,6 +333,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const Tile w = walk.at(i);
       const int m = w.m0 + (int)me * LANES + sub * 32;
       TO* dst = out + (MODE == TN ? ((long long)w.e * a.jdim + w.j0) * a.ldo : (long long)w.j0 * a.ldo) + m;
+      if (SPLIT && w.r1 <= w.r0) {   // no rows for this part
+        send_columns(0, sub, half * 32, w.n, inbox, cluster_ctarank(), columns_of_part(w.n, share), true);
+        continue;
+      }
       if (w.r1 <= w.r0) {   // a group without rows: its matrix of sums is zero
         if (m + lane < a.mdim)
           for (int j = half; j < w.n; j += 2) dst[(long long)j * a.ldo + lane] = to_out<TO>(0.f);
@@ -375,10 +380,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     tmem_free<CG>(tmem, 2 * COLS);
   }
-  if (SPLIT && warp >= 2 && walk.has(walk.start(group, groups))) {
+  if (SPLIT && warp >= 2 && warp < FIX_WARP && walk.has(walk.start(group, groups))) {
     const Tile w = walk.at(walk.start(group, groups));
-    add_up<TO>(inbox, w.n, columns_of_part(w.n, share), cluster_ctarank(), share, 64, 32 * EPI_WARPS, static_cast<TO*>(a.out) + (long long)w.j0 * a.ldo + w.m0,
-               a.ldo, a.mdim - w.m0);
+    add_up<TO>(inbox, w.n, columns_of_part(w.n, share), cluster_ctarank(), share, 64, 32 * EPI_WARPS,
+               static_cast<TO*>(a.out) + (MODE == TN ? (long long)w.e * a.jdim + w.j0 : (long long)w.j0) * a.ldo + w.m0, a.ldo, a.mdim - w.m0);
   }
 }
 
@@ -415,7 +420,7 @@ enum Shape { FEW, SOME, MANY, PAIR };
 constexpr int FEW_COLS = 64, SOME_COLS = 128;
 constexpr int SHAPE_COLS[] = {FEW_COLS, SOME_COLS, MAX_COLS, MAX_COLS / 2 /* of each CTA */};
 
-// tn takes the last two only: with few rows to a group its tiles have few stages, and 64 columns instead of 256 in each took 11.1 instead of 9.2 us for 1000
+// tn without a cluster takes the last two only: with few rows to a group its tiles have few stages, and 64 columns instead of 256 in each took 11.1 instead of 9.2 us for 1000
 // rows of 24 groups, 520 x 264.
 bool pairs_pay(long long chunks, int mdim) { return chunks * ((mdim + LANES - 1) / LANES) >= 2 * SMS; }
 
@@ -443,6 +448,35 @@ int launch_shape(Shape shape, int in_type, int out_type, const CUtensorMap& p, c
                      : launch_as<MODE, 1, FEW_COLS, false>(in_type, out_type, p, q, qs, o, a, 1, stream);
   }
   return (int)cudaErrorInvalidValue;
+}
+
+// How tn is done: by pairs, by single CTAs, or by clusters that share the reduction of a tile of 64 or 128 columns, whichever takes the shortest time where all
+// groups have the same rows.  In ns, fitted to the measurements: a stage of a cluster's CTA takes 1.6 for every line of 128 bytes (all SMs load), of a single CTA 0.9,
+// or 72 for each of its loads where these are more; to send and add up the parts takes 800 and 28 for every column.  us without and with clusters: one group of 8192
+// rows, 1024 x 1024: 50 and 34; of 65536 rows, 256 x 512: 357 and 52; three of 15399 rows, 1144 x 128: 42.5 and 19.5; 8 of 4096 rows, 128 x 256: 7.0 and 8.2, so
+// not taken.
+struct TnPlan {
+  bool pair;
+  int parts, cols;   // CTAs of a cluster, columns of a CTA
+};
+
+TnPlan tn_plan(long long rows, int groups, int N, int K, bool wide) {
+  auto blocks = [&](int cols) { return (N + cols - 1) / cols; };
+  if (pairs_pay((long long)groups * blocks(MAX_COLS), K)) return {true, 1, MAX_COLS / 2};
+  const long long each = (rows + groups - 1) / groups, steps = (each + BR - 1) / BR;
+  auto width = [&](int cols) { return (N + blocks(cols) - 1) / blocks(cols); };   // columns of a tile
+  TnPlan plan{false, 1, MAX_COLS};
+  const int loads = wide ? 2 : 2 + (width(MAX_COLS) + 63) / 64;
+  long long least = steps * max(9 * (LANES + width(MAX_COLS)) / 10, 72 * loads);
+  for (const int cols : {FEW_COLS, SOME_COLS}) {
+    const int parts = parts_of((long long)groups * blocks(cols) * ((K + LANES - 1) / LANES), (int)steps);
+    const long long t = (steps + parts - 1) / parts * 16 * (LANES + width(cols)) / 10 + 800 + 28 * cols;
+    if (parts > 1 && t < least) {
+      least = t;
+      plan = {false, parts, cols};
+    }
+  }
+  return plan;
 }
 
 bool sizes_ok(int in_type, long long rows, int groups, int N, int K) {
@@ -569,14 +603,14 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
                            cudaStream_t stream) {
   if (!sizes_ok(in_type, rows, groups, N, K) || rows == 0) return (int)cudaErrorInvalidValue;
   const CUtensorMapDataType t = in_type == TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const bool pair = pairs_pay((long long)groups * ((N + MAX_COLS - 1) / MAX_COLS), K);
   // (a block that is not full would reach into the next row, and behind the last one)
   const bool wide = N % 64 == 0 && K % 64 == 0;
+  const TnPlan plan = tn_plan(rows, groups, N, K, wide);
   CUtensorMap p, q, o;
   int rc = 0;
   if (wide) {
     rc = make_map_3d(&p, t, X, 64, rows, K / 64, ldx * 2, 128, 64, BR, CU_TENSOR_MAP_SWIZZLE_128B, LANES / 64);
-    if (rc == 0) rc = make_map_3d(&q, t, Y, 64, rows, N / 64, ldy * 2, 128, 64, BR, CU_TENSOR_MAP_SWIZZLE_128B, MAX_COLS / (pair ? 2 : 1) / 64);
+    if (rc == 0) rc = make_map_3d(&q, t, Y, 64, rows, N / 64, ldy * 2, 128, 64, BR, CU_TENSOR_MAP_SWIZZLE_128B, plan.cols / 64);
   } else {
     rc = make_map_3d(&p, t, X, K, rows, 1, ldx * 2, ldx * 2, 64, BR);
     if (rc == 0) rc = make_map_3d(&q, t, Y, N, rows, 1, ldy * 2, ldy * 2, 64, BR);
@@ -584,7 +618,10 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
   if (rc) return rc;
   Args a{out, K, Offsets{offsets, off64, groups, (int)rows}, K, N, 0, in_type == TYPE_BF16 ? 1u : 0u, 0, false, wide};
   a.boxed = make_out_map(&o, p, out_type, out, K, N, groups, K, (long long)N * K);
-  return launch_shape<TN>(pair ? PAIR : MANY, in_type, out_type, p, q, q, o, a, stream);
+  if (plan.parts > 1)
+    return plan.cols == FEW_COLS ? launch_as<TN, 1, FEW_COLS, true>(in_type, out_type, p, q, q, o, a, plan.parts, stream)
+                                 : launch_as<TN, 1, SOME_COLS, true>(in_type, out_type, p, q, q, o, a, plan.parts, stream);
+  return launch_shape<TN>(plan.pair ? PAIR : MANY, in_type, out_type, p, q, q, o, a, stream);
 }
 
 // Copies the status block of the grouped products to `host` and clears it (waits for the stream).

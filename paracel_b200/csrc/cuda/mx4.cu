@@ -289,14 +289,14 @@ struct Form {
   static constexpr int STAGE_BYTES = P_BYTES + (FUSED ? 0 : COLS * 128);
   static constexpr int SCALE_BYTES = (FUSED ? 1 : 3) * 1024;   // P, Q rows 0-127, Q rows 128-255: two blocks of 512 bytes each
   static constexpr int SMALL_BOX = small_box(COLS);
-  static constexpr int STAGES = FUSED ? 6 : (192 * 1024 - (SPLIT ? INBOX_BYTES : 0)) / (STAGE_BYTES + SCALE_BYTES);
-  static constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (SPLIT ? INBOX_BYTES : 0);   // and Shared
+  static constexpr int STAGES = FUSED ? 6 : (192 * 1024 - (SPLIT ? inbox_bytes(64) : 0)) / (STAGE_BYTES + SCALE_BYTES);
+  static constexpr int SMEM_BYTES = 1024 + STAGES * (STAGE_BYTES + SCALE_BYTES) + EPI_WARPS * PIECE_BYTES + (SPLIT ? inbox_bytes(64) : 0);   // and Shared
   static_assert(STAGES <= MAX_STAGES, "barriers");
   static_assert(2 * COLS + STAGES * SCALE_COLS <= TMEM_COLS, "accumulators and scales share the tensor memory");
   static_assert(COLS % 16 == 0, "a chunk rounded up to the product's columns fits an accumulator, and none is left empty");
 };
 constexpr int FEW_COLS = 64, SOME_COLS = 128, MANY_COLS = 208;
-constexpr int FUSED_MOST = 56 * 1024;          // bytes of a tile's quantised rows that leave room for the rest
+constexpr int FUSED_MOST = 44 * 1024;          // bytes of a tile's quantised rows that leave room for the rest
 // Bytes of `rows` quantised rows over `steps` stages: 128 of values each, and a block of scales for either half
 constexpr int fused_bytes(int rows, int steps) { return steps * (rows * 128 + 1024); }
 
@@ -468,7 +468,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   uint8_t* scales = room + (FUSED ? a.room : 0);
   uint8_t* pieces = scales + STAGES * SCALE_BYTES;
   float* inbox = reinterpret_cast<float*>(pieces + EPI_WARPS * PIECE_BYTES);   // SPLIT
-  Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES + (SPLIT ? INBOX_BYTES : 0));
+  Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES + (SPLIT ? inbox_bytes(64) : 0));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
 

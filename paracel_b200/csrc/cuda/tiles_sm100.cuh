@@ -341,24 +341,25 @@ static __device__ __forceinline__ uint32_t cluster_size() {
   return r;
 }
 
-constexpr int INBOX_BYTES = (64 + 8) * 128 * 4;   // up to 64 columns, rounded up to 8 parts
-__device__ __forceinline__ int columns_of_part(int n, int parts) { return (n + parts - 1) / parts; }
+constexpr int inbox_bytes(int cols) { return (cols + 4 * 8) * 128 * 4; }   // up to `cols` columns, four to each of 8 parts more
+__device__ __forceinline__ int columns_of_part(int n, int parts) { return ((n + parts - 1) / parts + 3) & ~3; }
 
-// This warp's quarter of the accumulator to the CTAs that add it up: columns [o * each, (o + 1) * each) go to CTA o, there into inbox[rank][column][lane]
-static __device__ __forceinline__ void send_columns(uint32_t taddr, int sub, int first, int n, const float* inbox, uint32_t rank, int each) {
+// This warp's quarter of the accumulator (zeros for `none`) to the CTAs that add it up: columns [o * each, (o + 1) * each) go to CTA o, there into
+// inbox[rank][column / 4][lane][column mod 4]
+static __device__ __forceinline__ void send_columns(uint32_t taddr, int sub, int first, int n, const float* inbox, uint32_t rank, int each,
+                                                    bool none = false) {
   const int lane = threadIdx.x & 31;
 #pragma unroll 1
   for (int c = first; c < n; c += ((c & 31) == 24 ? 40 : 8)) {   // 32 columns of every 64, eight at a time
-    uint32_t v[8];
-    tmem_ld8(taddr + (uint32_t)c, v);
-    int owner = c / each, col = c - owner * each;
+    uint32_t v[8] = {};
+    if (!none) tmem_ld8(taddr + (uint32_t)c, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 8; j += 4) {
       if (c + j < n) {
-        const uint32_t at = map_to_cta(smem_u32(inbox + ((int)rank * each + col) * 128 + sub * 32 + lane), (uint32_t)owner);
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v[j]) : "memory");
+        const int owner = (c + j) / each, col = c + j - owner * each;
+        const uint32_t at = map_to_cta(smem_u32(inbox + ((int)rank * each + col) * 128 + (sub * 32 + lane) * 4), (uint32_t)owner);
+        asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[j]), "r"(v[j + 1]), "r"(v[j + 2]), "r"(v[j + 3]) : "memory");
       }
-      if (++col == each) { col = 0; ++owner; }
     }
     __syncwarp();
   }
@@ -368,11 +369,21 @@ static __device__ __forceinline__ void send_columns(uint32_t taddr, int sub, int
 template <class TO>
 __device__ __forceinline__ void add_up(const float* inbox, int n, int each, uint32_t rank, int parts, int first, int threads, TO* dst, long long ldo, int lanes) {
   const int mine = min(each, n - (int)rank * each);
-  for (int i = (int)threadIdx.x - first; i < mine * 128; i += threads) {
-    const int col = i >> 7, l = i & 127;
-    float v = 0.f;
-    for (int p = 0; p < parts; ++p) v += inbox[(p * each + col) * 128 + l];
-    if (l < lanes) dst[((long long)rank * each + col) * ldo + l] = pcl_group::to_out<TO>(v);
+  for (int i = (int)threadIdx.x - first; i < (mine + 3) / 4 * 128; i += threads) {
+    const int col = i >> 7 << 2, l = i & 127;
+    float v[4] = {};
+    for (int p = 0; p < parts; ++p) {
+      const float4 u = *reinterpret_cast<const float4*>(inbox + (p * each + col) * 128 + l * 4);
+      v[0] += u.x;
+      v[1] += u.y;
+      v[2] += u.z;
+      v[3] += u.w;
+    }
+    if (l < lanes) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < mine) dst[((long long)rank * each + col + j) * ldo + l] = pcl_group::to_out<TO>(v[j]);
+    }
   }
 }
 
@@ -396,11 +407,15 @@ static inline long long likely_chunks(long long rows, int groups, int cols) {
   return taken <= 1 ? all : (taken > all + taken / 2 ? taken : all + taken / 2);
 }
 
-// Parts that a tile's reduction of `steps` stages is cut into where `tiles` of them leave more than half the SMs idle: as many as fill these, at most
+// Clusters of 1 to 8 CTAs that run at the same time, one CTA to an SM, as the runtime counts them: they do not straddle the processor's parts of some 16 SMs,
+// and one more runs alone behind the others (16 clusters of 8: 19.2 us where 8 took 10.2).
+constexpr int CLUSTERS[] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+
+// Parts that a tile's reduction of `steps` stages is cut into: as many as `tiles` clusters that run at the same time can have, at most
 // eight (the largest portable cluster), and two stages at least for each.  1: not cut.
 static inline int parts_of(long long tiles, int steps) {
-  int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= SMS && steps >= max(8, parts * 4)) parts *= 2;
+  int parts = steps < 8 ? 1 : steps < 16 ? steps / 2 : 8;
+  while (parts > 1 && tiles > CLUSTERS[parts]) --parts;
   return parts;
 }
 

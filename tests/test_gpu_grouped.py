@@ -80,6 +80,9 @@ SHAPES = [
     ([700, 0, 1300, 33, 256], 5, 4008, 3800), ([257, 15, 1000, 0, 500, 470, 60], 0, 3777, 4001),
     # tn by pairs with columns in whole blocks of 64, an odd number of them
     ([30, 0, 65, 64, 1] * 20, 0, 320, 256), ([200, 7] * 40, 3, 64, 640), ([63, 65, 128, 0] * 16, 0, 448, 320),
+    # tn by clusters: groups without rows for some of the CTAs, or for any; ends of every kind; 64 columns and 128
+    ([1500, 0, 3, 70], 9, 96, 200), ([2000], 0, 1, 9), ([0, 4000, 65], 0, 72, 520), ([3000, 5000, 129], 2, 200, 328),
+    ([9001], 1, 777, 1030), ([8192, 0], 0, 512, 512), ([700, 1400, 0, 31], 0, 1144, 128), ([20000], 0, 67, 65),
 ]
 
 
