@@ -172,13 +172,14 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   const int share = SPLIT ? (int)cluster_size() : CG;
   const int group = blockIdx.x / share, groups = gridDim.x / share;
   const Walk<MODE, CG, COLS, SPLIT> walk(a, s.table);
+  using Turn = Tiles<Walk<MODE, CG, COLS, SPLIT>, SPLIT>;
   bool ok = true;
 
   if (warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
-    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
-      const Tile w = walk.at(i);
+    for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
+      const Tile w = i.tile();
       const int steps = (w.r1 - w.r0 + BR - 1) / BR;
       const int mine = w.ncol / CG;
       const int j = w.j0 + (int)me * mine;
@@ -255,8 +256,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;   // bit i of acc_phase: accumulator i
       bool ready = false;                  // the next stage has arrived
-      for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
-        const Tile w = walk.at(i);
+      for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
+        const Tile w = i.tile();
         const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
         if (len <= 0) continue;
         if (!mbar_wait(s.tempty + acc, (acc_phase >> acc & 1u) ^ 1u, abort_flag)) {
@@ -299,8 +300,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   } else if (MODE == TN && warp == FIX_WARP) {
     int stage = 0;
     uint32_t phases = 0;   // bit i: parity of the next wait on tail[i]
-    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
-      const Tile w = walk.at(i);
+    for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
+      const Tile w = i.tile();
       const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
       const int last = (stage + steps + STAGES - 1) % STAGES;
       stage = (stage + steps) % STAGES;
@@ -329,8 +330,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     TO* out = static_cast<TO*>(a.out);
     int acc = 0;
     uint32_t acc_phase = 0;                   // bit i: accumulator i
-    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
-      const Tile w = walk.at(i);
+    for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
+      const Tile w = i.tile();
       const int m = w.m0 + (int)me * LANES + sub * 32;
       TO* dst = out + (MODE == TN ? ((long long)w.e * a.jdim + w.j0) * a.ldo : (long long)w.j0 * a.ldo) + m;
       if (SPLIT && w.r1 <= w.r0) {   // no rows for this part

@@ -497,6 +497,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   const int share = SPLIT ? (int)cluster_size() : 1;
   const int group = blockIdx.x / share, groups = gridDim.x / share;
   const Walk<SPLIT> walk(a, s.table);
+  using Turn = Tiles<Walk<SPLIT>, SPLIT || FUSED>;
   bool ok = true;
   auto gave_up = [&](int where, int x, int y) {
     if (lane == 0) report(&g_status, 0, where, x, y);
@@ -514,8 +515,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     after_previous();   // A may still be being quantised
     int stage = 0;
     uint32_t phase = 0;
-    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
-      const Tile w = walk.at(i);
+    for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
+      const Tile w = i.tile();
       constexpr int SMALL_BOX = F::SMALL_BOX;
       const bool whole = w.ncol > 3 * SMALL_BOX;
       const int boxes = whole ? 1 : (w.ncol + SMALL_BOX - 1) / SMALL_BOX;
@@ -548,8 +549,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;   // bit i of acc_phase: accumulator i
     bool ready = false;                  // the next stage has arrived
-    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
-      const Tile w = walk.at(i);
+    for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
+      const Tile w = i.tile();
       if (!mbar_wait(s.tempty + acc, (acc_phase >> acc & 1u) ^ 1u, abort_flag)) { gave_up(42, acc, 0); break; }
       acc_phase ^= 1u << acc;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -602,8 +603,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     const int last_bytes = 4 - (a.words * 4 - a.blocks);   // codes of the last word; those that no block has become zero
     int stage = 0;
     uint32_t phase = 0;
-    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
-      const Tile w = walk.at(i);
+    for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
+      const Tile w = i.tile();
       const bool used = part < 2 || w.ncol > 128;
       const long long r0 = part == 0 ? (long long)w.e * a.N + w.m0 : (long long)w.j0 + (part - 1) * 128;
       const uint8_t* at[4];
@@ -634,8 +635,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     TO* out = static_cast<TO*>(a.out);
     int acc = 0;
     uint32_t acc_phase = 0;                   // bit i: accumulator i
-    for (Counter i = walk.start(group, groups); walk.has(i) && ok; i.next()) {
-      const Tile w = walk.at(i);
+    for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
+      const Tile w = i.tile();
       if (!wait_full(s.tfull + acc, acc_phase >> acc & 1u, abort_flag, tile_ns(w.k1 - w.k0))) { gave_up(44, acc, 0); break; }
       acc_phase ^= 1u << acc;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
