@@ -324,8 +324,9 @@ __device__ __forceinline__ void store_singly(uint32_t taddr, int n, TO* dst, lon
 
 // A warp's part of an accumulator goes to out: column j of [0, n) and the warp's 32 lanes to dst[j * ldo + lane], lanes < `lanes` only.  Columns 32 at a time,
 // first + 0, 64, 128 ..  16-bit results turn around in shared memory (stmatrix) and leave as boxes of 32 rows
-// x 64 bytes, where `boxed` says that the map can take them; what is left of a chunk, and 32-bit results, are stored lane by lane, a row's 32 neighbours at a
-// time (stored so throughout, nt of 16 groups of 1024 rows, 2048 x 1024 took 81 instead of 68 us).
+// x 64 bytes, where `boxed` says that the map can take them; what is left of a chunk, and rows that begin anywhere, are stored lane by lane, a row's 32
+// neighbours at a time (stored so throughout, nt of 16 groups of 1024 rows, 2048 x 1024 took 81 instead of 68 us: a store of one row takes an SM 11 cycles, of
+// 64 bytes or of 128).
 template <class TO>
 __device__ __forceinline__ void store_columns(uint32_t taddr, int first, int n, TO* dst, long long ldo, int lanes, bool boxed, uint8_t* piece,
                                               const CUtensorMap* map, int x, int y, int z) {
@@ -367,10 +368,35 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, int first, int n, 
     __syncwarp();
   }
 }
+// 32 bits a value: sixteen columns at a time go through shared memory, and leave as four rows a store where these begin at multiples of 16 bytes (four-bit product
+// of 16384 rows of 32 groups, 4096 x 256: 101 us by single rows, 59 so; tn of 1537 rows of 11 groups, 1001 x 776: 26 and 18)
 template <>
-__device__ __forceinline__ void store_columns<float>(uint32_t taddr, int first, int n, float* dst, long long ldo, int lanes, bool, uint8_t*,
+__device__ __forceinline__ void store_columns<float>(uint32_t taddr, int first, int n, float* dst, long long ldo, int lanes, bool, uint8_t* piece,
                                                      const CUtensorMap*, int, int, int) {
-  for (int c = first; c < n; c += 64) store_singly(taddr + (uint32_t)c, min(32, n - c), dst + (long long)c * ldo, ldo, lanes);
+  const int lane = threadIdx.x & 31;
+  const bool quads = lanes >= 32 && (((uintptr_t)dst | (uintptr_t)ldo * 4) & 15) == 0;
+  for (int c0 = first; c0 < n; c0 += 64) {
+#pragma unroll 1
+    for (int c = c0; c < min(c0 + 32, n); c += 16) {
+      float* to = dst + (long long)c * ldo;
+      if (quads && c + 16 <= n) {
+        uint32_t v[16];
+        tmem_ld8(taddr + (uint32_t)c, v);
+        tmem_ld8(taddr + (uint32_t)c + 8, v + 8);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) *reinterpret_cast<uint32_t*>(piece + j * 128 + lane * 4) = v[j];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * i + (lane >> 3);
+          *reinterpret_cast<uint4*>(to + j * ldo + (lane & 7) * 4) = *reinterpret_cast<const uint4*>(piece + j * 128 + (lane & 7) * 16);
+        }
+        __syncwarp();
+      } else {
+        store_singly(taddr + (uint32_t)c, min(16, n - c), to, ldo, lanes);
+      }
+    }
+  }
 }
 
 // ---- one tile by a cluster: every CTA has a part of the reduction, and adds up the parts of some of the columns

@@ -439,3 +439,20 @@ def test_operands_are_copied_to_whole_rows(mats, rows, cols, step, extra, start)
         assert torch.equal(dst[..., :cols], src) and not dst[..., cols:].any()
         assert bool((room[:8] == 77).all()) and bool((room[-8:] == 77).all())
         assert torch.equal(second[:, :5], other) == both and bool((second[:, 5:] == (0 if both else 77)).all())
+
+
+@pytest.mark.parametrize("N,K,left", [(64, 128, 0), (200, 132, 1), (72, 260, 4), (130, 96, 8), (16, 33, 0), (256, 512, 3)])
+def test_results_of_32_bits_in_strided_rows(N, K, left):
+    """Rows at multiples of 16 bytes and elsewhere, m that ends inside a store, column counts that are no multiple of 16."""
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt
+    counts = [17, 0, 70, 300, 1]
+    T = sum(counts)
+    X, dY, W = _whole(T, 5, N, K, BF)
+    off = _offsets(counts)
+    for call, A, M, cols in ((grouped_nt, X, W, N), (grouped_nn, dY, W.transpose(1, 2), K)):
+        for room in (left + cols, left + cols + 4, left + (cols + 7) // 4 * 4):
+            wide = torch.full((T, room), 5.0, device="cuda")
+            call(A, W, off, out=wide[:, left:left + cols])
+            ref = torch.full((T, room), 5.0, device="cuda", dtype=torch.float64)
+            ref[:, left:left + cols] = _ref_rows(A, M, off)[0]
+            assert torch.equal(wide.double(), ref)
