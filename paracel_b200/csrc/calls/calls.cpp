@@ -21,7 +21,7 @@ using Rows = int (*)(int, int, int, const void*, long long, const void*, long lo
 using Tn = int (*)(int, int, const void*, long long, const void*, long long, const void*, int, void*, long long, int, int, int,
                    cudaStream_t);
 using PadFn = int (*)(const void*, long long, long long, long long, long long, int, void*, const void*, long long, long long, long long, long long, int,
-                      void*, cudaStream_t);
+                      void*, const void*, int, cudaStream_t);
 using Quantize = int (*)(const void*, long long, int, void*, void*, long long, int, cudaStream_t);
 using Dequantize = int (*)(const void*, const void*, void*, long long, int, long long, int, cudaStream_t);
 using Mx4Rows = int (*)(const void*, long long, int, void*, void*, const void*, const void*, const void*, int, void*, long long, int, long long,
@@ -95,16 +95,14 @@ at::Tensor room_for(const Operand& a, const Operand& b, const at::TensorOptions&
   return a.copy || b.copy ? at::empty({a.bytes() + b.bytes()}, options.dtype(at::kByte)) : at::Tensor();
 }
 
-// Copies it there, and points the operands to it
-int copy_operands(Operand& a, Operand& b, const at::Tensor& room, cudaStream_t stream) {
+// Copies it there, and points the operands to it; `offsets`: b has a matrix for each group of them
+int copy_operands(Operand& a, Operand& b, const at::Tensor& room, const at::Tensor* offsets, cudaStream_t stream) {
   if (!a.copy && !b.copy) return 0;
   char* to = static_cast<char*>(room.data_ptr());
   const Operand na = a.copied(to), nb = b.copied(to + a.bytes());
-  const Operand& x = a.copy ? a : b;
-  void* dst = const_cast<void*>((a.copy ? na : nb).at);
-  const bool both = a.copy && b.copy;
-  const int rc = pad_fn(x.at, x.step_e, x.step, x.mats, x.rows, (int)x.cols, dst, both ? b.at : nullptr, b.step_e, b.step, b.mats, b.rows, (int)b.cols,
-                        both ? const_cast<void*>(nb.at) : nullptr, stream);
+  const int rc = pad_fn(a.copy ? a.at : nullptr, a.step_e, a.step, a.mats, a.rows, (int)a.cols, const_cast<void*>(na.at), b.copy ? b.at : nullptr, b.step_e,
+                        b.step, b.mats, b.rows, (int)b.cols, const_cast<void*>(nb.at), offsets ? offsets->data_ptr() : nullptr,
+                        offsets && offsets->scalar_type() == at::kLong, stream);
   a = na;
   b = nb;
   return rc;
@@ -165,7 +163,7 @@ PyObject* grouped_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
   const at::Tensor room = room_for(x, w, X.options());
   return launched("pcl_grouped_rows", [&] {
-    const int rc = copy_operands(x, w, room, stream);
+    const int rc = copy_operands(x, w, room, &offsets, stream);
     return rc ? rc : rows_fn((int)mode, in, type_of(out_type), x.at, x.step, w.at, w.step_e, w.step, offsets.data_ptr(),
                              offsets.scalar_type() == at::kLong, out.data_ptr(), cols, T, (int)E, (int)N, (int)K, 1, stream);
   }, out);
@@ -193,7 +191,7 @@ PyObject* grouped_tn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
   const at::Tensor room = room_for(x, y, X.options());
   return launched("pcl_grouped_tn", [&] {
-    const int rc = copy_operands(x, y, room, stream);
+    const int rc = copy_operands(x, y, room, nullptr, stream);
     return rc ? rc : tn_fn(in, type_of(out_type), y.at, y.step, x.at, x.step, offsets.data_ptr(), offsets.scalar_type() == at::kLong, out.data_ptr(), T,
                            (int)E, (int)N, (int)K, stream);
   }, out);

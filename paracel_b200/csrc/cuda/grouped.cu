@@ -488,91 +488,120 @@ bool sizes_ok(int in_type, long long rows, int groups, int N, int K) {
 // ---- operands whose rows do not start at multiples of 16 bytes ----
 //
 // The tensor copies cannot read these, so a call copies them first, both of a product in one launch: rows of any distance to rows of whole 16 bytes, the last one
-// filled up with zeros.  A thread has a chunk of 16 bytes of up to PAD_CHUNKS places of a row, and reads it in the largest units that the rows' starts share
-// (WIDTH values: an odd number of columns leaves two bytes).  Bound by the launch for small operands, by memory for large ones.
-constexpr int PAD_THREADS = 256, PAD_CHUNKS = 4;
+// filled up with zeros.  Matrices of groups without rows are left out.  A block has some 1024 chunks of 16 bytes, of as many rows as these make or of a part of one;
+// a thread has four.  Bound by the launch for small operands, by memory for large ones:
+// 16384 x 1023 takes 18 us, 32768 x 2047 57 us, 4.7 TB/s (a general copy of strided rows 39 and 147 us).
+constexpr int PAD_THREADS = 256, PAD_EACH = 4, PAD_CHUNKS = PAD_THREADS * PAD_EACH;
 
 struct Pad {
   const uint16_t* src;
   uint4* dst;
-  long long step_e, step, rows, per;   // `per` rows of a matrix
-  int cols, shift, col_blocks, width;  // 2^shift threads to a row
+  long long step_e, step, rows;
+  unsigned per;                          // rows of a matrix
+  int cols, in_block, col_blocks;        // rows of a block, blocks of a row
+  bool eights;                           // rows begin at multiples of eight bytes
   long long blocks;
 };
 
-template <class U>
-__device__ __forceinline__ uint4 load_chunk(const uint16_t* src) {
-  constexpr int N = 16 / sizeof(U);
-  U v[N];
+// 16 bytes from any even address, out of the one or two aligned words of 16 bytes that they lie in (either holds a byte of them, so both can be read); or from a multiple
+// of eight
+__device__ __forceinline__ uint4 load_chunk(const uint16_t* src, bool eights) {
+  if (eights) {
+    const uint2 a = reinterpret_cast<const uint2*>(src)[0], b = reinterpret_cast<const uint2*>(src)[1];
+    return make_uint4(a.x, a.y, b.x, b.y);
+  }
+  const uint4* at = reinterpret_cast<const uint4*>((uintptr_t)src & ~(uintptr_t)15);
+  const uint32_t off = (uint32_t)(uintptr_t)src & 15u;
+  const uint4 lo = at[0], hi = off ? at[1] : lo;
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  if (off & 8)
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const U*>(src)[i];
-  uint4 r;
-  memcpy(&r, v, 16);
-  return r;
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  if (off & 4)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  const uint32_t bits = (off & 2) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                    __funnelshift_r(w[3], w[4], bits));
 }
 
-__global__ void __launch_bounds__(PAD_THREADS) pad_kernel(const __grid_constant__ Pad first, const __grid_constant__ Pad second) {
+// off: null, or the bounds of the groups that have the matrices of `second`
+__global__ void __launch_bounds__(PAD_THREADS) pad_kernel(const __grid_constant__ Pad first, const __grid_constant__ Pad second, const void* off, int off64) {
   after_previous();
   let_next_begin();
   const bool other = blockIdx.x >= first.blocks;
   const Pad& p = other ? second : first;
   const unsigned b = blockIdx.x - (other ? (unsigned)first.blocks : 0u);
   const unsigned row_block = b / (unsigned)p.col_blocks, col_block = b - row_block * p.col_blocks;
-  const long long r = (long long)row_block * (PAD_THREADS >> p.shift) + (threadIdx.x >> p.shift);
-  if (r >= p.rows) return;
-  const int chunks = (p.cols + 7) >> 3, lanes = 1 << p.shift;
-  const int c0 = (int)col_block * (lanes * PAD_CHUNKS) + ((int)threadIdx.x & (lanes - 1));
-  const long long e = p.per == p.rows ? 0 : r / p.per;
-  const uint16_t* src = p.src + e * p.step_e + (r - e * p.per) * p.step;
-  uint4 v[PAD_CHUNKS];
+  const int chunks = (p.cols + 7) >> 3, c0 = (int)col_block * PAD_CHUNKS, across = min(chunks - c0, PAD_CHUNKS);
+  const long long r0 = (long long)row_block * p.in_block;
+  const int rows = (int)min((long long)p.in_block, p.rows - r0);
+  const long long e0 = p.per == p.rows ? 0 : r0 / p.per;
+  const unsigned first_row = (unsigned)(r0 - e0 * p.per);
+  const float inverse = 1.f / (float)across;
+  uint4 v[PAD_EACH];
+  bool there[PAD_EACH];
+  long long to[PAD_EACH];
 #pragma unroll
-  for (int i = 0; i < PAD_CHUNKS; ++i) {
-    const int c = c0 + i * lanes;
+  for (int i = 0; i < PAD_EACH; ++i) {
+    const int at = (int)threadIdx.x + i * PAD_THREADS;
+    const int r = (int)(((float)at + 0.5f) * inverse);   // at / across: below 2^10 a half is further from a whole number than the product is wrong
+    const int c = c0 + at - r * across;
+    there[i] = r < rows;
     v[i] = make_uint4(0, 0, 0, 0);
-    if (c * 8ll + 8 <= p.cols) {
-      const uint16_t* at = src + c * 8ll;
-      v[i] = p.width == 4 ? load_chunk<uint2>(at) : p.width == 2 ? load_chunk<uint32_t>(at) : load_chunk<uint16_t>(at);
-    } else if (c < chunks) {
+    if (!there[i]) continue;
+    const unsigned row = first_row + (unsigned)r, more = p.per == p.rows ? 0 : row / p.per;
+    const long long e = e0 + more;
+    if (other && off != nullptr) {
+      const long long begin = off64 ? static_cast<const long long*>(off)[e] : static_cast<const int*>(off)[e];
+      const long long end = off64 ? static_cast<const long long*>(off)[e + 1] : static_cast<const int*>(off)[e + 1];
+      there[i] = end > begin;   // (a group whose end is moved up has the rows of none)
+      if (!there[i]) continue;
+    }
+    const uint16_t* src = p.src + e * p.step_e + (long long)(row - more * p.per) * p.step + c * 8ll;
+    to[i] = (r0 + r) * chunks + c;
+    const int left = p.cols - c * 8;
+    if (left >= 8) {
+      v[i] = load_chunk(src, p.eights);
+    } else {
       uint16_t t[8] = {};
-      const int left = p.cols - c * 8;
 #pragma unroll
       for (int j = 0; j < 7; ++j)
-        if (j < left) t[j] = src[c * 8ll + j];
+        if (j < left) t[j] = src[j];
       memcpy(&v[i], t, 16);
     }
   }
 #pragma unroll
-  for (int i = 0; i < PAD_CHUNKS; ++i)
-    if (c0 + i * lanes < chunks) p.dst[r * chunks + c0 + i * lanes] = v[i];
+  for (int i = 0; i < PAD_EACH; ++i)
+    if (there[i]) p.dst[to[i]] = v[i];
 }
 
 // matrices [mats, rows, cols] of 16-bit values, the columns contiguous
 bool pad_of(Pad* p, const void* src, long long step_e, long long step, long long mats, long long rows, long long cols, void* dst) {
-  if (mats < 1 || rows < 1 || cols < 1 || cols >= (1 << 30) || ((uintptr_t)src & 1) || ((uintptr_t)dst & 15)) return false;
-  *p = Pad{static_cast<const uint16_t*>(src), static_cast<uint4*>(dst), step_e, step, mats * rows, rows, (int)cols, 0, 1, 1, 0};
-  if (step_e == rows * step) p->per = p->rows;
-  const unsigned long long bits = (uintptr_t)src / 2 | (unsigned long long)(p->per == p->rows ? 0 : step_e) | (unsigned long long)step;
-  p->width = bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
-  const long long chunks = (cols + 7) / 8;
-  while (p->shift < 5 && (1ll << p->shift) < chunks) ++p->shift;
-  const long long place = (long long)PAD_CHUNKS << p->shift;
-  p->col_blocks = (int)((chunks + place - 1) / place);
-  const long long per_block = PAD_THREADS >> p->shift;
-  p->blocks = (p->rows + per_block - 1) / per_block * p->col_blocks;
+  if (mats < 1 || rows < 1 || rows >= (1ll << 31) - 512 || cols < 1 || cols >= (1 << 30) || ((uintptr_t)src & 1) || ((uintptr_t)dst & 15)) return false;
+  *p = Pad{static_cast<const uint16_t*>(src), static_cast<uint4*>(dst), step_e, step, mats * rows, (unsigned)rows, (int)cols, 1, 1, false, 0};
+  p->eights = (((uintptr_t)src | (unsigned long long)(mats == 1 ? 0 : step_e) * 2 | (unsigned long long)(rows == 1 ? 0 : step) * 2) & 7) == 0;
+  const int chunks = (int)((cols + 7) / 8);
+  p->in_block = chunks < PAD_CHUNKS ? PAD_CHUNKS / chunks : 1;
+  p->col_blocks = (chunks + PAD_CHUNKS - 1) / PAD_CHUNKS;
+  p->blocks = (p->rows + p->in_block - 1) / p->in_block * p->col_blocks;
   return p->blocks < (1ll << 30);
 }
 
 }  // namespace
 
 // Copies of one or two operands [mats, rows, cols] of 16-bit values, matrices step_e and rows step values apart, the columns contiguous: dst has
-// mats * rows rows of ceil(cols / 8) * 8 values.  second may be null.
+// mats * rows rows of ceil(cols / 8) * 8 values.  first or second may be null; offsets, where given, are the bounds of mats2 groups, and matrices of groups without rows are
+// not copied.
 PCL_API int pcl_grouped_pad(const void* first, long long step_e, long long step, long long mats, long long rows, int cols, void* dst, const void* second,
-                            long long step_e2, long long step2, long long mats2, long long rows2, int cols2, void* dst2, cudaStream_t stream) {
+                            long long step_e2, long long step2, long long mats2, long long rows2, int cols2, void* dst2, const void* offsets, int off64,
+                            cudaStream_t stream) {
   Pad a{}, b{};
-  if (!pad_of(&a, first, step_e, step, mats, rows, cols, dst)) return (int)cudaErrorInvalidValue;
+  if (first != nullptr && !pad_of(&a, first, step_e, step, mats, rows, cols, dst)) return (int)cudaErrorInvalidValue;
   if (second != nullptr && !pad_of(&b, second, step_e2, step2, mats2, rows2, cols2, dst2)) return (int)cudaErrorInvalidValue;
+  if (a.blocks + b.blocks == 0) return (int)cudaErrorInvalidValue;
   Launch l((unsigned)(a.blocks + b.blocks), PAD_THREADS, 0, 1, stream);
-  return (int)cudaLaunchKernelEx(&l.cfg, pad_kernel, a, b);
+  return (int)cudaLaunchKernelEx(&l.cfg, pad_kernel, a, b, offsets, off64);
 }
 
 // mode 0: X [rows, K] -> out [rows, N]; mode 1: X [rows, N] -> out [rows, K].  W [groups, N, K] with strides (ws_e, ws_n, 1); rows of X and W

@@ -77,7 +77,7 @@ SIGS = {
     "pcl_ssp_wait": "piqQpip",
     "pcl_grouped_rows": "iiipqpqqpipqqiiiip",
     "pcl_grouped_tn": "iipqpqpipqiiip",
-    "pcl_grouped_pad": "pqqqqippqqqqipp",
+    "pcl_grouped_pad": "pqqqqippqqqqippip",
     "pcl_grouped_status": "pp",
     "pcl_mx4_quantize": "pqippqip",
     "pcl_mx4_dequantize": "pppqiqip",

@@ -112,7 +112,7 @@ def aligned(x: torch.Tensor) -> torch.Tensor:
     step = stride_of(x, -2, pitch)
     step_e = stride_of(x, 0, rows * step) if mats else rows * step
     _lib.call_on(x.get_device(), "pcl_grouped_pad", x.data_ptr(), step_e, step, mats[0] if mats else 1, rows, cols, buf.data_ptr(),
-                 0, 0, 0, 0, 0, 0, 0)
+                 0, 0, 0, 0, 0, 0, 0, 0, 0)
     return buf[..., :cols]
 
 

@@ -434,7 +434,7 @@ def test_operands_are_copied_to_whole_rows(mats, rows, cols, step, extra, start)
     for both in (False, True):
         room = torch.full((8 + mats * rows * pitch + 8,), 77, dtype=torch.int16, device="cuda")
         dst = room[8:-8].view(mats, rows, pitch)
-        tail = (other.data_ptr(), 95, 5, 1, 19, 5, second.data_ptr()) if both else (0,) * 7
+        tail = (other.data_ptr(), 95, 5, 1, 19, 5, second.data_ptr(), 0, 0) if both else (0,) * 9
         _lib.call_on(0, "pcl_grouped_pad", src.data_ptr(), step_e, step, mats, rows, cols, dst.data_ptr(), *tail)
         assert torch.equal(dst[..., :cols], src) and not dst[..., cols:].any()
         assert bool((room[:8] == 77).all()) and bool((room[-8:] == 77).all())
@@ -456,3 +456,28 @@ def test_results_of_32_bits_in_strided_rows(N, K, left):
             ref = torch.full((T, room), 5.0, device="cuda", dtype=torch.float64)
             ref[:, left:left + cols] = _ref_rows(A, M, off)[0]
             assert torch.equal(wide.double(), ref)
+
+
+@pytest.mark.parametrize("bounds,dtype", [([0, 0, 3, 3, 40], torch.int32), ([5, 4, 9, 9, 2], torch.int64), ([0, 1, 2, 3, 4], torch.int64), ([7, 7, 7, 7, 7], torch.int32),
+                                          ([-3, 2, -1, 50, 60], torch.int32)])
+def test_only_matrices_of_groups_with_rows_are_copied(bounds, dtype):
+    """What a call does not copy it does not read: the memory of a copy is whatever was there before."""
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt
+    N, K, T = 45, 37, 40
+    X, dY, W = _whole(T, 4, N, K, BF)
+    off = torch.tensor(bounds, dtype=dtype, device="cuda")
+    fixed, top = [], 0
+    for v in bounds:
+        top = max(top, min(max(v, 0), T))
+        fixed.append(top)
+    good = torch.tensor(fixed, dtype=dtype, device="cuda")
+    f = torch.float32
+    for _ in range(3):
+        spoiled = [torch.full((4 * N * 48,), float("nan"), dtype=BF, device="cuda") for _ in range(4)]
+        del spoiled
+        assert torch.equal(grouped_nt(X, W, off, out_dtype=f).double(), _ref_rows(X, W, good)[0])
+        assert torch.equal(grouped_nn(dY, W, off, out_dtype=f).double(), _ref_rows(dY, W.transpose(1, 2), good)[0])
+    try:
+        check_status()
+    except Exception:
+        assert bounds != fixed
