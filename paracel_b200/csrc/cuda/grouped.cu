@@ -339,8 +339,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         continue;
       }
       if (w.r1 <= w.r0) {   // a group without rows: its matrix of sums is zero
-        if (m + lane < a.mdim)
-          for (int j = half; j < w.n; j += 2) dst[(long long)j * a.ldo + lane] = to_out<TO>(0.f);
+        // the tile's rows have no gaps: every m block takes a part of them all
+        zero_part(out + ((long long)w.e * a.jdim + w.j0) * a.ldo, (long long)w.n * a.ldo, w.m0 / LANES + (int)me, walk.mb * CG, (int)threadIdx.x - 64, 32 * EPI_WARPS);
         continue;
       }
       if (!wait_full(s.tfull + acc, acc_phase >> acc & 1u, abort_flag, tile_ns((w.r1 - w.r0) / BR))) {

@@ -481,3 +481,19 @@ def test_only_matrices_of_groups_with_rows_are_copied(bounds, dtype):
         check_status()
     except Exception:
         assert bounds != fixed
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("E,N,K,shift", [(3, 1, 1, 0), (40, 300, 7, 1), (9, 257, 129, 3), (600, 256, 640, 2), (300, 513, 258, 5), (5, 64, 1000, 0)])
+def test_gradients_of_groups_without_rows_are_zero(E, N, K, shift, dtype):
+    """Every value of the result is written, and none outside, wherever it begins."""
+    from paracel_b200.ops.grouped import grouped_tn
+    counts = [0] * E
+    counts[E // 2] = 5
+    X, dY, _ = _whole(5, 1, N, K, BF)
+    off = _offsets(counts)
+    flat = torch.full((E * N * K + 16,), 7.0, device="cuda", dtype=dtype)
+    out = flat[shift:shift + E * N * K].view(E, N, K)
+    grouped_tn(dY, X, off, out=out)
+    assert torch.equal(out.double(), _ref_tn(dY, X, off)[0].to(dtype).double())
+    assert bool((flat[:shift] == 7).all()) and bool((flat[shift + E * N * K:] == 7).all())
