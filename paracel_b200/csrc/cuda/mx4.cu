@@ -691,8 +691,8 @@ int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, co
   if (e != cudaSuccess) return (int)e;
   const long long mb = (a.N + LANES - 1) / LANES;
   const long long chunks = most_chunks(a.off.rows, a.off.groups, COLS);
-  // a cluster that shares a tile has no other
-  const unsigned grid = SPLIT ? (unsigned)(chunks * mb) * parts : (unsigned)min((long long)sms, chunks * mb);
+  // a cluster that shares a tile has no other, nor has a CTA that quantises its rows
+  const unsigned grid = SPLIT ? (unsigned)(chunks * mb) * parts : FUSED ? (unsigned)(chunks * mb) : (unsigned)min((long long)sms, chunks * mb);
   const Launch l(grid, THREADS, smem, parts, stream);
   e = cudaLaunchKernelEx(&l.cfg, kernel, p, q, qs, o, a);
   return e != cudaSuccess ? (int)e : pcl_last_error();

@@ -109,6 +109,9 @@ def aligned(x: torch.Tensor) -> torch.Tensor:
     *mats, rows, cols = x.shape
     pitch = (cols + 7) // 8 * 8
     buf = torch.empty(*mats, rows, pitch, dtype=x.dtype, device=x.device)
+    if not x.is_cuda:
+        buf[..., :cols] = x
+        return buf[..., :cols]
     step = stride_of(x, -2, pitch)
     step_e = stride_of(x, 0, rows * step) if mats else rows * step
     _lib.call_on(x.get_device(), "pcl_grouped_pad", x.data_ptr(), step_e, step, mats[0] if mats else 1, rows, cols, buf.data_ptr(),
