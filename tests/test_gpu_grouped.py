@@ -497,3 +497,41 @@ def test_gradients_of_groups_without_rows_are_zero(E, N, K, shift, dtype):
     grouped_tn(dY, X, off, out=out)
     assert torch.equal(out.double(), _ref_tn(dY, X, off)[0].to(dtype).double())
     assert bool((flat[:shift] == 7).all()) and bool((flat[shift + E * N * K:] == 7).all())
+
+
+def test_odd_widths_into_given_results_on_a_stream_and_in_a_graph():
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    counts, N, K = [33, 0, 100, 7], 45, 77
+    T, E = sum(counts), 4
+    X, dY, W = _whole(T, E, N, K, BF)
+    off = _offsets(counts)
+    f = torch.float32
+    y, z, d = torch.empty(T, N, device="cuda"), torch.empty(T, K, device="cuda"), torch.empty(E, N, K, device="cuda")
+
+    def calls():
+        grouped_nt(X, W, off, out=y)
+        grouped_nn(dY, W, off, out=z)
+        grouped_tn(dY, X, off, out=d)
+        return grouped_nt(X, W, off, out_dtype=f), grouped_nn(dY, W, off, out_dtype=f), grouped_tn(dY, X, off, out_dtype=f)
+
+    def right(made):
+        for got, want in ((y, _ref_rows(X, W, off)[0]), (z, _ref_rows(dY, W.transpose(1, 2), off)[0]), (d, _ref_tn(dY, X, off)[0])):
+            assert torch.equal(got.double(), want)
+        for got, same in zip(made, (y, z, d)):
+            assert torch.equal(got, same)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        made = calls()
+    torch.cuda.current_stream().wait_stream(side)
+    right(made)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made = calls()
+    for seed in (2, 3):
+        for t, new in zip((X, dY, W), _whole(T, E, N, K, BF, seed=seed)):
+            t.copy_(new)
+        off.copy_(_offsets([7, 100, 0, 33] if seed == 2 else [0, 0, 140, 0]))
+        graph.replay()
+        right(made)
