@@ -47,7 +47,11 @@ template <int CG, int COLS, bool SPLIT>
 struct Form {
   static constexpr int Q_BYTES = COLS / CG * BR * 2;
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
-  static constexpr int STAGES = (OPERAND_BYTES - (SPLIT ? inbox_bytes(COLS) : 0)) / STAGE_BYTES;
+  // A cluster's 128 columns: the parts are sent to where the operands were, behind a barrier of the cluster more; three stages beside them left the loads waiting
+  // (one group of 131072 rows, 512 x 512: 135 and 113 us)
+  static constexpr bool AFTER = SPLIT && COLS == 128;
+  static constexpr int STAGES = (OPERAND_BYTES - (SPLIT && !AFTER ? inbox_bytes(COLS) : 0)) / STAGE_BYTES;
+  static_assert(!AFTER || inbox_bytes(COLS) <= OPERAND_BYTES, "room for the parts");
   static constexpr int M = LANES * CG;   // m of a tile
   // Rows of Q that a load brings: all that fit, or a quarter of them, up to three times.  A load takes the warp that issues it 135 cycles, and the products of a
   // stage 512 at most: four or five loads to a stage were what bound a call.
@@ -142,7 +146,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* pieces = stages + OPERAND_BYTES;
   Shared& s = *reinterpret_cast<Shared*>(pieces + EPI_WARPS * PIECE_BYTES);
-  float* inbox = reinterpret_cast<float*>(stages + STAGES * STAGE_BYTES);   // SPLIT
+  float* inbox = reinterpret_cast<float*>(stages + (F::AFTER ? 0 : STAGES * STAGE_BYTES));   // SPLIT
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t me = CG == 2 ? cluster_ctarank() : 0;   // 0 leads the pair
   volatile int* abort_flag = &s.abort_flag;
@@ -331,11 +335,14 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     TO* out = static_cast<TO*>(a.out);
     int acc = 0;
     uint32_t acc_phase = 0;                   // bit i: accumulator i
+    bool free = false;                        // AFTER: no CTA of the cluster reads its operands any more
     for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
       const Tile w = i.tile();
       const int m = w.m0 + (int)me * LANES + sub * 32;
       TO* dst = out + (MODE == TN ? ((long long)w.e * a.jdim + w.j0) * a.ldo : (long long)w.j0 * a.ldo) + m;
       if (SPLIT && w.r1 <= w.r0) {   // no rows for this part
+        if (F::AFTER) cluster_sync_all();
+        free = true;
         send_columns(0, sub, half * 32, w.n, inbox, cluster_ctarank(), columns_of_part(w.n, share), true);
         continue;
       }
@@ -354,6 +361,9 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * COLS);
       if (SPLIT) {   // the cluster has this one tile
+        __syncwarp();
+        if (F::AFTER) cluster_sync_all();
+        free = true;
         send_columns(t0, sub, half * 32, w.n, inbox, cluster_ctarank(), columns_of_part(w.n, share));
         continue;
       }
@@ -363,6 +373,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
       acc ^= 1;
     }
+    __syncwarp();
+    if (F::AFTER && !free) cluster_sync_all();
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the copy engine has read and written all boxes
     if (MODE != TN && a.fill) {
       const int first = s.table.bounds[0], last = s.table.bounds[a.off.groups];
@@ -374,6 +386,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     }
   }
 
+  if (F::AFTER && (warp < 2 || warp == FIX_WARP)) {
+    __syncwarp();
+    cluster_sync_all();
+  }
   // Nobody leaves while the pair still reads this CTA's shared memory or signals its barriers; the parts of a split tile are in their inboxes
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncwarp();
@@ -453,9 +469,9 @@ int launch_shape(Shape shape, int in_type, int out_type, const CUtensorMap& p, c
 }
 
 // How tn is done: by pairs, by single CTAs, or by clusters that share the reduction of a tile of 64 or 128 columns, whichever takes the shortest time where all
-// groups have the same rows.  In ns, fitted to the measurements: a stage of a cluster's CTA takes 1.6 for every line of 128 bytes (all SMs load), of a single CTA 0.9,
-// or 72 for each of its loads where these are more; to send and add up the parts takes 800 and 28 for every column.  us without and with clusters: one group of 8192
-// rows, 1024 x 1024: 50 and 34; of 65536 rows, 256 x 512: 357 and 52; three of 15399 rows, 1144 x 128: 42.5 and 19.5; 8 of 4096 rows, 128 x 256: 7.0 and 8.2, so
+// groups have the same rows.  In ns, fitted to the measurements: a stage of a cluster's CTA takes 1.6 for every line of 128 bytes (all SMs load), 1.3 with 128 columns,
+// of a single CTA 0.9, or 72 for each of its loads where these are more; to send and add up the parts takes 2600 or 4900.  us without and with clusters: one group of 8192
+// rows, 1024 x 1024: 50 and 28.6; of 65536 rows, 256 x 512: 357 and 45; three of 15399 rows, 1144 x 128: 42.5 and 16.4; 8 of 4096 rows, 128 x 256: 7.0 and 8.2, so
 // not taken.
 struct TnPlan {
   bool pair;
@@ -472,7 +488,7 @@ TnPlan tn_plan(long long rows, int groups, int N, int K, bool wide) {
   long long least = steps * max(9 * (LANES + width(MAX_COLS)) / 10, 72 * loads);
   for (const int cols : {FEW_COLS, SOME_COLS}) {
     const int parts = parts_of((long long)groups * blocks(cols) * ((K + LANES - 1) / LANES), (int)steps);
-    const long long t = (steps + parts - 1) / parts * 16 * (LANES + width(cols)) / 10 + 800 + 28 * cols;
+    const long long t = (steps + parts - 1) / parts * (cols == FEW_COLS ? 16 : 13) * (LANES + width(cols)) / 10 + (cols == FEW_COLS ? 2600 : 4900);
     if (parts > 1 && t < least) {
       least = t;
       plan = {false, parts, cols};
