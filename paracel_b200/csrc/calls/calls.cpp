@@ -219,8 +219,10 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   uint8_t* data = static_cast<uint8_t*>(buf.data_ptr());
   uint8_t* scales = data + data_bytes(rows, K);
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  // a contiguous stack has rows of K values one behind the other, whatever a dimension of one index reports as its stride
+  const int64_t ldx = d == 2 ? X.stride(0) : K;
   PyObject* t = launched("pcl_mx4_quantize", [&] {
-    return quantize_fn(X.data_ptr(), X.stride(d - 2), type_of(X.scalar_type()), data, scales, rows, (int)K, stream);
+    return quantize_fn(X.data_ptr(), ldx, type_of(X.scalar_type()), data, scales, rows, (int)K, stream);
   }, buf);
   if (t == nullptr) return nullptr;
   return Py_BuildValue("(NiLLKK)", t, device, (long long)rows, (long long)K, (unsigned long long)(uintptr_t)data,

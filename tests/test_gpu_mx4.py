@@ -115,6 +115,26 @@ def test_quantising_strided_rows_and_stacks():
     assert mx4_dequantize(mx4_quantize(torch.empty(0, 40, device="cuda"))).shape == (0, 40)
 
 
+@pytest.mark.parametrize("dtype", [F, BF])
+@pytest.mark.parametrize("E,N,K", [(5, 1, 64), (9, 1, 100), (300, 1, 1056), (1, 7, 96), (6, 5, 1), (4, 1, 1), (1, 1, 40)])
+def test_stacks_with_a_dimension_of_one(E, N, K, dtype):
+    """Such a dimension may report any stride, and the stack still counts as contiguous: rows lie K values apart all the same."""
+    from paracel_b200.ops.mx4 import mx4_dequantize, mx4_grouped_nt, mx4_quantize
+    big = _rows(max(E, N) * E * N, K, dtype)              # as far as any of these strides would lead
+    w = big[:E * N].view(N, E, K).transpose(0, 1) if N == 1 else big[:E * N].view(E, N, K)
+    odd = big.as_strided((E, N, K), (K * N, K if N > 1 else K * E, 1 if K > 1 else 7))
+    want = _define(big[:E * N])
+    for x in (w, odd, odd.clone()):
+        assert x.shape == (E, N, K) and x.is_contiguous()
+        q = mx4_quantize(x)
+        assert q.rows == E * N and q.cols == K
+        _same(mx4_dequantize(q), want)
+        _same(mx4_dequantize(mx4_quantize(x[:, 0])), _define(x[:, 0]))
+    A, kept = _grid(E, K, 3), _grid(big.shape[0], K, 4)
+    got = mx4_grouped_nt(A, mx4_quantize(kept.as_strided(odd.shape, odd.stride())), torch.arange(E + 1, device="cuda"))
+    assert torch.equal(got.double(), torch.stack([A[e].double() @ kept[e * N:(e + 1) * N].double().T for e in range(E)]))
+
+
 def _near(got, a, b):
     """got against a @ b.T of the values that the four bits stand for."""
     a, b = a.double(), b.double()
