@@ -535,3 +535,21 @@ def test_odd_widths_into_given_results_on_a_stream_and_in_a_graph():
         off.copy_(_offsets([7, 100, 0, 33] if seed == 2 else [0, 0, 140, 0]))
         graph.replay()
         right(made)
+
+
+@pytest.mark.parametrize("E,N,K", [(5, 1, 64), (9, 1, 33), (1, 7, 24), (6, 5, 1), (4, 1, 1)])
+def test_matrices_and_rows_with_a_dimension_of_one(E, N, K):
+    """Such a dimension may report any stride: it is not looked at."""
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt, grouped_tn
+    T = 3 * E
+    X, dY, flat = _whole(T, 1, N, K, BF)[0], _whole(T, 1, N, K, BF)[1], _whole(1, max(E, N) * E, N, K, BF)[2].view(-1)
+    W = flat.as_strided((E, N, K), (N * K, K if N > 1 else K * E, 1 if K > 1 else 7))
+    one = X.as_strided((1, K), (5, 1))
+    off, f = _offsets([3] * E), torch.float32
+    y, z, d = (torch.empty(s, device="cuda") for s in ((T, N), (T, K), (E, N, K)))
+    grouped_nt(X, W, off, out=y), grouped_nn(dY, W, off, out=z), grouped_tn(dY, X, off, out=d)
+    for got, given, ref in ((grouped_nt(X, W, off, out_dtype=f), y, _ref_rows(X, W, off)[0]),
+                            (grouped_nn(dY, W, off, out_dtype=f), z, _ref_rows(dY, W.transpose(1, 2), off)[0]),
+                            (grouped_tn(dY, X, off, out_dtype=f), d, _ref_tn(dY, X, off)[0])):
+        assert torch.equal(got.double(), ref) and torch.equal(given, got)
+    assert torch.equal(grouped_nt(one, W, _offsets([1] + [0] * (E - 1)), out_dtype=f).double(), X[:1].double() @ W[0].double().T)
