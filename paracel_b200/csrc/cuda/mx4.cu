@@ -682,12 +682,14 @@ template <int COLS, bool SPLIT, bool FUSED, class TO>
 int launch(const CUtensorMap& p, const CUtensorMap& q, const CUtensorMap& qs, const CUtensorMap& o, const Args& a, int parts, cudaStream_t stream) {
   auto kernel = product_kernel<COLS, SPLIT, FUSED, TO>;
   constexpr int fixed = Form<COLS, SPLIT, FUSED>::SMEM_BYTES + (int)sizeof(Shared);
-  static_assert(fixed + (FUSED ? FUSED_MOST : 0) <= 227 * 1024, "shared memory of an SM");
+  // The limit belongs to the function, not to the launch: it is the same in every call, since another thread's call may come between the two
+  constexpr int limit = fixed + (FUSED ? FUSED_MOST : 0);
+  static_assert(limit <= 227 * 1024, "shared memory of an SM");
   const int smem = fixed + (FUSED ? a.room : 0);
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
   if (e != cudaSuccess) return (int)e;
   const long long mb = (a.N + LANES - 1) / LANES;
   const long long chunks = most_chunks(a.off.rows, a.off.groups, COLS);

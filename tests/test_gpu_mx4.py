@@ -374,3 +374,33 @@ def test_experts_trained_in_16_bits_answer_from_four():
             assert torch.equal(s[r], ref)          # the groups' products are the plain product's, row for row
             _near(out[r], s4[r], w2[e])
             _near(mx4_grouped_nt(X, q1, off, out_dtype=F)[r], x4[r], w1[e])
+
+
+def test_two_threads_with_rows_of_different_lengths():
+    """Few rows are quantised by the product's own blocks, whose shared memory goes with the rows' length: calls of one thread do not change what
+    another's may take.  The launcher is called directly, so that the threads are in it nearly all the time."""
+    import threading
+    from paracel_b200.ops import _lib
+    from paracel_b200.ops.mx4 import check_status, mx4_quantize
+    lib, N, start, wrong, kept = _lib.load(), 1000, threading.Barrier(4), [], []
+
+    def serve(i, K):
+        A, B, out, stream = _grid(1, K, i), _grid(N, K, 9 + i), torch.empty(1, N, device="cuda"), torch.cuda.Stream()
+        q = mx4_quantize(B)
+        kept.append((A, B, q, out))
+        args = (A.data_ptr(), K, 0, None, None, q.data.data_ptr(), q.scales.data_ptr(), None, 0, out.data_ptr(), N, 0, 1, 1, N, K, 1, stream.cuda_stream)
+        torch.cuda.synchronize()
+        start.wait()
+        wrong.extend(filter(None, (lib.pcl_mx4_rows(*args) for _ in range(30000))))
+
+    assert all(lib.pcl_mx4_room(0, 1, 1, N, K) == 0 for K in (100, 1792))         # both are of that kind
+    threads = [threading.Thread(target=serve, args=a) for a in enumerate((100, 1792, 100, 1792))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    check_status()
+    assert not wrong
+    for A, B, _, out in kept:
+        assert torch.equal(out.double(), A.double() @ B.double().T)
