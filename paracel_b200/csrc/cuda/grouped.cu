@@ -305,19 +305,22 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   } else if (MODE == TN && warp == FIX_WARP) {
     int stage = 0;
     uint32_t phases = 0;   // bit i: parity of the next wait on tail[i]
+    long long since = 0;   // stages since the last wait: tiles without a tail are passed over at once, and the next tail comes behind all of theirs
     for (Turn i(walk, group, groups); i.has() && ok; i.next()) {
       const Tile w = i.tile();
       const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
       const int last = (stage + steps + STAGES - 1) % STAGES;
       stage = (stage + steps) % STAGES;
+      since += steps;
       if (len % BR == 0) continue;
-      if (!wait_full(s.tail + last, (phases >> last) & 1u, abort_flag, tile_ns(steps))) {
+      if (!wait_full(s.tail + last, (phases >> last) & 1u, abort_flag, tile_ns(since))) {
         if (lane == 0) report(&g_status, 0, 45, last, 0);
         abort_all<CG>(abort_flag, me ^ 1u);
         ok = false;
         break;
       }
       phases ^= 1u << last;
+      since = 0;
       // the products stop at the next multiple of 16 steps
       uint8_t* st = stages + last * STAGE_BYTES;
       const int left = len % BR, upto = (left + 15) & ~15;

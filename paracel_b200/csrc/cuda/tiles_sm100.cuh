@@ -117,8 +117,8 @@ __device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, volati
     }
   }
 }
-// What a tile of `steps` stages may take beyond the usual limit (a stage takes a fraction of a microsecond; a reduction over 2^31 rows has 2^25)
-__device__ __forceinline__ unsigned long long tile_ns(int steps) { return 2000ull * (unsigned)steps; }
+// What `steps` stages may take beyond the usual limit (a stage takes a fraction of a microsecond; a reduction over 2^31 rows has 2^25)
+__device__ __forceinline__ unsigned long long tile_ns(long long steps) { return 2000ull * (unsigned long long)steps; }
 
 // arrive on a barrier given by its cluster address, after this CTA's writes to its shared memory
 __device__ __forceinline__ void arrive_cluster(uint32_t cluster_addr) {

@@ -553,3 +553,20 @@ def test_matrices_and_rows_with_a_dimension_of_one(E, N, K):
                             (grouped_tn(dY, X, off, out_dtype=f), d, _ref_tn(dY, X, off)[0])):
         assert torch.equal(got.double(), ref) and torch.equal(given, got)
     assert torch.equal(grouped_nt(one, W, _offsets([1] + [0] * (E - 1)), out_dtype=f).double(), X[:1].double() @ W[0].double().T)
+
+
+def test_a_tail_behind_seconds_of_other_tiles():
+    """A group of whole stages takes some 2.5 s before the first tile of a group with an odd number of rows: the warp that waits for such an end passes over
+    the tiles without one at once, and its limit (2 s, and 2 us a stage) counts theirs.  Rows that overlap (8 values apart) keep the operands small; sums
+    of -1, 0 and 1 over 7.3 million rows are exact in fp32."""
+    from paracel_b200.ops.grouped import check_status, grouped_tn
+    first, last, N, K = 64 * 114688, 37, 16384, 16384
+    T = first + last
+    g = torch.Generator(device="cuda").manual_seed(5)
+    X, dY = (torch.randint(-1, 2, (8 * T + K,), device="cuda", generator=g, dtype=torch.int8).to(BF).as_strided((T, K), (8, 1)) for _ in range(2))
+    off = torch.tensor([0, first, T], device="cuda")
+    d = grouped_tn(dY, X, off, out_dtype=torch.float32)
+    check_status()
+    n, k = (torch.randint(0, K, (12,), device="cuda", generator=g) for _ in range(2))
+    assert torch.equal(d[0][n][:, k].double(), dY[:first, n].double().T @ X[:first, k].double())
+    assert torch.equal(d[1].double(), dY[first:].double().T @ X[first:].double())
