@@ -141,23 +141,40 @@ def calls_path() -> Path:
     return LIB / ("_pcl_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
+def _calls_stamp() -> str:
+    """Of the source, the flags and torch, whose C++ interface the module is bound to; not of where the tree lies."""
+    import torch
+
+    src = CSRC / "calls" / "calls.cpp"
+    return hashlib.sha1(" ".join(CXX_FLAGS).encode() + torch.__version__.encode() + src.read_bytes()).hexdigest()
+
+
+def calls_current() -> bool:
+    """Whether the built module is of this source and of the torch that runs."""
+    stamp_file = LIB / "calls.stamp"
+    return calls_path().exists() and stamp_file.exists() and stamp_file.read_text() == _calls_stamp()
+
+
 def build_calls(force=False, verbose=False) -> Path:
     import torch
 
     LIB.mkdir(exist_ok=True)
     src = CSRC / "calls" / "calls.cpp"
     out = calls_path()
-    st = _stamp([src], " ".join(CXX_FLAGS) + torch.__version__)
-    stamp_file = LIB / "calls.stamp"
-    if not force and out.exists() and stamp_file.exists() and stamp_file.read_text() == st:
+    if not force and calls_current():
         return out
     root = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parent.parent
-    _run(["g++", *CXX_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", root / "include",
-          "-isystem", root / "include" / "torch" / "csrc" / "api" / "include", "-isystem", cuda / "include",
-          "-isystem", sysconfig.get_paths()["include"], "-shared", "-o", out, src, "-L", root / "lib",
-          "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"], verbose)
-    stamp_file.write_text(st)
+    made = out.with_name(f"{out.name}.{os.getpid()}")      # ranks that build at once do not load each other's halves
+    try:
+        _run(["g++", *CXX_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", root / "include",
+              "-isystem", root / "include" / "torch" / "csrc" / "api" / "include", "-isystem", cuda / "include",
+              "-isystem", sysconfig.get_paths()["include"], "-shared", "-o", made, src, "-L", root / "lib",
+              "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"], verbose)
+        os.replace(made, out)
+    finally:
+        made.unlink(missing_ok=True)
+    (LIB / "calls.stamp").write_text(_calls_stamp())
     return out
 
 
