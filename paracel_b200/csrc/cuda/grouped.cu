@@ -30,6 +30,8 @@ using namespace pcl_tiles;
 
 __device__ PclStatus g_status;
 
+__global__ void take_kernel(PclStatus* to) { take(&g_status, to); }
+
 constexpr int NT = 0, NN = 1, TN = 2;
 constexpr int BR = 64;                         // reduction steps of a stage
 constexpr int LANES = 128;
@@ -193,7 +195,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       const uint32_t q_bytes = whole ? (uint32_t)Q_BYTES : MODE == TN ? boxes * 8192u : boxes * (uint32_t)(F::SMALL_BOX * BR * 2);
       for (int kb = 0; kb < steps; ++kb) {
         if (!mbar_wait(s.empty + stage, phase ^ 1, abort_flag)) {
-          if (lane == 0) report(&g_status, 0, 41, kb, stage);
+          if (lane == 0) post(&g_status, CODE_WAIT, 41, kb, stage);
           abort_all<CG>(abort_flag, me ^ 1u);
           ok = false;
           break;
@@ -266,7 +268,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
         if (len <= 0) continue;
         if (!mbar_wait(s.tempty + acc, (acc_phase >> acc & 1u) ^ 1u, abort_flag)) {
-          if (lane == 0) report(&g_status, 0, 42, acc, 0);
+          if (lane == 0) post(&g_status, CODE_WAIT, 42, acc, 0);
           abort_all<CG>(abort_flag, me ^ 1u);
           ok = false;
           break;
@@ -277,7 +279,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         const uint32_t d = tmem + (uint32_t)(acc * COLS);
         for (int r = 0; r < steps; ++r) {
           if (!ready && !wait_full(s.full + stage, phase, abort_flag)) {
-            if (lane == 0) report(&g_status, 0, 43, r, stage);
+            if (lane == 0) post(&g_status, CODE_WAIT, 43, r, stage);
             abort_all<CG>(abort_flag, me ^ 1u);
             ok = false;
             break;
@@ -314,7 +316,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       since += steps;
       if (len % BR == 0) continue;
       if (!wait_full(s.tail + last, (phases >> last) & 1u, abort_flag, tile_ns(since))) {
-        if (lane == 0) report(&g_status, 0, 45, last, 0);
+        if (lane == 0) post(&g_status, CODE_WAIT, 45, last, 0);
         abort_all<CG>(abort_flag, me ^ 1u);
         ok = false;
         break;
@@ -355,7 +357,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         continue;
       }
       if (!wait_full(s.tfull + acc, acc_phase >> acc & 1u, abort_flag, tile_ns((w.r1 - w.r0) / BR))) {
-        if (lane == 0) report(&g_status, 0, 44, acc, 0);
+        if (lane == 0) post(&g_status, CODE_WAIT, 44, acc, 0);
         abort_all<CG>(abort_flag, me ^ 1u);
         ok = false;
         break;
@@ -674,13 +676,8 @@ PCL_API int pcl_grouped_tn(int in_type, int out_type, const void* Y, long long l
   return launch_shape<TN>(plan.pair ? PAIR : MANY, in_type, out_type, p, q, q, o, a, stream);
 }
 
-// Copies the status block of the grouped products to `host` and clears it (waits for the stream).
-PCL_API int pcl_grouped_status(PclStatus* host, cudaStream_t stream) {
-  cudaError_t e = cudaMemcpyFromSymbolAsync(host, g_status, sizeof(PclStatus), 0, cudaMemcpyDeviceToHost, stream);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-  if (e != cudaSuccess || host->code == 0) return (int)e;
-  const PclStatus none{};
-  e = cudaMemcpyToSymbolAsync(g_status, &none, sizeof(none), 0, cudaMemcpyHostToDevice, stream);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-  return (int)e;
+// Moves the report that the status block of the grouped products holds, if any, to `to` in the device's memory, behind what the stream has so far.
+PCL_API int pcl_grouped_status(PclStatus* to, cudaStream_t stream) {
+  take_kernel<<<1, 1, 0, stream>>>(to);
+  return pcl_last_error();
 }

@@ -326,6 +326,8 @@ struct Shared {
 
 __device__ PclStatus g_status;
 
+__global__ void take_kernel(PclStatus* to) { take(&g_status, to); }
+
 // a block of 32 rows x 16 bytes without swizzle: eight rows are 128 bytes in one piece
 __device__ __forceinline__ uint64_t desc_scales(uint32_t saddr) {
   return ((uint64_t)(8u | (1u << 14)) << 32) | ((saddr >> 4) & 0x3FFFu) | (8u << 16);
@@ -500,7 +502,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
   using Turn = Tiles<Walk<SPLIT>, SPLIT || FUSED>;
   bool ok = true;
   auto gave_up = [&](int where, int x, int y) {
-    if (lane == 0) report(&g_status, 0, where, x, y);
+    if (lane == 0) post(&g_status, CODE_WAIT, where, x, y);
     *abort_flag = 1;
     ok = false;
   };
@@ -840,13 +842,8 @@ PCL_API int pcl_mx4_rows(const void* x, long long ldx, int x_type, void* A, void
   return plan.parts > 1 ? launch_as<FEW_COLS, true, false>(out_type, p, q, qs, o, a, plan.parts, stream) : launch_as<FEW_COLS, false, false>(out_type, p, q, qs, o, a, 1, stream);
 }
 
-// Copies the status block of these products to `host` and clears it (waits for the stream).
-PCL_API int pcl_mx4_status(PclStatus* host, cudaStream_t stream) {
-  cudaError_t e = cudaMemcpyFromSymbolAsync(host, g_status, sizeof(PclStatus), 0, cudaMemcpyDeviceToHost, stream);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-  if (e != cudaSuccess || host->code == 0) return (int)e;
-  const PclStatus none{};
-  e = cudaMemcpyToSymbolAsync(g_status, &none, sizeof(none), 0, cudaMemcpyHostToDevice, stream);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-  return (int)e;
+// Moves the report that the status block of these products holds, if any, to `to` in the device's memory, behind what the stream has so far.
+PCL_API int pcl_mx4_status(PclStatus* to, cudaStream_t stream) {
+  take_kernel<<<1, 1, 0, stream>>>(to);
+  return pcl_last_error();
 }

@@ -25,7 +25,7 @@ struct Table {
   // holds, so that no row is in two groups; the first one that had to be moved goes into the status block.
   __device__ __forceinline__ void build(int groups, int most, PclStatus* st) {
     const int lane = threadIdx.x;
-    int top = bounds[0], carry = 0;
+    int top = bounds[0], carry = 0, moved = -1, from = 0;
     for (int i0 = 0; i0 < groups; i0 += 32) {
       const int i = i0 + lane + 1;
       const int own = i <= groups ? bounds[i] : 0;
@@ -40,7 +40,10 @@ struct Table {
       top = __shfl_sync(0xffffffffu, v, 31);
       if (i <= groups) {
         bounds[i] = v;
-        if (v != own) pcl_report_bad_id(st, 0, 110, i, own);
+        if (v != own && moved < 0) {
+          moved = i;
+          from = own;
+        }
       }
       const int parts = i <= groups ? (v - before + most - 1) / most : 0;
       int sum = parts;
@@ -53,6 +56,7 @@ struct Table {
       carry += __shfl_sync(0xffffffffu, sum, 31);
     }
     if (lane == 0) chunks[groups] = carry;
+    if (moved >= 0) pcl_group::post(st, pcl_group::CODE_BOUNDS, 110, moved, from);
   }
 
   // `step` divides `most`: a chunk is then at most `most` rows, and all but the last of a group's chunks cannot hold all its rows.

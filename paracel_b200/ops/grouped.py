@@ -32,15 +32,19 @@ MAX_ROWS = (1 << 31) - 512
 
 def check_status(device=None) -> None:
     """Raise if a grouped product on ``device`` met bounds that it had to move, or gave up on a wait (synchronises the
-    current stream)."""
+    current stream).
+
+    The device keeps one report for all streams and threads, the first since it was last asked: it is raised once, to whoever asks first.  What runs on
+    other streams counts once it has run, and what a graph's replay reports as well."""
     read_status("pcl_grouped_status", device, "grouped product")
 
 
 def read_status(entry: str, device, what: str) -> None:
     index = None if device is None else torch.device(device).index
-    host = torch.zeros(4, dtype=torch.int64)
-    _lib.call_on(torch.cuda.current_device() if index is None else index, entry, host.data_ptr())
-    _lib.raise_status(host, what)
+    index = torch.cuda.current_device() if index is None else index
+    status = torch.empty(4, dtype=torch.int64, device=f"cuda:{index}")
+    _lib.call_on(index, entry, status.data_ptr())
+    _lib.raise_status(status.cpu(), what)
 
 
 def check_operand(t: torch.Tensor, name: str, dims: int, dtype=None) -> None:

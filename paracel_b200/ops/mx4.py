@@ -98,7 +98,7 @@ class Mx4Matrix:
 
 def check_status(device=None) -> None:
     """Raise if a grouped four-bit product on ``device`` met bounds that it had to move, or one of these products gave up on
-    a wait (synchronises the current stream)."""
+    a wait (synchronises the current stream; one report for all streams and threads, as ``ops.grouped.check_status`` says)."""
     read_status("pcl_mx4_status", device, "four-bit product")
 
 

@@ -570,3 +570,45 @@ def test_a_tail_behind_seconds_of_other_tiles():
     n, k = (torch.randint(0, K, (12,), device="cuda", generator=g) for _ in range(2))
     assert torch.equal(d[0][n][:, k].double(), dY[:first, n].double().T @ X[:first, k].double())
     assert torch.equal(d[1].double(), dY[first:].double().T @ X[first:].double())
+
+
+@pytest.mark.parametrize("four_bits", [False, True])
+def test_a_report_is_taken_whole_and_once(four_bits):
+    """Three threads ask on streams of their own while calls report one at a time: every report reaches one of them, and none two."""
+    import threading
+    import time
+    from paracel_b200.ops import grouped, mx4
+    from paracel_b200.ops._lib import BadDeviceId
+    X, W, off = torch.ones(2, 16, device="cuda", dtype=BF), torch.ones(1, 16, 16, device="cuda", dtype=BF), torch.tensor([0, 5], device="cuda")
+    q = mx4.mx4_quantize(W)
+    call, check = ((lambda: mx4.mx4_grouped_nt(X, q, off)), mx4.check_status) if four_bits else ((lambda: grouped.grouped_nt(X, W, off)), grouped.check_status)
+    raised, odd, stop = [], [], threading.Event()
+
+    def ask():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                while not stop.is_set():
+                    try:
+                        check()
+                    except BadDeviceId as e:
+                        raised.append((e.position, e.bad_id))
+        except Exception as e:
+            odd.append(e)
+
+    threads = [threading.Thread(target=ask) for _ in range(3)]
+    for t in threads:
+        t.start()
+    try:
+        for n in range(1, 201):
+            call()                                       # one block, in which one thread meets the bound
+            torch.cuda.current_stream().synchronize()
+            until = time.monotonic() + 20
+            while len(raised) < n and not odd and time.monotonic() < until:
+                time.sleep(0.0005)
+            time.sleep(0.002)                            # room for another to have it too
+    finally:
+        stop.set()
+        for t in threads:
+            t.join()
+    assert not odd and raised == [(1, 5)] * 200
+    check()
