@@ -361,7 +361,7 @@ __device__ __forceinline__ void zero_part(TO* dst, long long n, int part, int pa
 
 // A warp's part of an accumulator goes to out: column j of [0, n) and the warp's 32 lanes to dst[j * ldo + lane], lanes < `lanes` only.  Columns 32 at a time,
 // first + 0, 64, 128 ..  16-bit results turn around in shared memory (stmatrix) and leave as boxes of 32 rows
-// x 64 bytes, where `boxed` says that the map can take them, or by words of eight or four bytes; what is left of a chunk, and rows that begin anywhere, are stored lane by lane, a row's 32
+// x 64 bytes, where `boxed` says that the map can take them, or by words of eight or four bytes (the last lanes of rows whose length is no multiple of 16 bytes always); what is left of a chunk, and rows that begin anywhere, are stored lane by lane, a row's 32
 // neighbours at a time (stored so throughout, nt of 16 groups of 1024 rows, 2048 x 1024 took 81 instead of 68 us: a store of one row takes an SM 11 cycles, of
 // 64 bytes or of 128).
 template <class TO>
@@ -370,6 +370,8 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, int first, int n, 
   const int lane = threadIdx.x & 31;
   const uint32_t bits = (uint32_t)(uintptr_t)dst | (uint32_t)ldo * 2u;
   const int word = (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : 2;   // bytes
+  // The copy engine writes 16 bytes whole, those behind a map's last column among them, which in a strided result are someone else's
+  boxed = boxed && (lanes >= 32 || (lanes & 7) == 0);
   for (int c = first; c < n; c += 64) {
     if (sizeof(TO) == 2 && (boxed || word > 2) && c + 32 <= n) {
       uint32_t lo[16], hi[16];

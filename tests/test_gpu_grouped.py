@@ -612,3 +612,28 @@ def test_a_report_is_taken_whole_and_once(four_bits):
             t.join()
     assert not odd and raised == [(1, 5)] * 200
     check()
+
+
+@pytest.mark.parametrize("cols", [1, 3, 7, 8, 9, 15, 19, 30, 31, 33, 37, 130, 291, 1999])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_columns_beside_a_given_result_stay(cols, dtype):
+    """Rows at multiples of 16 bytes whose length is none: nothing is written behind a row's last value, nor before its first."""
+    from paracel_b200.ops.grouped import grouped_nn, grouped_nt
+    from paracel_b200.ops.mx4 import mx4_dequantize, mx4_gemm_nt, mx4_grouped_nt, mx4_quantize
+    R = 24
+    for counts in ([70, 0, 33], [5, 0, 64], [1500, 600, 700]):
+        T, E = sum(counts) + 3, len(counts)
+        X, _, W = _whole(T, E, cols, R, dtype)
+        off, q = _offsets(counts), mx4_quantize(W)
+        ref, n = _ref_rows(X, W, off)[0], T - 3
+        x4 = mx4_dequantize(mx4_quantize(X)).double()
+        ref4 = torch.cat([x4[a:b] @ mx4_dequantize(q)[e * cols:(e + 1) * cols].double().T for e, (a, b) in enumerate(zip(off.tolist(), off.tolist()[1:]))])
+        calls = [(lambda o: grouped_nt(X, W, off, out=o), ref), (lambda o: grouped_nn(X, W.transpose(1, 2).contiguous(), off, out=o), ref),
+                 (lambda o: mx4_grouped_nt(X, q, off, out=o), ref4), (lambda o: mx4_gemm_nt(X[:n], mx4_quantize(W[0]), out=o[:n]), x4[:n] @ mx4_dequantize(q)[:cols].double().T)]
+        for before, behind in ((0, 0), (0, 8), (8, 0), (8, 16)):
+            for call, want in calls:
+                wide = torch.full((T, before + (cols + 7) // 8 * 8 + behind), -7.0, device="cuda", dtype=dtype)
+                call(wide[:, before:before + cols])
+                full = torch.full_like(wide, -7.0)
+                full[:n, before:before + cols] = want[:n]
+                assert torch.equal(wide, full)
