@@ -425,7 +425,8 @@ gemm_tf32_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     constexpr int HC = TN / 2;                // columns per epilogue warp
     float* stg = reinterpret_cast<float*>(sE + (warp - 2) * 4096);
     const uint32_t tempty_leader0 = map_to_cta(smem_u32(tempty), 0);
-    const bool vec_ok = ((a.ldc & 3) == 0) && ((((uintptr_t)a.C) & 15) == 0);
+    // (the copy engine writes whole 16 bytes: with another N it would write behind the rows of a C that lies in longer ones)
+    const bool vec_ok = (((a.ldc | a.N) & 3) == 0) && ((((uintptr_t)a.C) & 15) == 0);
     int acc = 0;
     uint32_t acc_phase[2] = {0, 0};
     bool ok = true;
@@ -620,9 +621,9 @@ PCL_API int pcl_gemm_tf32_2sm(const float* A, float* b_stage, float* C, int M, i
   if (rc) return rc;
   rc = make_map2(&tmB, b_stage, N, K, HN, BK);
   if (rc) return rc;
-  // bulk tensor stores need a 16-byte aligned base and row stride; otherwise (and for the arg-min
+  // bulk tensor stores need a 16-byte aligned base and row stride, and rows of whole 16 bytes; otherwise (and for the arg-min
   // epilogue) the map is a stand-in over A that the kernel never uses
-  const bool c_ok = (epi == 0) && ((ldc & 3) == 0) && ((((uintptr_t)C) & 15) == 0);
+  const bool c_ok = (epi == 0) && (((ldc | N) & 3) == 0) && ((((uintptr_t)C) & 15) == 0);
   rc = c_ok ? make_map_c(&tmC, C, M, N, ldc) : make_map2(&tmC, A, M, K, HM, BK);
   if (rc) return rc;
   Gemm2Args a;

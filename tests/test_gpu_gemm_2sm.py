@@ -72,3 +72,19 @@ def test_dense_read_gemm_2sm_single_rank(wide):
     ref = _ref(A, op.shard)
     assert (C - ref).abs().max().item() / ref.abs().max().item() < 5e-3
     op.free()
+
+
+@pytest.mark.parametrize("wide", [0, 1])
+@pytest.mark.parametrize("N", [1, 2, 3, 5, 31, 33, 127, 130, 255, 519])
+def test_columns_beside_a_strided_output_stay(N, wide):
+    """Rows at multiples of 16 bytes whose length is none: nothing is written beside them.  Whole numbers: the products are exact."""
+    from paracel_b200.ops.gemm import check_status, gemm_nt
+    g = torch.Generator(device="cuda").manual_seed(12)
+    A, B = (torch.randint(-4, 5, (r, 64), device="cuda", generator=g).float() for r in (300, N))
+    for before, behind in ((0, 0), (0, 4), (4, 8)):
+        big = torch.full((300, before + (N + 3) // 4 * 4 + behind), -7.0, device="cuda")
+        gemm_nt(A, B, out=big[:, before:before + N], kernel="2sm", wide=wide)
+        check_status()
+        want = torch.full_like(big, -7.0)
+        want[:, before:before + N] = A @ B.T
+        assert torch.equal(big, want)
