@@ -383,7 +383,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the copy engine has read and written all boxes
     if (MODE != TN && a.fill) {
       const int first = s.table.bounds[0], last = s.table.bounds[a.off.groups];
-      const int rows = first + a.off.rows - last;
+      const int rows = first + (a.off.rows - last);
       for (long long q = (long long)blockIdx.x * EPI_WARPS + warp - 2; q < rows; q += (long long)gridDim.x * EPI_WARPS) {
         TO* row = out + (q < first ? q : q - first + last) * a.ldo;
         for (int c = lane; c < a.mdim; c += 32) row[c] = to_out<TO>(0.f);

@@ -16,6 +16,18 @@ using namespace pcl_sm100;
 constexpr int MAX_COLS = 256;   // columns of an accumulator
 constexpr int SMS = 148;        // that the rules for a call's shape count on
 
+// Rows of a chunk where `rows` are cut into `parts` chunks, as equal as multiples of `step` allow.  (Not (rows + parts - 1) / parts: that leaves 32 bits from 2.11e9 rows on.)
+__host__ __device__ constexpr int chunk_size(int rows, int parts, int step) { return ((rows - 1) / parts + 1 + step - 1) / step * step; }
+
+constexpr int MOST_ROWS = (int)((1ll << 31) - 513);   // of a call
+__host__ __device__ constexpr int chunks_of(int rows, int most) { return (rows + most - 1) / most; }
+constexpr bool cut_right(int rows, int most, int step) {
+  const int parts = chunks_of(rows, most), size = chunk_size(rows, parts, step);
+  return size > 0 && size <= most && (long long)size * parts >= rows && (long long)size * (parts - 1) < rows;
+}
+static_assert(cut_right(MOST_ROWS, 64, 16) && cut_right(MOST_ROWS, 128, 16) && cut_right(MOST_ROWS, 208, 16) && cut_right(MOST_ROWS, 256, 32), "as many rows as a call takes");
+static_assert(cut_right(MOST_ROWS - 1601, 64, 16) && cut_right(2114537830, 64, 16) && cut_right(1, 64, 16) && cut_right(65, 64, 16) && cut_right(257, 256, 32), "and others");
+
 // The rows of a group are cut into chunks of at most MAX_COLS, as equal as multiples of `step` allow.
 struct Table {
   int bounds[pcl_group::MAX_GROUPS + 1];
@@ -45,7 +57,7 @@ struct Table {
           from = own;
         }
       }
-      const int parts = i <= groups ? (v - before + most - 1) / most : 0;
+      const int parts = i <= groups ? chunks_of(v - before, most) : 0;
       int sum = parts;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -70,7 +82,7 @@ struct Table {
       else hi = mid;
     }
     const int rows = bounds[e + 1] - bounds[e], parts = chunks[e + 1] - chunks[e];
-    const int size = ((rows + parts - 1) / parts + step - 1) / step * step;
+    const int size = chunk_size(rows, parts, step);
     begin = bounds[e] + (c - chunks[e]) * size;
     n = min(size, bounds[e + 1] - begin);
   }

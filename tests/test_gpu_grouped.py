@@ -637,3 +637,34 @@ def test_columns_beside_a_given_result_stay(cols, dtype):
                 full = torch.full_like(wide, -7.0)
                 full[:n, before:before + cols] = want[:n]
                 assert torch.equal(wide, full)
+
+
+def test_as_many_rows_as_a_call_takes():
+    """2^31 - 513 rows, nearly all of one group, its bounds included; rows are zero but for three windows, and whole numbers."""
+    from paracel_b200.ops.grouped import MAX_ROWS, check_status, grouped_nn, grouped_nt, grouped_tn
+    T, C = MAX_ROWS - 1, 8
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("not enough memory")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    bounds = [0, 100, T - 1501, T]
+    off = torch.tensor(bounds, device="cuda")
+    X, W = torch.zeros(T, C, device="cuda", dtype=BF), torch.randint(-3, 4, (3, C, C), device="cuda", generator=g).to(BF)
+    windows = [(a, a + 3000) for a in (0, T // 2, T - 3000)]
+    for a, b in windows:
+        X[a:b] = torch.randint(-3, 4, (b - a, C), device="cuda", generator=g).to(BF)
+    parts = [(max(a, lo), min(b, hi), e) for a, b in windows for e, (lo, hi) in enumerate(zip(bounds, bounds[1:])) if max(a, lo) < min(b, hi)]
+    for call, M in ((grouped_nt, W.transpose(1, 2)), (grouped_nn, W)):
+        y = call(X, W, off)
+        check_status()
+        for a, b, e in parts:
+            assert torch.equal(y[a:b].double(), X[a:b].double() @ M[e].double())
+        del y
+    d = grouped_tn(X, X, off, out_dtype=torch.float32)
+    check_status()
+    want = torch.zeros(3, C, C, device="cuda", dtype=torch.float64)
+    for a, b, e in parts:
+        want[e] += X[a:b].double().T @ X[a:b].double()
+    assert torch.equal(d.double(), want)
+    del X
+    torch.cuda.empty_cache()

@@ -404,3 +404,35 @@ def test_two_threads_with_rows_of_different_lengths():
     assert not wrong
     for A, B, _, out in kept:
         assert torch.equal(out.double(), A.double() @ B.double().T)
+
+
+def test_as_many_rows_as_a_call_takes():
+    """2^31 - 513 rows against a few: quantised, multiplied by one and given back, the same values at both ends and in the middle."""
+    from paracel_b200.ops.grouped import MAX_ROWS
+    from paracel_b200.ops.mx4 import check_status, mx4_dequantize, mx4_gemm_nt, mx4_grouped_nt, mx4_quantize
+    T, C = MAX_ROWS - 1, 8
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip("not enough memory")
+    X = torch.zeros(T, C, device="cuda", dtype=BF)
+    windows = [slice(a, a + 3000) for a in (0, T // 2, T - 3000)]
+    for i, w in enumerate(windows):
+        X[w] = _grid(3000, C, i).to(BF)
+    q = mx4_quantize(X)
+    kept = [X[w].clone() for w in windows]
+    del X
+    torch.cuda.empty_cache()
+    B = torch.stack((torch.eye(C, device="cuda"), 2 * torch.eye(C, device="cuda").flip(0)))
+    off = torch.tensor([0, T - 1501, T], device="cuda")
+    for make, factor in ((lambda: mx4_gemm_nt(q, mx4_quantize(B[0]), out_dtype=BF), None), (lambda: mx4_grouped_nt(q, mx4_quantize(B), off, out_dtype=BF), off),
+                         (lambda: mx4_dequantize(q, BF), None)):
+        y = make()
+        check_status()
+        for w, x in zip(windows, kept):
+            want = x.clone()
+            if factor is not None and w.stop == T:
+                want[-1501:] = 2 * x[-1501:].flip(1)
+            assert torch.equal(y[w], want)
+        del y
+    del q
+    torch.cuda.empty_cache()
