@@ -267,41 +267,50 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         const Tile w = i.tile();
         const int len = w.r1 - w.r0, steps = (len + BR - 1) / BR;
         if (len <= 0) continue;
-        if (!mbar_wait(s.tempty + acc, (acc_phase >> acc & 1u) ^ 1u, abort_flag)) {
-          if (lane == 0) post(&g_status, CODE_WAIT, 42, acc, 0);
-          abort_all<CG>(abort_flag, me ^ 1u);
-          ok = false;
-          break;
-        }
-        acc_phase ^= 1u << acc;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t idesc = idesc0 | ((uint32_t)(w.ncol >> 3) << 17);
         const uint32_t d = tmem + (uint32_t)(acc * COLS);
-        for (int r = 0; r < steps; ++r) {
-          if (!ready && !wait_full(s.full + stage, phase, abort_flag)) {
-            if (lane == 0) post(&g_status, CODE_WAIT, 43, r, stage);
-            abort_all<CG>(abort_flag, me ^ 1u);
-            ok = false;
-            break;
-          }
-          const int next = stage + 1 == STAGES ? 0 : stage + 1;
-          ready = has_passed(s.full + next, phase ^ (uint32_t)(next == 0));
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (elect()) {
-            const uint64_t dp = dp0 + (uint32_t)(stage * STAGE_BYTES) / 16, dq = dq0 + (uint32_t)(stage * STAGE_BYTES) / 16;
-            if (r * BR + BR <= len) {
-#pragma unroll
-              for (int k = 0; k < BR / 16; ++k) umma_f16<CG>(d, dp + k * STEP_P, dq + k * STEP_Q, idesc, (r > 0 || k > 0) ? 1u : 0u);
-            } else {
-              for (int k = 0; r * BR + 16 * k < len; ++k) umma_f16<CG>(d, dp + k * STEP_P, dq + k * STEP_Q, idesc, (r > 0 || k > 0) ? 1u : 0u);
+        // Parts of LONG stages: each waits until the one before it has been added up.  The sum is in the other accumulator, which counts as used from the second part on (the
+        // warps that store take it up in turn behind the tile that was there) until it is stored; the next tile does not wait for that, but takes this accumulator.
+        for (int begin = 0; begin < steps && ok; begin += LONG) {
+          for (int b = acc;; b = acc ^ 1) {
+            if (!mbar_wait(s.tempty + b, (acc_phase >> b & 1u) ^ 1u, abort_flag)) {
+              if (lane == 0) post(&g_status, CODE_WAIT, 42, b, 0);
+              abort_all<CG>(abort_flag, me ^ 1u);
+              ok = false;
+              break;
             }
-            commit<CG>(smem_u32(s.empty + stage));
-            if (r + 1 == steps) commit<CG>(smem_u32(s.tfull + acc));
+            acc_phase ^= 1u << b;
+            if (b != acc || begin != LONG) break;
           }
-          __syncwarp();
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const int end = min(steps, begin + LONG);
+          for (int r = begin; r < end; ++r) {
+            if (!ready && !wait_full(s.full + stage, phase, abort_flag)) {
+              if (lane == 0) post(&g_status, CODE_WAIT, 43, r, stage);
+              abort_all<CG>(abort_flag, me ^ 1u);
+              ok = false;
+              break;
+            }
+            const int next = stage + 1 == STAGES ? 0 : stage + 1;
+            ready = has_passed(s.full + next, phase ^ (uint32_t)(next == 0));
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect()) {
+              const uint64_t dp = dp0 + (uint32_t)(stage * STAGE_BYTES) / 16, dq = dq0 + (uint32_t)(stage * STAGE_BYTES) / 16;
+              if (r * BR + BR <= len) {
+#pragma unroll
+                for (int k = 0; k < BR / 16; ++k) umma_f16<CG>(d, dp + k * STEP_P, dq + k * STEP_Q, idesc, (r > begin || k > 0) ? 1u : 0u);
+              } else {
+                for (int k = 0; r * BR + 16 * k < len; ++k) umma_f16<CG>(d, dp + k * STEP_P, dq + k * STEP_Q, idesc, (r > begin || k > 0) ? 1u : 0u);
+              }
+              commit<CG>(smem_u32(s.empty + stage));
+              if (r + 1 == end) commit<CG>(smem_u32(s.tfull + acc));
+            }
+            __syncwarp();
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
         }
-        acc ^= 1;
+        if (steps <= LONG) acc ^= 1;
       }
     }
   } else if (MODE == TN && warp == FIX_WARP) {
@@ -356,15 +365,28 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
         zero_part(out + ((long long)w.e * a.jdim + w.j0) * a.ldo, (long long)w.n * a.ldo, w.m0 / LANES + (int)me, walk.mb * CG, (int)threadIdx.x - 64, 32 * EPI_WARPS);
         continue;
       }
-      if (!wait_full(s.tfull + acc, acc_phase >> acc & 1u, abort_flag, tile_ns((w.r1 - w.r0) / BR))) {
-        if (lane == 0) post(&g_status, CODE_WAIT, 44, acc, 0);
-        abort_all<CG>(abort_flag, me ^ 1u);
-        ok = false;
-        break;
+      const int steps = (w.r1 - w.r0 + BR - 1) / BR;
+      const uint32_t lanes0 = tmem + ((uint32_t)(sub * 32) << 16), part0 = lanes0 + (uint32_t)(acc * COLS), sum0 = lanes0 + (uint32_t)((acc ^ 1) * COLS);
+      for (int done = LONG;; done += LONG) {   // stages, parts of them
+        if (!wait_full(s.tfull + acc, acc_phase >> acc & 1u, abort_flag, tile_ns(LONG))) {
+          if (lane == 0) post(&g_status, CODE_WAIT, 44, acc, 0);
+          abort_all<CG>(abort_flag, me ^ 1u);
+          ok = false;
+          break;
+        }
+        acc_phase ^= 1u << acc;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (steps <= LONG) break;
+        __syncwarp();
+        add_part(part0, sum0, half * 32, w.n, done == LONG);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
+        if (done >= steps) break;
       }
-      acc_phase ^= 1u << acc;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t t0 = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(acc * COLS);
+      if (!ok) break;
+      const int from = steps <= LONG ? acc : acc ^ 1;   // accumulator to store
+      const uint32_t t0 = steps <= LONG ? part0 : sum0;
       if (SPLIT) {   // the cluster has this one tile
         __syncwarp();
         if (F::AFTER) cluster_sync_all();
@@ -375,8 +397,8 @@ product_kernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__
       store_columns<TO>(t0, half * 32, w.n, dst, a.ldo, a.mdim - m, a.boxed, pieces + (warp - 2) * PIECE_BYTES, &mapOut, m, w.j0, MODE == TN ? w.e : 0);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + acc), 0) : smem_u32(s.tempty + acc));
-      acc ^= 1;
+      if (lane == 0) mbar_arrive_cluster(CG == 2 ? map_to_cta(smem_u32(s.tempty + from), 0) : smem_u32(s.tempty + from));
+      if (steps <= LONG) acc ^= 1;
     }
     __syncwarp();
     if (F::AFTER && !free) cluster_sync_all();

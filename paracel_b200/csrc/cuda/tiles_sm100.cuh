@@ -321,6 +321,59 @@ static __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
                : "memory");
 }
 
+// The tensor cores cut off what they add to an accumulator, always towards zero, so that its error grows with the number of additions: a sum of a million terms of one sign
+// lost 0.7 % in one accumulator (1.2e-3 where signs differ).  A reduction of more stages than LONG is therefore done in parts of LONG stages, and the
+// parts are added up in fp32, rounded, by the warps that store: the error stays that of 8192 terms (9e-6, 3.5e-5 of one sign).  The tensor cores wait meanwhile: 0 to 2.5 % of such a call
+// (one group of 65536 rows, 4096 x 4096: 1503 us in one accumulator, 1534 so; with parts of 64 stages, and the next tile behind the sum's store, 1580).
+constexpr int LONG = 128;
+
+// 16 columns of the warp's 32 lanes, from and to tensor memory; loaded registers are read behind a wait that names them
+static __device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+static __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// The warp's columns (32 of every 64 from `first` on, up to n) of the accumulator `part` begin those of `sum`, or are added to them.
+static __device__ __noinline__ void add_part(uint32_t part, uint32_t sum, int first, int n, bool begin) {
+#pragma unroll 1
+  for (int c = first; c < n; c += ((c & 31) == 16 ? 48 : 16)) {
+    uint32_t v[16];
+    tmem_ld16_issue(part + (uint32_t)c, v);
+    if (begin) {
+      asm volatile("tcgen05.wait::ld.sync.aligned;"
+                   : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                     "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                   :
+                   : "memory");
+      tmem_st16(sum + (uint32_t)c, v);
+    } else {
+      uint32_t u[16];
+      tmem_ld16_issue(sum + (uint32_t)c, u);
+      asm volatile("tcgen05.wait::ld.sync.aligned;"
+                   : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                     "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]),
+                     "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]),
+                     "+r"(u[14]), "+r"(u[15])
+                   :
+                   : "memory");
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u[j]));
+      tmem_st16(sum + (uint32_t)c, v);
+    }
+  }
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
 // n columns lane by lane, a row's 32 neighbours at a time: short code, for the few columns of short calls
 template <class TO>
 __device__ __forceinline__ void store_singly(uint32_t taddr, int n, TO* dst, long long ldo, int lanes) {

@@ -668,3 +668,49 @@ def test_as_many_rows_as_a_call_takes():
     assert torch.equal(d.double(), want)
     del X
     torch.cuda.empty_cache()
+
+
+def _one_sign(shape, g):
+    return torch.rand(shape, device="cuda", generator=g).to(BF)
+
+
+@pytest.mark.parametrize("T,N,K,which", [(6000, 512, 300_001, "nt"), (300, 64, 1_000_000, "nt"), (6000, 262_144, 512, "nn"), (262_144, 2560, 2560, "tn"),
+                                         (262_144, 4096, 4096, "tn"), (1_000_003, 200, 264, "tn"), (3_000_000, 128, 64, "tn")])
+def test_the_error_of_long_sums_does_not_grow(T, N, K, which):
+    """Sums of hundreds of thousands of terms of one sign, the worst case of additions that cut off: a part of at most 8192 terms is off by 8192 2^-23 of its own
+    sum, as at the head of this file, and adding P parts up by P 2^-24 of the whole, rounded."""
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt, grouped_tn
+    g = torch.Generator(device="cuda").manual_seed(7)
+    f = torch.float32
+    if which == "tn":
+        X, dY, off = _one_sign((T, K), g), _one_sign((T, N), g), torch.tensor([0, T], device="cuda")
+        got, R = grouped_tn(dY, X, off, out_dtype=f)[0][:64, :64], T
+        ref = dY[:, :64].double().T @ X[:, :64].double()
+    else:
+        A, W, off = _one_sign((T, K if which == "nt" else N), g), _one_sign((1, N, K), g), torch.tensor([0, T], device="cuda")
+        got, R = (grouped_nt if which == "nt" else grouped_nn)(A, W, off, out_dtype=f)[-64:, :64], A.shape[1]
+        M = W[0, :64].T if which == "nt" else W[0, :, :64]
+        ref = A[-64:].double() @ M.double()
+    check_status()
+    parts = -(-R // 8192) + 8                            # and a last one for each of eight CTAs
+    worst = float(((got.double() - ref).abs() / ref).max())
+    assert worst <= 8192 * 2.0 ** -23 + parts * 2.0 ** -24, worst
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("counts,N,K", [([8192], 64, 8192), ([8193, 0, 8256], 72, 8257), ([40_000, 3, 0, 9000], 136, 20_000), ([9000] * 4, 8200, 264),
+                                        ([8200] * 9, 1000, 16_448), ([140_000], 1030, 520), ([100, 30_000, 64 * 129], 520, 1048),
+                                        # pairs of CTAs with several tiles each: short, long, long, short, empty
+                                        ([64, 9000, 20_000, 100, 0, 8300, 5, 5, 16_385] * 2, 1536, 1280), ([9000, 17, 200, 8300] * 9, 1030, 1001)])
+def test_long_reductions_of_whole_numbers_are_exact(counts, N, K, dtype):
+    """Reductions in several parts and in one next to each other, in every direction and shape of tiles."""
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt, grouped_tn
+    T, E = sum(counts), len(counts)
+    X, dY, W = _whole(T, E, N, K, dtype)
+    off, f = _offsets(counts), torch.float32
+    for od in (f, dtype):
+        y, z, d = grouped_nt(X, W, off, out_dtype=od), grouped_nn(dY, W, off, out_dtype=od), grouped_tn(dY, X, off, out_dtype=od)
+        check_status()
+        assert torch.equal(y, _ref_rows(X, W, off)[0].to(f).to(od))
+        assert torch.equal(z, _ref_rows(dY, W.transpose(1, 2), off)[0].to(f).to(od))
+        assert torch.equal(d, _ref_tn(dY, X, off)[0].to(f).to(od))
