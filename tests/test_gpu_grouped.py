@@ -714,3 +714,29 @@ def test_long_reductions_of_whole_numbers_are_exact(counts, N, K, dtype):
         assert torch.equal(y, _ref_rows(X, W, off)[0].to(f).to(od))
         assert torch.equal(z, _ref_rows(dY, W.transpose(1, 2), off)[0].to(f).to(od))
         assert torch.equal(d, _ref_tn(dY, X, off)[0].to(f).to(od))
+
+
+@pytest.mark.parametrize("bounds", [[0, 0, 3, 3, 40], [5, 4, 9, 9, 2], [0, 1, 2, 3, 4], [7, 7, 7, 7, 7], [-3, 2, -1, 50, 60]])
+@pytest.mark.parametrize("N,K", [(45, 37), (48, 40)])
+def test_moved_bounds_and_no_others_are_reported_as_such(bounds, N, K):
+    """By every product, with operands that are copied first and with others: the place and the number of a bound that had to be moved."""
+    from paracel_b200.ops import mx4
+    from paracel_b200.ops._lib import BadDeviceId
+    from paracel_b200.ops.grouped import check_status, grouped_nn, grouped_nt, grouped_tn
+    T = 40
+    X, dY, W = _whole(T, 4, N, K, BF)
+    off, q = torch.tensor(bounds, device="cuda"), mx4.mx4_quantize(W)
+    moved, top = {}, 0
+    for i, v in enumerate(bounds):
+        top = max(top, min(max(v, 0), T))
+        if v != top:
+            moved[i] = {v, min(max(v, 0), T)}            # as given, or as cut to the rows before it is made ascending
+    for call, check in ((lambda: grouped_nt(X, W, off), check_status), (lambda: grouped_nn(dY, W, off), check_status), (lambda: grouped_tn(dY, X, off), check_status),
+                        (lambda: mx4.mx4_grouped_nt(X, q, off), mx4.check_status)):
+        check()
+        call()
+        if moved:
+            with pytest.raises(BadDeviceId) as e:
+                check()
+            assert e.value.position in moved and e.value.bad_id in moved[e.value.position]
+        check()
