@@ -382,7 +382,7 @@ def test_two_threads_with_rows_of_different_lengths():
     import threading
     from paracel_b200.ops import _lib
     from paracel_b200.ops.mx4 import check_status, mx4_quantize
-    lib, N, start, wrong, kept = _lib.load(), 1000, threading.Barrier(4), [], []
+    lib, N, start, wrong, kept = _lib.load(), 1000, threading.Barrier(4, timeout=60), [], []
 
     def serve(i, K):
         A, B, out, stream = _grid(1, K, i), _grid(N, K, 9 + i), torch.empty(1, N, device="cuda"), torch.cuda.Stream()
@@ -401,7 +401,7 @@ def test_two_threads_with_rows_of_different_lengths():
         t.join()
     torch.cuda.synchronize()
     check_status()
-    assert not wrong
+    assert not wrong and len(kept) == 4
     for A, B, _, out in kept:
         assert torch.equal(out.double(), A.double() @ B.double().T)
 
