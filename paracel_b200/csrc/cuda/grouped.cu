@@ -17,9 +17,9 @@
 //   warp 10    of tn: clears what a group's last stage holds of the next group
 // Where tiles are few a cluster of CTAs shares a tile's reduction and adds it up through each other's shared memory.
 //
-// Measured on one B200: nt, 32 groups of together 32768 rows, 4096 x 2048: 463 us = 1190 TFLOP/s in a stream of calls, at the power cap (cuBLAS, 32 equal
-// groups: 436 us), 1500 TFLOP/s for a call alone; there the products take 16,384 of the 16,280 to 17,000 cycles from tile to tile.  nn and tn of 16 groups, 16384 rows,
-// 2048 x 1024: 67 and 77 us.  Small calls are bound by latency, 3.4 us for the smallest, or by the weights: 16 rows of 32 groups, 1536 x 1024, read 38 MB in
+// Measured on one B200: nt, 32 groups of together 32768 rows, 4096 x 2048: 463 to 502 us by the chip = 1095 to 1190 TFLOP/s in a stream of calls, at the power cap (cuBLAS, 32 equal
+// groups: 439 to 450 us, these here 441 to 452), 385 us = 1430 TFLOP/s for a call after a pause; a trace has 16,280 to 17,000 cycles from tile to tile, nominally 16,384 for its
+// products.  nn and tn of 16 groups, 16384 rows, 2048 x 1024: 64 to 69 and 70 to 77 us.  Small calls are bound by latency, 3.4 us for the smallest, or by the weights: 16 rows of 32 groups, 1536 x 1024, read 38 MB in
 // 10.9 us where they fall to 12 of these, in 9.2 out of the L2.
 #include "tiles_sm100.cuh"
 
@@ -50,7 +50,7 @@ struct Form {
   static constexpr int Q_BYTES = COLS / CG * BR * 2;
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
   // A cluster's 128 columns: the parts are sent to where the operands were, behind a barrier of the cluster more; three stages beside them left the loads waiting
-  // (one group of 131072 rows, 512 x 512: 135 and 113 us)
+  // (one group of 131072 rows, 512 x 512: 135 and 113 us; 114 to 118 with its sums in parts)
   static constexpr bool AFTER = SPLIT && COLS == 128;
   static constexpr int STAGES = (OPERAND_BYTES - (SPLIT && !AFTER ? inbox_bytes(COLS) : 0)) / STAGE_BYTES;
   static_assert(!AFTER || inbox_bytes(COLS) <= OPERAND_BYTES, "room for the parts");

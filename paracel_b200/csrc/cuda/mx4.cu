@@ -264,8 +264,8 @@ __global__ void __launch_bounds__(QTHREADS) dequantize_kernel(DequantArgs a) {
 // and 1000 cycles go by per stage, 270 us for 8192^3.)
 // Roles in a CTA: warp 0 loads operands, warp 1 issues products, warps 2-9 store, warps 10-12 fetch scales.
 //
-// Measured: 8192^3 in 261 us = 4.2 PFLOP/s (nominal peak 9), 32 groups of together 16384 rows x 4096 x 2048 in 100 us, with A from bf16 290 and 117; one row
-// against 8192 x 4096 10.2 us.  Bound by the tensor pipe: a stage takes 600 cycles of it, 416 for the products of 208 columns and 30 for each of the six
+// Measured, in streams of calls: 8192^3 of packed matrices in 261 to 269 us = 4.1 to 4.2 PFLOP/s (nominal peak 9), 32 groups of together 16384 rows x 4096 x 2048 in 100 to 103 us,
+// with A from bf16, its quantisation included, 311 to 328 and 120 to 125; one row from bf16 against 8192 x 4096 8.5 to 8.9 us.  Bound by the tensor pipe: a stage takes 600 cycles of it, 416 for the products of 208 columns and 30 for each of the six
 // copies of scales; by the bytes that an SM takes in (45 KB a stage) where a reduction is short; by latency, about 4 us, for the smallest.  Pairs of
 // CTAs, which load less, took 283 us: the leader has to be told of the other's scales.
 constexpr int LANES = 128;
@@ -781,7 +781,7 @@ struct Plan {
 };
 
 // Tiles of the number of rows that takes the shortest time; and whether A, of x_type, is quantised by the product's own CTAs: where each has one tile at most, and the words
-// of its rows go through its warps in one pass (QUANT_WARPS * 4 of them).  One row against 8192 x 4096 takes 9.3 us so, 10.2 with a kernel for the quantisation,
+// of its rows go through its warps in one pass (QUANT_WARPS * 4 of them).  One row against 8192 x 4096 takes 8.5 us so, 9.6 with a kernel for the quantisation,
 // most of it the second launch; 64 rows of 8 words a CTA 20 us, and 8.
 static Plan plan_of(int x_type, long long rows, int groups, int N, int K) {
   Plan plan{0, 1, 0, 0, false};
